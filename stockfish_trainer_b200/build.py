@@ -1,12 +1,14 @@
-"""Build the native library in-tree: ``stockfish_trainer_b200/libnnue_ft.so``.
+"""Build the native libraries in-tree: ``stockfish_trainer_b200/libnnue_ft.so``
+(the feature transformer) and ``libnnue_ls.so`` (the layer stacks).
 
     python -m stockfish_trainer_b200.build [--force] [--verbose]
 
-One nvcc invocation compiles the CUDA kernels for sm_100a (nnue_ft.cu) and the
+For libnnue_ft.so one nvcc invocation compiles the CUDA kernels for sm_100a (nnue_ft.cu) and the
 host-side position / feature-index code (features.cpp) into a single shared
 library with a plain C ABI (include/nnue_ft.h).  ``-fmad=false`` keeps every
 fp32 operation a separately rounded IEEE op, which the bit-exact parity with
-the reference relies on.
+the reference relies on.  libnnue_ls.so (csrc/layer_stacks/, include/nnue_ls.h)
+is compiled without it: its sums are not tied to a reference order.
 """
 
 from __future__ import annotations
@@ -37,23 +39,24 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found (set NVCC or put CUDA's bin directory on PATH)")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+LS_CSRC = os.path.join(CSRC, "layer_stacks")
+LS_LIB_PATH = os.path.join(PKG, "libnnue_ls.so")
+
+
+def _stale(lib: str, deps: list[str]) -> bool:
+    if not os.path.exists(lib):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(CSRC, d) for d in DEPS] + [os.path.join(INCLUDE, "nnue_ft.h")]
+    t = os.path.getmtime(lib)
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not _stale():
-        return LIB_PATH
-    tmp = LIB_PATH + ".tmp"
+def _compile(lib: str, sources: list[str], flags: list[str], verbose: bool) -> str:
+    tmp = lib + ".tmp"
     cmd = [
-        nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-fmad=false",
+        nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", *flags,
         "-Xcompiler", "-fPIC,-O3,-pthread", "-shared",
         "-I", INCLUDE,
-        *(os.path.join(CSRC, s) for s in SOURCES),
+        *sources,
         "-o", tmp, "-lpthread",
     ]
     if verbose:
@@ -63,9 +66,24 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
     if verbose:
         sys.stderr.write(res.stderr)
-    os.replace(tmp, LIB_PATH)
-    return LIB_PATH
+    os.replace(tmp, lib)
+    return lib
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    deps = [os.path.join(CSRC, d) for d in DEPS] + [os.path.join(INCLUDE, "nnue_ft.h")]
+    if not force and not _stale(LIB_PATH, deps):
+        return LIB_PATH
+    return _compile(LIB_PATH, [os.path.join(CSRC, s) for s in SOURCES], ["-fmad=false"], verbose)
+
+
+def build_layer_stacks(force: bool = False, verbose: bool = False) -> str:
+    deps = [os.path.join(LS_CSRC, d) for d in sorted(os.listdir(LS_CSRC)) if d.endswith((".cu", ".cuh"))]
+    if not force and not _stale(LS_LIB_PATH, deps + [os.path.join(INCLUDE, "nnue_ls.h")]):
+        return LS_LIB_PATH
+    return _compile(LS_LIB_PATH, [os.path.join(LS_CSRC, "nnue_ls.cu")], [], verbose)
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    for fn in (build, build_layer_stacks):
+        print(fn(force="--force" in sys.argv, verbose="--verbose" in sys.argv))

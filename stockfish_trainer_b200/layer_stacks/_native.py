@@ -1,0 +1,176 @@
+"""ctypes binding of ``libnnue_ls.so`` (C ABI declared in include/nnue_ls.h).
+
+Built in-tree by ``stockfish_trainer_b200.build``.  There is no fallback: if
+the library cannot be loaded every entry point raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import os
+import threading
+
+import torch
+
+from .. import build as _build
+from .._native import NativeError
+
+_P, _I64, _I32, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
+_U64, _SZ = ctypes.c_uint64, ctypes.c_size_t
+
+OK = 0
+ERR_INVALID_ARGUMENT = -1
+ERR_UNSUPPORTED = -2
+ERR_WORKSPACE = -3
+ERR_CUDA = -4
+DEVERR_WAIT_TIMEOUT = 1
+DEVERR_BAD_INDEX = 2
+NORM_MAX_WIDTH = 65536
+MAX_EXPERTS = 1024
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class Linear(ctypes.Structure):
+    _fields_ = [("rows", _I64), ("inputs", _I64), ("outputs", _I64), ("dtype", _I32), ("bias_dtype", _I32),
+                ("activation", _I32), ("reserved", _I32), ("x", _P), ("weight", _P), ("bias", _P), ("residual", _P),
+                ("ldx", _I64), ("ldw", _I64), ("ldr", _I64), ("out", _P), ("act_grad", _P), ("grad_out", _P),
+                ("ldg", _I64), ("grad_x", _P), ("grad_weight", _P), ("grad_bias", _P)]
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [("rows", _I64), ("width", _I32), ("dtype", _I32), ("params_dtype", _I32), ("gate_dtype", _I32),
+                ("kind", _I32), ("gate_mode", _I32), ("gate_sigmoid", _I32), ("scale_value", _F), ("eps", _F),
+                ("reserved", _I32), ("x", _P), ("f", _P), ("gate", _P), ("post_weight", _P), ("post_bias", _P),
+                ("scale", _P), ("pre_weight", _P), ("pre_bias", _P), ("y", _P), ("h", _P), ("stats", _P),
+                ("grad_y", _P), ("grad_h", _P), ("grad_x", _P), ("grad_f", _P), ("grad_gate", _P),
+                ("grad_post_weight", _P), ("grad_post_bias", _P), ("grad_scale", _P), ("grad_pre_weight", _P),
+                ("grad_pre_bias", _P)]
+
+
+class Route(ctypes.Structure):
+    _fields_ = [("rows", _I64), ("experts", _I32), ("k", _I32), ("dtype", _I32), ("renormalize", _I32),
+                ("logits", _P), ("ld", _I64), ("valid", _P), ("indices", _P), ("gates", _P), ("counts", _P),
+                ("loss", _P), ("grad_gates", _P), ("grad_loss", _P), ("grad_logits", _P)]
+
+
+_SIGNATURES = {
+    "nnue_ls_version": (_I32, []),
+    "nnue_ls_last_error": (ctypes.c_char_p, []),
+    "nnue_ls_launch_count": (_U64, []),
+    "nnue_ls_device_errors": (_I32, [ctypes.POINTER(ctypes.c_uint32), _I32]),
+    "nnue_ls_linear_forward_workspace_size": (_SZ, [ctypes.POINTER(Linear)]),
+    "nnue_ls_linear_forward": (_I32, [ctypes.POINTER(Linear), _P, _SZ, _P]),
+    "nnue_ls_linear_backward_workspace_size": (_SZ, [ctypes.POINTER(Linear)]),
+    "nnue_ls_linear_backward": (_I32, [ctypes.POINTER(Linear), _P, _SZ, _P]),
+    "nnue_ls_norm_forward": (_I32, [ctypes.POINTER(Norm), _P]),
+    "nnue_ls_norm_backward_workspace_size": (_SZ, [ctypes.POINTER(Norm)]),
+    "nnue_ls_norm_backward": (_I32, [ctypes.POINTER(Norm), _P, _SZ, _P]),
+    "nnue_ls_route_forward_workspace_size": (_SZ, [ctypes.POINTER(Route)]),
+    "nnue_ls_route_forward": (_I32, [ctypes.POINTER(Route), _P, _SZ, _P]),
+    "nnue_ls_route_backward": (_I32, [ctypes.POINTER(Route), _P]),
+}
+
+_lib = None
+_lock = threading.Lock()
+
+
+def load(build_if_missing: bool | None = None) -> ctypes.CDLL:
+    """Load (building first if allowed and needed) the native library."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    with _lock:
+        if _lib is not None:
+            return _lib
+        if build_if_missing is None:
+            build_if_missing = os.environ.get("NNUE_FT_NO_BUILD", "0") != "1"
+        path = _build.build_layer_stacks() if build_if_missing else _build.LS_LIB_PATH
+        if not os.path.exists(path):
+            raise ImportError(
+                f"{path} is missing: build it with `python -m stockfish_trainer_b200.build` "
+                "(there is no non-native implementation of this path)")
+        L = ctypes.CDLL(path)
+        for name, (res, args) in _SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype = res
+            fn.argtypes = args
+        _lib = L
+    return _lib
+
+
+def exported_symbols() -> list[str]:
+    return list(_SIGNATURES)
+
+
+def last_error() -> str:
+    msg = load().nnue_ls_last_error()
+    return msg.decode() if msg else ""
+
+
+def launch_count() -> int:
+    """Kernels launched by the library so far (process-wide)."""
+    return int(load().nnue_ls_launch_count())
+
+
+def device_errors(clear: bool = True) -> int:
+    """Sticky device error flags of the current device (synchronises)."""
+    flags = ctypes.c_uint32(0)
+    check("nnue_ls_device_errors", load().nnue_ls_device_errors(ctypes.byref(flags), int(clear)))
+    return int(flags.value)
+
+
+def check(func: str, rc: int) -> None:
+    if rc != OK:
+        raise NativeError(func, rc, last_error())
+
+
+def run(func: str, args: ctypes.Structure, device: torch.device, sized: bool = True) -> None:
+    """Enqueue ``func(args)`` on the device's current stream; with ``sized`` the
+    call takes a workspace, allocated here from PyTorch's caching allocator."""
+    lib = _lib or load()
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return run(func, args, device, sized)
+    ref = ctypes.byref(args)
+    stream = torch.cuda.current_stream().cuda_stream
+    if not sized:
+        return check(func, getattr(lib, func)(ref, stream))
+    nbytes = getattr(lib, func + "_workspace_size")(ref)
+    if nbytes == 0:
+        return check(func, getattr(lib, func)(ref, None, 0, stream))
+    # the caching allocator returns 512-byte aligned blocks; the ABI needs 256
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    check(func, getattr(lib, func)(ref, ws.data_ptr(), nbytes, stream))
+
+
+def ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def check_tensor(t: torch.Tensor, name: str, device: torch.device | None = None, dtypes=tuple(DTYPES)) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as a matrix of its last dimension's rows, with unit column stride
+    and rows that do not overlap; copied only where the layout asks for it."""
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if (m.stride(1) != 1 and m.shape[1] > 1) or (m.stride(0) < m.shape[1] and m.shape[0] > 1):
+        m = m.contiguous()
+    return m
+
+
+def row_stride(m: torch.Tensor) -> int:
+    return max(m.stride(0), m.shape[1])
+
+
+def needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

@@ -1,0 +1,127 @@
+"""Linear layer with bias, activation and residual in the product's epilogue.
+
+The layers of the reference's stacks are separate torch calls: a product with
+bias, a (squared) clamp to [0, 1], and a skip term added at the end
+(src/model/modules/layer_stacks.py:15-68, stacked_linear.py:14-65).
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+ACTIVATIONS = ("none", "relu", "crelu", "sqr_crelu", "silu", "gelu")
+_ACT = {name: i for i, name in enumerate(ACTIVATIONS)}
+
+
+def _args(x, weight, bias, residual, act):
+    a = _native.Linear()
+    a.rows, a.inputs = x.shape
+    a.outputs = weight.shape[0]
+    a.dtype = _native.DTYPES[x.dtype]
+    a.bias_dtype = a.dtype if bias is None else _native.DTYPES[bias.dtype]
+    a.activation = act
+    a.x, a.ldx = x.data_ptr(), _native.row_stride(x)
+    a.weight, a.ldw = weight.data_ptr(), _native.row_stride(weight)
+    if bias is not None:
+        a.bias = bias.data_ptr()
+    if residual is not None:
+        a.residual, a.ldr = residual.data_ptr(), _native.row_stride(residual)
+    return a
+
+
+def _forward(x, weight, bias, residual, act, want_act_grad):
+    a = _args(x, weight, bias, residual, act)
+    out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
+    a.out = out.data_ptr()
+    act_grad = None
+    if want_act_grad and act:
+        act_grad = torch.empty_like(out)
+        a.act_grad = act_grad.data_ptr()
+    _native.run("nnue_ls_linear_forward", a, x.device)
+    return out, act_grad
+
+
+class LinearActFunction(torch.autograd.Function):
+    """All matrices 2-D with unit column stride; bias contiguous."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        out, act_grad = _forward(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, bias, act_grad)
+        ctx.act = act
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, weight, bias, act_grad = ctx.saved_tensors
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        grad_x = grad_w = grad_b = None
+        if need_x or need_w or need_b:
+            g = _native.rows_of(grad_out)
+            a = _args(x, weight, bias, None, ctx.act)
+            a.grad_out, a.ldg = g.data_ptr(), _native.row_stride(g)
+            a.act_grad = _native.ptr(act_grad)
+            if need_x:
+                grad_x = torch.empty(a.rows, a.inputs, dtype=x.dtype, device=x.device)
+                a.grad_x = grad_x.data_ptr()
+            if need_w:
+                grad_w = torch.empty(a.outputs, a.inputs, dtype=x.dtype, device=x.device)
+                a.grad_weight = grad_w.data_ptr()
+            if need_b:
+                grad_b = torch.empty_like(bias)
+                a.grad_bias = grad_b.data_ptr()
+            _native.run("nnue_ls_linear_backward", a, x.device)
+        return grad_x, grad_w, grad_b, grad_out if need_r else None, None
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+               residual: torch.Tensor | None = None, activation: str = "none") -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``.
+
+    ``x`` is ``[..., inputs]`` and ``weight`` ``[outputs, inputs]``, both fp32,
+    bf16 or fp16 (one type for both and for ``residual``; ``bias``
+    ``[outputs]`` may also be fp32).  ``residual`` has the output's shape
+    ``[..., outputs]`` or broadcasts to it.  ``activation`` is one of
+    ``ACTIVATIONS``: ``crelu`` clamps to [0, 1] and ``sqr_crelu`` squares the
+    result; ``gelu`` is the exact form.  Sums are held in fp32 and the result
+    is rounded once; fp32 products are accurate to fp32 rounding, but a
+    non-finite fp32 operand may turn an infinite sum into NaN.  Rows may be
+    strided; other layouts are copied.
+
+    The backward keeps ``x``, ``weight`` and the activation's derivative (in
+    the output's type); it is differentiable once.
+    """
+    _native.check_tensor(x, "x")
+    dev, dt = x.device, x.dtype
+    _native.check_tensor(weight, "weight", dev, (dt,))
+    if activation not in _ACT:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    n = weight.shape[0]
+    if n < 1 or weight.shape[1] < 1:
+        raise ValueError("weight must not be empty")
+    shape = x.shape[:-1] + (n,)
+    if bias is not None:
+        _native.check_tensor(bias, "bias", dev, (dt,) if dt == torch.float32 else (dt, torch.float32))
+        if bias.dim() != 1 or bias.shape[0] != n:
+            raise ValueError(f"bias must have shape ({n},), got {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    if residual is not None:
+        _native.check_tensor(residual, "residual", dev, (dt,))
+        if residual.shape != shape:
+            try:
+                residual = residual.expand(shape)
+            except RuntimeError:
+                raise ValueError(f"residual {tuple(residual.shape)} does not broadcast to {tuple(shape)}") from None
+        residual = _native.rows_of(residual)
+    x, weight = _native.rows_of(x), _native.rows_of(weight)
+    if _native.needs_grad(x, weight, bias, residual):
+        out = LinearActFunction.apply(x, weight, bias, residual, _ACT[activation])
+    else:
+        out = _forward(x, weight, bias, residual, _ACT[activation], False)[0]
+    return out if len(shape) == 2 else out.view(shape)

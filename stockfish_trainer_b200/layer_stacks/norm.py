@@ -1,0 +1,164 @@
+"""Norms before and after a residual block, fused with the block's gate and
+residual scale, as one kernel each way."""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_KINDS = {"rms": 0, "layer": 1}
+_PARAMS = ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")
+
+
+def _args(x, f, gate, params, meta):
+    a = _native.Norm()
+    a.rows, a.width = x.shape
+    a.dtype = _native.DTYPES[x.dtype]
+    a.params_dtype = a.gate_dtype = a.dtype
+    a.kind, a.gate_mode, a.gate_sigmoid, a.scale_value, a.eps = meta
+    a.x = x.data_ptr()
+    if f is not None:
+        a.f = f.data_ptr()
+    if gate is not None:
+        a.gate, a.gate_dtype = gate.data_ptr(), _native.DTYPES[gate.dtype]
+    for name, t in zip(_PARAMS, params):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+            a.params_dtype = _native.DTYPES[t.dtype]
+    return a
+
+
+def _forward(x, f, gate, params, meta, want_stats):
+    a = _args(x, f, gate, params, meta)
+    y = h = stats = None
+    if f is not None:
+        y = torch.empty_like(x)
+        a.y = y.data_ptr()
+    if params[3] is not None:
+        h = torch.empty_like(x)
+        a.h = h.data_ptr()
+    if want_stats:
+        stats = torch.empty(x.shape[0], 4, dtype=torch.float32, device=x.device)
+        a.stats = stats.data_ptr()
+    _native.run("nnue_ls_norm_forward", a, x.device, sized=False)
+    return y, h, stats
+
+
+class BlockNormFunction(torch.autograd.Function):
+    """Returns (y, h); without ``f`` y is ``None`` (it is x), without
+    ``pre_weight`` h is ``None``.  All tensors contiguous, x and f 2-D."""
+
+    @staticmethod
+    def forward(ctx, x, f, gate, post_weight, post_bias, scale, pre_weight, pre_bias, meta):
+        params = (post_weight, post_bias, scale, pre_weight, pre_bias)
+        y, h, stats = _forward(x, f, gate, params, meta, True)
+        ctx.save_for_backward(x, f, gate, stats, *params)
+        ctx.meta = meta
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, grad_h):
+        x, f, gate, stats, *params = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        a = _args(x, f, gate, params, ctx.meta)
+        a.stats = stats.data_ptr()
+        held = [None if g is None else g.contiguous() for g in (grad_y, grad_h)]
+        a.grad_y, a.grad_h = (_native.ptr(g) for g in held)
+        grads = [None] * 8
+        names = ("grad_x", "grad_f", "grad_gate") + tuple("grad_" + n for n in _PARAMS)
+        for i, (name, t) in enumerate(zip(names, (x, f, gate, *params))):
+            if need[i] and t is not None:
+                grads[i] = torch.empty_like(t)
+                setattr(a, name, grads[i].data_ptr())
+        _native.run("nnue_ls_norm_backward", a, x.device)
+        return (*grads, None)
+
+
+def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: torch.Tensor | None = None,
+               post_bias: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_activation: str = "none",
+               residual_scale: float | torch.Tensor = 1.0, pre_weight: torch.Tensor | None = None,
+               pre_bias: torch.Tensor | None = None, kind: str = "rms",
+               eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Close one residual block and open the next::
+
+        n = norm(f) * post_weight + post_bias      # n = f without post_weight
+        y = residual_scale * x + gate * n          # y = x without f
+        h = norm(y) * pre_weight + pre_bias        # h is None without pre_weight
+
+    and return ``(y, h)``.  ``x`` (the residual stream) and ``f`` (the block's
+    output) are ``[..., width]`` in fp32, bf16 or fp16; ``norm`` is the
+    ``"rms"`` or ``"layer"`` norm of a row.  ``gate`` is one value per row
+    (``[...]`` or ``[..., 1]``, also in fp32), or elementwise (broadcast to
+    x's shape, in x's type); with ``gate_activation="sigmoid"`` it goes through
+    a sigmoid first.  ``residual_scale`` is a number or a learned ``[width]``
+    tensor.  The parameters share one type, x's or fp32.  Statistics and sums
+    are held in fp32, h is normalised from the unrounded y, and each output is
+    rounded once.  Differentiable once, in every tensor argument.
+    """
+    _native.check_tensor(x, "x")
+    dev, dt = x.device, x.dtype
+    mixed = (dt,) if dt == torch.float32 else (dt, torch.float32)
+    if kind not in _KINDS:
+        raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
+    if gate_activation not in ("none", "sigmoid"):
+        raise ValueError(f"gate_activation must be 'none' or 'sigmoid', got {gate_activation!r}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _native.NORM_MAX_WIDTH:
+        raise ValueError(f"x must be [..., width] with 1 <= width <= {_native.NORM_MAX_WIDTH}, got {tuple(x.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    shape, width = x.shape, x.shape[-1]
+    scale, scale_value = None, 1.0
+    if isinstance(residual_scale, torch.Tensor):
+        scale = residual_scale
+    else:
+        scale_value = float(residual_scale)
+    if f is None:
+        if post_weight is not None or gate is not None or scale is not None or scale_value != 1.0:
+            raise ValueError("post_weight, gate and residual_scale belong to a block's output f")
+        if pre_weight is None:
+            raise ValueError("nothing to do: give f, pre_weight or both")
+    else:
+        _native.check_tensor(f, "f", dev, (dt,))
+        if f.shape != shape:
+            raise ValueError(f"f {tuple(f.shape)} must have x's shape {tuple(shape)}")
+    if (post_bias is not None and post_weight is None) or (pre_bias is not None and pre_weight is None):
+        raise ValueError("a norm's bias needs its weight")
+    params, params_dtype = [], None
+    for name, t in zip(("post_weight", "post_bias", "residual_scale", "pre_weight", "pre_bias"),
+                       (post_weight, post_bias, scale, pre_weight, pre_bias)):
+        if t is not None:
+            _native.check_tensor(t, name, dev, mixed if params_dtype is None else (params_dtype,))
+            params_dtype = t.dtype
+            if t.dim() != 1 or t.shape[0] != width:
+                raise ValueError(f"{name} must have shape ({width},), got {tuple(t.shape)}")
+            t = t.contiguous()
+        params.append(t)
+    mode = 0
+    if gate is not None:
+        if gate.shape == shape[:-1] or (gate.shape == shape[:-1] + (1,) and width > 1):
+            mode = 1
+            _native.check_tensor(gate, "gate", dev, mixed)
+            gate = gate.reshape(-1)
+        else:
+            mode = 2
+            _native.check_tensor(gate, "gate", dev, (dt,))
+            try:
+                gate = gate.expand(shape)
+            except RuntimeError:
+                raise ValueError(f"gate {tuple(gate.shape)} fits neither x's rows nor its shape {tuple(shape)}") \
+                    from None
+            gate = gate.reshape(-1, width)
+        gate = gate.contiguous()
+    x2 = x.reshape(-1, width).contiguous()
+    f2 = None if f is None else f.reshape(-1, width).contiguous()
+    meta = (_KINDS[kind], mode, int(gate_activation == "sigmoid"), scale_value, float(eps))
+    if _native.needs_grad(x2, f2, gate, *params):
+        y, h = BlockNormFunction.apply(x2, f2, gate, *params, meta)
+    else:
+        y, h, _ = _forward(x2, f2, gate, params, meta, False)
+    y = x if f is None else y.view(shape)
+    return y, None if h is None else h.view(shape)

@@ -56,7 +56,7 @@ int nnue_ls_device_errors(uint32_t *flags, int clear);
  *   z = x W^T + bias;  out = act(z) + residual
  * x: [rows, inputs]; weight: [outputs, inputs]; bias: [outputs] or null;
  * residual, out: [rows, outputs] (residual may be null).  1 <= inputs,
- * outputs < 2^31, 0 <= rows < 2^31. */
+ * outputs < 2^30, 0 <= rows < 2^30. */
 #define NNUE_LS_ACT_NONE 0
 #define NNUE_LS_ACT_RELU 1
 #define NNUE_LS_ACT_CRELU 2     /* clamp(z, 0, 1) */
@@ -73,8 +73,9 @@ typedef struct {
   const void *x, *weight, *bias, *residual;
   int64_t ldx, ldw, ldr;
   void *out;      /* forward; row stride outputs */
-  void *act_grad; /* act'(z), row stride outputs: written by the forward when not null, read by the
-                     backward, which needs it for every activation but NNUE_LS_ACT_NONE */
+  void *act_grad; /* act'(z) in a form of the library's own, [rows, outputs] values as wide as dtype:
+                     written by the forward when not null, read by the backward, which needs it for every
+                     activation but NNUE_LS_ACT_NONE */
   const void *grad_out; /* backward */
   int64_t ldg;
   void *grad_x, *grad_weight, *grad_bias; /* contiguous; null = not wanted */

@@ -1,0 +1,428 @@
+// Matrix product of the linear layer on the 5th-generation tensor cores:
+//   C[m, n] = sum_k A(m, k) B(n, k)
+// A and B are 16-bit, each either K-major (a row of the matrix is contiguous
+// along k) or MN-major (contiguous along m or n): the forward's x and W are
+// K-major, the input gradient reads W MN-major, the weight gradient reads dz
+// and x MN-major, so no operand is ever transposed in memory.
+//
+// fp32 operands come as three bf16 planes whose sum is the value (8 + 8 + 8
+// bits, exact); six of the nine plane products are formed, the three left out
+// are below 2^-23 of the product.
+//
+// One persistent block per SM (or a pair of blocks on two SMs, CG = 2, sharing
+// a 256-row tile: each holds half of A's rows and half of B's, which halves
+// what is read from L2 per product).  Warp 0 copies tiles by TMA into a ring
+// of shared-memory stages, warp 1 issues the products into TMEM, warps 4-11
+// read finished accumulators back while the next tile's products run.
+#pragma once
+
+#include <cuda.h>
+
+#include "ls_common.cuh"
+#include "ls_epilogue.cuh"
+
+namespace nnue_ls {
+
+constexpr int kGemmThreads = 384;
+constexpr int kEpilogueWarp0 = 4, kEpilogueWarps = 8;
+constexpr int kTileM = 128;          // rows of C per block
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+
+// Shared memory: stages of A and B tiles, one transpose buffer per epilogue
+// warp, barriers.  Planes = 1: 64 k values per stage; 3: 32.
+template <int PLANES, int CG>
+struct GemmShape {
+  static constexpr int kBK = PLANES == 1 ? 64 : 32;
+  static constexpr int kMaxBN = PLANES == 3 && CG == 1 ? 128 : 256;  // columns of C per tile
+  static constexpr int kRowsB = kMaxBN / CG;                         // rows of B held by one block
+  static constexpr int kPlaneA = kTileM * kBK * 2, kPlaneB = kRowsB * kBK * 2;
+  static constexpr int kStage = PLANES * (kPlaneA + kPlaneB);
+  static constexpr int kStages = PLANES == 1 ? (CG == 1 ? 4 : 6) : 4;
+  static constexpr int kTranspose = kEpilogueWarps * 32 * 33 * 4;
+  static constexpr int kSmem = 1024 + kStages * kStage + kTranspose + 256;
+  // k blocks summed in TMEM before the epilogue warps take the sum into
+  // registers.  The tensor cores' running sums lose up to a unit of the last
+  // place per instruction; with fp32 operands that would show, so there a
+  // chain is 2 blocks x 2 steps x 6 products long.  0: all of the item's.
+  static constexpr int kChunk = PLANES == 1 ? 0 : 2;
+};
+
+struct GemmParams {
+  CUtensorMap a, b;  // [planes][rows][columns], the contiguous direction first
+  int64_t M, N;
+  int32_t k_blocks, splits;      // k blocks in all; pieces the k range is cut into
+  int32_t m_tiles, n_tiles, bn;  // bn: columns of C per tile, a multiple of 16
+  int32_t a_mn, b_mn;            // 1: MN-major
+  uint32_t idesc;
+  float* partial;  // splits > 1: [splits, M, N] sums, joined by another kernel
+  EpilogueParams e;
+};
+
+// ---- PTX ---------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Arrives on the barrier at the same offset in the pair's first block.
+__device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
+  asm volatile(
+      "{\n .reg .b32 ra;\n mapa.shared::cluster.u32 ra, %0, 0;\n"
+      " mbarrier.arrive.shared::cluster.b64 _, [ra];\n}" ::"r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint64_t global_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// Waits for the phase, for kWaitLimitNs at most; a wait that runs out raises
+// the device flag and ends every other wait of the block.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  while (!mbar_try(bar, parity)) {
+    if (*gave_up) return false;
+    if (global_ns() - t0 > kWaitLimitNs) {
+      *gave_up = 1;
+      flag_error(kErrWaitTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Copies one box; in a pair both blocks' copies count on the first block's barrier.
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CG == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar & 0xfeffffffu)  // bit 24 selects the block within the pair
+        : "memory");
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_slot) {
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+  if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 1) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// The barrier's phase ends when the products issued so far are done; in a pair
+// the barrier at this offset in both blocks.
+template <int CG>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+}
+__device__ __forceinline__ void tcgen_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcgen_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 lanes x 32 columns of accumulators: this thread's lane, 32 columns.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Shared-memory operand descriptors.  K-major: rows of BK values, 8-row groups
+// `8 * BK * 2` bytes apart, 128-byte swizzle for 64 values and 64-byte for 32.
+// MN-major: rows of 64 m (or n) values under the 128-byte swizzle, one row per
+// k; 8-k groups 1024 bytes apart, blocks of 64 values BK rows apart.
+template <int BK>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int mn_major) {
+  const uint64_t swizzle = mn_major || BK == 64 ? 2 : 4;
+  const uint64_t sbo = mn_major ? 1024 : 8 * BK * 2;
+  const uint64_t lbo = mn_major ? BK * 128 : 16;
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (lbo >> 4) << 16 | (sbo >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
+}
+
+// ---- the kernel -----------------------------------------------------------------
+template <typename T, int CG>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+  using S = GemmShape<PLANES, CG>;
+  constexpr int BK = S::kBK;
+  extern __shared__ uint8_t smem_raw[];
+  // the same offset in both blocks of a pair: the dynamic shared memory starts at the same address there
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float* transpose = reinterpret_cast<float*>(smem + S::kStages * S::kStage);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStage + S::kTranspose);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S::kStages;
+  const uint32_t acc_full0 = empty0 + 8 * S::kStages, acc_empty0 = acc_full0 + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 4);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 1 ? 0 : (int)cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full0 + 8 * i, 1);
+      mbar_init(acc_empty0 + 8 * i, kEpilogueWarps * CG);
+    }
+    *gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async;" ::: "memory");
+  }
+  if (warp == 2) tmem_alloc<CG>(smem_u32(tmem_slot));
+  tcgen_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  tcgen_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, items = tiles * p.splits;
+  const int rows_b = p.bn / CG;  // rows of B this block holds
+  const int blocks_b = (rows_b + 63) / 64;
+
+  if (warp == 0 && lane == 0) {
+    // ---- copies ----
+    const uint32_t bytes =
+        CG * PLANES * (S::kPlaneA + (p.b_mn ? blocks_b * 64 * BK * 2 : rows_b * BK * 2));
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (int64_t item = worker; item < items && ok; item += workers) {
+      const int64_t tile = item % tiles;
+      const int split = (int)(item / tiles);
+      const int m0 = (int)(tile / p.n_tiles) * (kTileM * CG) + rank * kTileM;
+      const int n0 = (int)(tile % p.n_tiles) * p.bn + rank * rows_b;
+      const int k0 = (int)((int64_t)p.k_blocks * split / p.splits), k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
+      for (int k = k0; k < k1; ++k) {
+        if (!(ok = mbar_wait(empty0 + 8 * stage, phase ^ 1, gave_up))) break;
+        const uint32_t bar = full0 + 8 * stage;
+        if (rank == 0) mbar_expect(bar, bytes);
+        const uint32_t sa = smem_u32(smem + stage * S::kStage), sb = sa + PLANES * S::kPlaneA;
+        for (int q = 0; q < PLANES; ++q) {
+          if (p.a_mn) {
+            for (int i = 0; i < kTileM / 64; ++i)
+              tma_load<CG>(sa + q * S::kPlaneA + i * 64 * BK * 2, &p.a, m0 + 64 * i, k * BK, q, bar);
+          } else {
+            tma_load<CG>(sa + q * S::kPlaneA, &p.a, k * BK, m0, q, bar);
+          }
+          if (p.b_mn) {
+            for (int i = 0; i < blocks_b; ++i)
+              tma_load<CG>(sb + q * S::kPlaneB + i * 64 * BK * 2, &p.b, n0 + 64 * i, k * BK, q, bar);
+          } else {
+            tma_load<CG>(sb + q * S::kPlaneB, &p.b, k * BK, n0, q, bar);
+          }
+        }
+        if (++stage == S::kStages) stage = 0, phase ^= 1;
+      }
+    }
+    // the last copies and products have to land before the block ends: wait for every stage to be free again
+    for (int i = 0; i < S::kStages; ++i) {
+      const uint64_t t0 = global_ns();
+      while (!mbar_try(empty0 + 8 * stage, phase ^ 1) && global_ns() - t0 < (ok ? kWaitLimitNs : kWaitLimitNs / 16)) {
+      }
+      if (++stage == S::kStages) stage = 0, phase ^= 1;
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---- products ----
+    const uint32_t step_a = (p.a_mn ? 16 * 128 : 32) >> 4, step_b = (p.b_mn ? 16 * 128 : 32) >> 4;
+    uint32_t stage = 0, phase = 0, chunk = 0;
+    bool ok = true;
+    for (int64_t item = worker; item < items && ok; item += workers) {
+      const int split = (int)(item / tiles);
+      const int k0 = (int)((int64_t)p.k_blocks * split / p.splits), k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
+      const int per_chunk = S::kChunk ? S::kChunk : k1 - k0;
+      for (int kc = k0; kc < k1 && ok; kc += per_chunk, ++chunk) {
+        const uint32_t acc = chunk & 1, d = tmem + acc * 256;
+        if (!(ok = mbar_wait(acc_empty0 + 8 * acc, ((chunk >> 1) & 1) ^ 1, gave_up))) break;
+        tcgen_fence_after();
+        uint32_t accumulate = 0;
+        for (int k = kc; k < min(kc + per_chunk, k1); ++k) {
+          if (!(ok = mbar_wait(full0 + 8 * stage, phase, gave_up))) break;
+          tcgen_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * S::kStage), sb = sa + PLANES * S::kPlaneA;
+          uint64_t da[PLANES], db[PLANES];
+#pragma unroll
+          for (int q = 0; q < PLANES; ++q) {
+            da[q] = operand_desc<BK>(sa + q * S::kPlaneA, p.a_mn);
+            db[q] = operand_desc<BK>(sb + q * S::kPlaneB, p.b_mn);
+          }
+#pragma unroll
+          for (int i = 0; i < BK / 16; ++i) {
+            // small products first
+#pragma unroll
+            for (int s = PLANES == 1 ? 0 : 2; s >= 0; --s)
+#pragma unroll
+              for (int q = 0; q <= s; ++q) {
+                mma<CG>(d, da[q] + i * step_a, db[s - q] + i * step_b, p.idesc, accumulate);
+                accumulate = 1;
+              }
+          }
+          mma_commit<CG>(empty0 + 8 * stage);
+          if (++stage == S::kStages) stage = 0, phase ^= 1;
+        }
+        if (ok) mma_commit<CG>(acc_full0 + 8 * acc);
+      }
+    }
+  } else if (warp >= kEpilogueWarp0) {
+    // ---- epilogue: warp's quarter of the lanes, every second block of 32 columns ----
+    const int quarter = warp & 3, half = (warp - kEpilogueWarp0) >> 2;
+    float* stage = transpose + (warp - kEpilogueWarp0) * 32 * 33;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int col_blocks = (p.bn + 31) / 32;
+    uint32_t chunk = 0;
+    bool ok = true;
+    for (int64_t item = worker; item < items && ok; item += workers) {
+      const int64_t tile = item % tiles;
+      const int split = (int)(item / tiles);
+      const int64_t m0 = (tile / p.n_tiles) * (kTileM * CG) + rank * kTileM + quarter * 32;
+      const int64_t n0 = (tile % p.n_tiles) * p.bn, n1 = min(p.N, n0 + p.bn);
+      float* partial = p.splits > 1 ? p.partial + (int64_t)split * p.M * p.N : nullptr;
+      auto finish = [&](int cb, const float (&v)[32]) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) stage[lane * 33 + j] = v[j];
+        __syncwarp();
+        if (partial) store_partial(stage, partial, m0, p.M, n0 + cb * 32, n1, p.N, lane);
+        else store_block<T>(stage, p.e, m0, p.M, n0 + cb * 32, n1, p.N, lane);
+      };
+      if constexpr (S::kChunk == 0) {
+        const uint32_t acc = chunk & 1;
+        if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk >> 1) & 1, gave_up))) break;
+        tcgen_fence_after();
+        for (int cb = half; cb < col_blocks; cb += 2) {
+          float v[32];
+          tmem_load32(lanes + acc * 256 + cb * 32, v);
+          if (cb + 2 >= col_blocks) {  // this warp's last read: the accumulator may be written again
+            tcgen_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CG == 1) mbar_arrive(acc_empty0 + 8 * acc);
+              else mbar_arrive_leader(acc_empty0 + 8 * acc);
+            }
+          }
+          finish(cb, v);
+        }
+        if (half >= col_blocks && lane == 0) {  // a narrow tile leaves this warp nothing to read
+          if constexpr (CG == 1) mbar_arrive(acc_empty0 + 8 * acc);
+          else mbar_arrive_leader(acc_empty0 + 8 * acc);
+        }
+        ++chunk;
+      } else {
+        constexpr int kMine = S::kMaxBN / 64;  // column blocks of 32 per warp
+        float sum[kMine][32];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[i][j] = 0.f;
+        const int k0 = (int)((int64_t)p.k_blocks * split / p.splits),
+                  k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
+        for (int kc = k0; kc < k1; kc += S::kChunk, ++chunk) {
+          const uint32_t acc = chunk & 1;
+          if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk >> 1) & 1, gave_up))) break;
+          tcgen_fence_after();
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const int cb = half + 2 * i;
+            if (cb < col_blocks) {
+              float v[32];
+              tmem_load32(lanes + acc * 256 + cb * 32, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum[i][j] += v[j];
+            }
+          }
+          tcgen_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) mbar_arrive(acc_empty0 + 8 * acc);
+            else mbar_arrive_leader(acc_empty0 + 8 * acc);
+          }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if (half + 2 * i < col_blocks) finish(half + 2 * i, sum[i]);
+      }
+    }
+  }
+  __syncwarp();
+  tcgen_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the other block may still signal barriers here
+  if (warp == 2) {
+    tcgen_fence_after();
+    tmem_free<CG>(tmem);
+  }
+}
+
+}  // namespace nnue_ls

@@ -1,131 +1,142 @@
-// Fused linear layer: out = act(x W^T + b) + residual, and its gradients.
+// The memory-bound passes around the linear layer's matrix products: operands
+// brought into the products' layout, the output gradient times act'(z) with
+// its column sums, the join of a product whose k range was cut into pieces.
 #pragma once
 
 #include "ls_common.cuh"
+#include "ls_epilogue.cuh"
 
 namespace nnue_ls {
 
-enum Activation : int { kNone = 0, kRelu = 1, kCrelu = 2, kSqrCrelu = 3, kSilu = 4, kGelu = 5, kActivations = 6 };
-
-// act(z) and act'(z).  At the kinks of the clipped forms the derivative is 0,
-// as in clamp's backward outside the open interval.
-__device__ __forceinline__ float activate(float z, int act, float& d) {
-  switch (act) {
-    case kRelu: d = z > 0.f ? 1.f : 0.f; return z > 0.f || z != z ? z : 0.f;
-    case kCrelu: d = z > 0.f && z < 1.f ? 1.f : 0.f; return z != z ? z : fminf(fmaxf(z, 0.f), 1.f);
-    case kSqrCrelu: {
-      const float c = z != z ? z : fminf(fmaxf(z, 0.f), 1.f);
-      d = z > 0.f && z < 1.f ? 2.f * z : 0.f;
-      return c * c;
+// The three bf16 planes of V fp32 values: each takes the leading 8 bits of
+// what is left, so their sum is the value.  An infinity or NaN stays in the
+// first plane.
+template <int V>
+__device__ __forceinline__ void split_planes(const float (&v)[V], uint16_t (&q)[3][V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float r = v[i];
+    const bool finite = (__float_as_uint(r) & 0x7f800000u) != 0x7f800000u;
+    if (!finite) {
+      q[0][i] = r != r ? 0x7fff : (uint16_t)(__float_as_uint(r) >> 16);
+      q[1][i] = q[2][i] = 0;
+      continue;
     }
-    case kSilu: {
-      const float s = 1.f / (1.f + expf(-z));
-      d = s * (1.f + z * (1.f - s));
-      return z * s;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint32_t top = __float_as_uint(r) & 0xffff0000u;
+      q[k][i] = (uint16_t)(top >> 16);
+      r -= __uint_as_float(top);
     }
-    case kGelu: {
-      const float phi = 0.5f * erfcf(-0.70710678118654752f * z);
-      d = phi + z * (0.39894228040143268f * expf(-0.5f * z * z));
-      return z * phi;
-    }
-    default: d = 1.f; return z;
   }
 }
 
-struct LinearEpilogue {
-  const void* bias;
-  const void* residual;
-  void* out;
-  void* act_grad;  // act'(z) in the tensors' type, [rows, outputs]; null when no gradient is wanted
-  int64_t ldr, ldo;
-  int act;
-  bool bias_f32;
+template <int V>
+struct alignas(2 * V) Pack16 {
+  uint16_t v[V];
 };
 
-// C[m, n] = sum_k A[m, k] B[n, k] with any strides, fp32 accumulation: 64 x 64
-// tiles through shared memory, 4 x 4 outputs per thread.
-constexpr int kTile = 64, kTileK = 16;
-template <typename T>
-__global__ void __launch_bounds__(256) simple_gemm_kernel(const T* __restrict__ a, int64_t sam, int64_t sak,
-                                                          const T* __restrict__ b, int64_t sbn, int64_t sbk, int64_t M,
-                                                          int64_t N, int64_t K, LinearEpilogue e) {
-  __shared__ float sa[kTileK][kTile + 1], sb[kTileK][kTile + 1];
-  const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += kTileK) {
-    for (int i = threadIdx.x; i < kTile * kTileK; i += 256) {
-      const int kk = i & (kTileK - 1), r = i / kTileK;
-      const int64_t k = k0 + kk;
-      sa[kk][r] = m0 + r < M && k < K ? to_f(a[(m0 + r) * sam + k * sak]) : 0.f;
-      sb[kk][r] = n0 + r < N && k < K ? to_f(b[(n0 + r) * sbn + k * sbk]) : 0.f;
+// Stores V neighbouring values in the products' layout: T itself, or planes
+// `plane` elements apart.
+template <typename T, int V>
+__device__ __forceinline__ void store_operand(void* dst, int64_t at, int64_t plane, const float (&v)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    uint16_t q[3][V];
+    split_planes(v, q);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      Pack16<V> o;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o.v[i] = q[k][i];
+      *reinterpret_cast<Pack16<V>*>(static_cast<uint16_t*>(dst) + k * plane + at) = o;
     }
-    __syncthreads();
+  } else {
+    struct alignas(2 * V) Out {
+      T v[V];
+    } o;
 #pragma unroll
-    for (int kk = 0; kk < kTileK; ++kk) {
-      float va[4], vb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        va[i] = sa[kk][ty + 16 * i];
-        vb[i] = sb[kk][tx + 16 * i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(va[i], vb[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty + 16 * i;
-    if (m >= M) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx + 16 * j;
-      if (n >= N) continue;
-      float z = acc[i][j], d;
-      if (e.bias) z += load_mixed<T>(e.bias, n, e.bias_f32);
-      float o = activate(z, e.act, d);
-      if (e.residual) o += to_f(static_cast<const T*>(e.residual)[m * e.ldr + n]);
-      static_cast<T*>(e.out)[m * e.ldo + n] = from_f<T>(o);
-      if (e.act_grad) static_cast<T*>(e.act_grad)[m * N + n] = from_f<T>(d);
-    }
+    for (int i = 0; i < V; ++i) o.v[i] = from_f<T>(v[i]);
+    *reinterpret_cast<Out*>(static_cast<T*>(dst) + at) = o;
   }
 }
 
-// dz = g * act'(z) (written when act_grad is given) and, per block, the column
-// sums of dz over a range of rows.  blockDim = (32 columns, 8 rows).
-template <typename T>
-__global__ void __launch_bounds__(256) dz_bias_kernel(const T* __restrict__ g, int64_t ldg,
-                                                      const T* __restrict__ act_grad, T* __restrict__ dz,
-                                                      float* __restrict__ partial, int64_t M, int64_t N,
-                                                      int64_t rows_per_block) {
-  __shared__ float red[8][33];
-  const int64_t n = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  const int64_t m0 = (int64_t)blockIdx.y * rows_per_block, m1 = min(M, m0 + rows_per_block);
-  float sum = 0.f;
-  if (n < N) {
-    for (int64_t m = m0 + threadIdx.y; m < m1; m += 8) {
-      float v = to_f(g[m * ldg + n]);
-      if (act_grad) {
-        v *= to_f(act_grad[m * N + n]);
-        dz[m * N + n] = from_f<T>(v);
+template <typename T, int V>
+struct alignas(sizeof(T) * V) VecT {
+  T v[V];
+};
+
+// [rows, cols] with row stride ld -> rows of ldo (a multiple of 8) values in
+// the products' layout; a thread moves 8 values.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
+                                                   void* __restrict__ dst, int64_t ldo) {
+  const int64_t groups = ldo / 8, total = rows * groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = (i - r * groups) * 8;
+    float v[8];
+    if (VEC && c + 8 <= cols) {
+      constexpr int W = 16 / sizeof(T);
+#pragma unroll
+      for (int j = 0; j < 8; j += W) {
+        const auto t = *reinterpret_cast<const VecT<T, W>*>(src + r * ld + c + j);
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[j + k] = to_f(t.v[k]);
       }
-      sum += v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f(src[r * ld + c + j]) : 0.f;
+    }
+    store_operand<T, 8>(dst, r * ldo + c, rows * ldo, v);
+  }
+}
+
+// dz = g * act'(z), written in the products' layout when dst is given, and per
+// block the fp32 column sums of the unrounded dz over a range of rows.
+// A block is `tx` groups of V columns wide and 256 / tx rows high.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ g, int64_t ldg,
+                                                 const typename Derivative<T>::Code* __restrict__ act_grad,
+                                                 void* __restrict__ dst, int64_t ldo, float* __restrict__ partial,
+                                                 int64_t M, int64_t N, int64_t rows_per_block, int tx) {
+  using D = Derivative<T>;
+  using Code = typename D::Code;
+  __shared__ float red[256 * V];
+  const int x = threadIdx.x % tx, y = threadIdx.x / tx, ty = 256 / tx;
+  const int64_t n = ((int64_t)blockIdx.x * tx + x) * V;
+  const int64_t m1 = min(M, ((int64_t)blockIdx.y + 1) * rows_per_block);
+  float sum[V] = {};
+  if (n < N) {
+#pragma unroll 4
+    for (int64_t m = (int64_t)blockIdx.y * rows_per_block + y; m < m1; m += ty) {
+      const auto t = *reinterpret_cast<const VecT<T, V>*>(g + m * ldg + n);
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = to_f(t.v[i]);
+      if (act_grad) {
+        const auto d = *reinterpret_cast<const VecT<Code, V>*>(act_grad + m * N + n);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= D::decode(d.v[i]);
+      }
+      if (dst) store_operand<T, V>(dst, m * ldo + n, M * ldo, v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += v[i];
     }
   }
   if (!partial) return;
-  red[threadIdx.y][threadIdx.x] = sum;
+#pragma unroll
+  for (int i = 0; i < V; ++i) red[i * 256 + threadIdx.x] = sum[i];
   __syncthreads();
-  if (threadIdx.y == 0 && n < N) {
-    for (int i = 1; i < 8; ++i) sum += red[i][threadIdx.x];
-    partial[(int64_t)blockIdx.y * N + n] = sum;
+  if (y == 0 && n < N) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      for (int j = 1; j < ty; ++j) sum[i] += red[i * 256 + j * tx + x];
+      partial[(int64_t)blockIdx.y * N + n + i] = sum[i];
+    }
   }
 }
 
-// out[n] = sum over parts of partial[part, n], in part order within each of
-// the block's 8 rows of threads.
+// out[n] = sum over parts of partial[part, n], in a fixed order: 8 rows of
+// threads take every eighth part, then their sums are added in turn.
 template <typename T>
 __global__ void __launch_bounds__(256) column_total_kernel(const float* __restrict__ partial, int64_t parts, int64_t N,
                                                            void* out, bool out_f32) {
@@ -139,6 +150,40 @@ __global__ void __launch_bounds__(256) column_total_kernel(const float* __restri
   if (threadIdx.y == 0 && n < N) {
     for (int i = 1; i < 8; ++i) sum += red[i][threadIdx.x];
     store_mixed<T>(out, n, out_f32, sum);
+  }
+}
+
+// z = sum over pieces, in piece order, then the epilogue.  VEC: N is a multiple
+// of 4 and rows are aligned; a thread takes 4 columns.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int64_t M, int64_t N,
+                                                   EpilogueParams e) {
+  using D = Derivative<T>;
+  using Code = typename D::Code;
+  constexpr int V = VEC ? 4 : 1;
+  const int64_t groups = N / V, total = M * groups, MN = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / groups, n = (i - m * groups) * V;
+    float z[V] = {};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const auto t = *reinterpret_cast<const VecT<float, V>*>(partial + s * MN + m * N + n);
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[j] += t.v[j];
+    }
+    VecT<T, V> out, res;
+    VecT<Code, V> d;
+    if (e.residual) res = *reinterpret_cast<const VecT<T, V>*>(static_cast<const T*>(e.residual) + m * e.ldr + n);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (e.bias) z[j] += load_mixed<T>(e.bias, n + j, e.bias_f32);
+      float dv, o = activate<T>(z[j], e.act, dv);
+      if (e.residual) o += to_f(res.v[j]);
+      out.v[j] = from_f<T>(o);
+      d.v[j] = D::encode(dv);
+    }
+    *reinterpret_cast<VecT<T, V>*>(static_cast<T*>(e.out) + m * N + n) = out;
+    if (e.act_grad) *reinterpret_cast<VecT<Code, V>*>(static_cast<Code*>(e.act_grad) + m * N + n) = d;
   }
 }
 

@@ -7,58 +7,18 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <atomic>
-#include <cstdarg>
-#include <cstdio>
 
 #include "../../../include/nnue_ls.h"
 #include "ls_common.cuh"
-#include "ls_linear.cuh"
+#include "ls_host.cuh"
+#include "ls_linear_host.cuh"
 #include "ls_norm.cuh"
 #include "ls_route.cuh"
 
 namespace nnue_ls {
 namespace {
 
-thread_local char g_last_error[512];
-std::atomic<unsigned long long> g_launches{0};
-
-inline void count_launch(unsigned n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
-
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-int check_launch(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-constexpr int64_t kMaxDim = INT32_MAX;
-
-bool bad_dtype(int t) { return t < NNUE_LS_F32 || t > NNUE_LS_F16; }
-
-int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
-  if (need == 0) return NNUE_LS_OK;
-  if (!ws || have < need) return fail(NNUE_LS_ERR_WORKSPACE, "%s: workspace has %zu bytes, needs %zu", what, have, need);
-  if (reinterpret_cast<uintptr_t>(ws) % 256) return fail(NNUE_LS_ERR_WORKSPACE, "%s: workspace not 256-byte aligned", what);
-  return NNUE_LS_OK;
-}
-
-// Calls fn(T{}) with the element type of `dtype`.
-template <typename F>
-void with_type(int dtype, const F& fn) {
-  if (dtype == NNUE_LS_F32) fn(float{});
-  else if (dtype == NNUE_LS_BF16) fn(bf16{});
-  else fn(f16{});
-}
+constexpr int64_t kMaxDim = (1 << 30) - 1;
 
 // ---- linear ----------------------------------------------------------------
 int check_linear(const char* what, const nnue_ls_linear* a) {
@@ -66,36 +26,12 @@ int check_linear(const char* what, const nnue_ls_linear* a) {
   if (a->rows < 0 || a->inputs < 1 || a->outputs < 1)
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: need rows >= 0, inputs >= 1, outputs >= 1", what);
   if (a->rows > kMaxDim || a->inputs > kMaxDim || a->outputs > kMaxDim)
-    return fail(NNUE_LS_ERR_UNSUPPORTED, "%s: sizes must be below 2^31", what);
+    return fail(NNUE_LS_ERR_UNSUPPORTED, "%s: sizes must be below 2^30", what);
   if (bad_dtype(a->dtype) || (a->bias_dtype != a->dtype && a->bias_dtype != NNUE_LS_F32))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: bad element type", what);
   if (a->activation < 0 || a->activation >= kActivations)
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, a->activation);
   return NNUE_LS_OK;
-}
-
-struct BackwardPlan {
-  size_t dz, partial, total;
-  int64_t parts, rows_per_part;
-};
-
-BackwardPlan plan_backward(const nnue_ls_linear& a) {
-  BackwardPlan p{};
-  const int64_t columns = ceil_div(a.outputs, 32);
-  p.parts = std::max<int64_t>(1, std::min(ceil_div(a.rows, 64), ceil_div(kNumSMs * 8, columns)));
-  p.rows_per_part = std::max<int64_t>(1, ceil_div(a.rows, p.parts));
-  p.dz = a.activation == NNUE_LS_ACT_NONE ? 0 : align256((size_t)a.rows * a.outputs * (a.dtype == NNUE_LS_F32 ? 4 : 2));
-  p.partial = a.grad_bias ? align256((size_t)p.parts * a.outputs * 4) : 0;
-  p.total = p.dz + p.partial;
-  return p;
-}
-
-template <typename T>
-void simple_gemm(const T* a, int64_t sam, int64_t sak, const T* b, int64_t sbn, int64_t sbk, int64_t M, int64_t N,
-                 int64_t K, const LinearEpilogue& e, cudaStream_t s) {
-  count_launch();
-  const dim3 grid((unsigned)ceil_div(M, kTile), (unsigned)ceil_div(N, kTile));
-  simple_gemm_kernel<T><<<grid, 256, 0, s>>>(a, sam, sak, b, sbn, sbk, M, N, K, e);
 }
 
 // ---- norm --------------------------------------------------------------------
@@ -234,32 +170,31 @@ int nnue_ls_device_errors(uint32_t* flags, int clear) {
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
 
-size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear*) { return 0; }
+size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear* a) {
+  if (check_linear("linear_forward", a) || a->rows == 0) return 0;
+  return with_type(a->dtype, [&](auto t) { return plan_forward<decltype(t)>(*a).total; });
+}
 
-int nnue_ls_linear_forward(const nnue_ls_linear* a, void*, size_t, void* stream) {
+int nnue_ls_linear_forward(const nnue_ls_linear* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_linear("linear_forward", a)) return rc;
   if (a->rows == 0) return NNUE_LS_OK;
   if (!a->x || !a->weight || !a->out) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: null pointer");
   if (a->ldx < a->inputs || a->ldw < a->inputs || (a->residual && a->ldr < a->outputs))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: row stride below the row length");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  LinearEpilogue e{a->bias, a->residual, a->out, a->act_grad, a->ldr, a->outputs, a->activation,
-                   a->bias_dtype == NNUE_LS_F32};
-  with_type(a->dtype, [&](auto t) {
+  return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    simple_gemm<T>(static_cast<const T*>(a->x), a->ldx, 1, static_cast<const T*>(a->weight), a->ldw, 1, a->rows,
-                   a->outputs, a->inputs, e, s);
+    if (int rc = check_workspace("linear_forward", workspace, workspace_bytes, plan_forward<T>(*a).total)) return rc;
+    return linear_forward<T>(*a, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
-  return check_launch("linear_forward");
 }
 
 size_t nnue_ls_linear_backward_workspace_size(const nnue_ls_linear* a) {
-  return check_linear("linear_backward", a) ? 0 : plan_backward(*a).total;
+  if (check_linear("linear_backward", a)) return 0;
+  return with_type(a->dtype, [&](auto t) { return plan_backward<decltype(t)>(*a).total; });
 }
 
 int nnue_ls_linear_backward(const nnue_ls_linear* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_linear("linear_backward", a)) return rc;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->rows > 0) {
     if (!a->grad_out || (a->activation != NNUE_LS_ACT_NONE && !a->act_grad) || (a->grad_x && !a->weight) ||
         (a->grad_weight && !a->x))
@@ -267,40 +202,11 @@ int nnue_ls_linear_backward(const nnue_ls_linear* a, void* workspace, size_t wor
     if (a->ldg < a->outputs || (a->grad_x && a->ldw < a->inputs) || (a->grad_weight && a->ldx < a->inputs))
       return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_backward: row stride below the row length");
   }
-  const BackwardPlan p = plan_backward(*a);
-  if (int rc = check_workspace("linear_backward", workspace, workspace_bytes, p.total)) return rc;
-  char* ws = static_cast<char*>(workspace);
-  with_type(a->dtype, [&](auto t) {
+  return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    const T* dz = static_cast<const T*>(a->grad_out);
-    int64_t lddz = a->ldg;
-    float* partial = p.partial ? reinterpret_cast<float*>(ws + p.dz) : nullptr;
-    if (p.dz || partial) {
-      T* out = p.dz ? reinterpret_cast<T*>(ws) : nullptr;
-      count_launch();
-      dz_bias_kernel<T><<<dim3((unsigned)ceil_div(a->outputs, 32), (unsigned)p.parts), dim3(32, 8), 0, s>>>(
-          dz, lddz, p.dz ? static_cast<const T*>(a->act_grad) : nullptr, out, partial, a->rows, a->outputs,
-          p.rows_per_part);
-      if (p.dz) dz = out, lddz = a->outputs;
-    }
-    if (partial) {
-      count_launch();
-      column_total_kernel<T><<<(unsigned)ceil_div(a->outputs, 32), dim3(32, 8), 0, s>>>(
-          partial, p.parts, a->outputs, a->grad_bias, a->bias_dtype == NNUE_LS_F32);
-    }
-    LinearEpilogue e{};
-    if (a->grad_x && a->rows > 0) {
-      e.out = a->grad_x;
-      e.ldo = a->inputs;
-      simple_gemm<T>(dz, lddz, 1, static_cast<const T*>(a->weight), 1, a->ldw, a->rows, a->inputs, a->outputs, e, s);
-    }
-    if (a->grad_weight) {
-      e.out = a->grad_weight;
-      e.ldo = a->inputs;
-      simple_gemm<T>(dz, 1, lddz, static_cast<const T*>(a->x), 1, a->ldx, a->outputs, a->inputs, a->rows, e, s);
-    }
+    if (int rc = check_workspace("linear_backward", workspace, workspace_bytes, plan_backward<T>(*a).total)) return rc;
+    return linear_backward<T>(*a, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
-  return check_launch("linear_backward");
 }
 
 int nnue_ls_norm_forward(const nnue_ls_norm* a, void* stream) {

@@ -2,6 +2,8 @@
 //   out = act(z + bias) + residual,  and act'(z) for the backward.
 #pragma once
 
+#include <type_traits>
+
 #include "ls_common.cuh"
 
 namespace nnue_ls {
@@ -10,31 +12,63 @@ enum Activation : int { kNone = 0, kRelu = 1, kCrelu = 2, kSqrCrelu = 3, kSilu =
 
 // act(z) and act'(z).  At the kinks of the clipped forms the derivative is 0,
 // as in clamp's backward outside the open interval.
-// For 16-bit results the short exponential (2^-21 relative) does.
-template <typename T>
-__device__ __forceinline__ float exponential(float v) { return sizeof(T) == 4 ? expf(v) : __expf(v); }
+//
+// gelu(z) = z Phi(z), Phi(z) = erfc(-z / sqrt 2) / 2.  For 16-bit results, with
+// u = |z| / sqrt 2 and t = 1 / (1 + 0.45 u), erfc(u) = exp(-u^2) P(t): P is the
+// polynomial of degree 6 without constant term whose largest relative error
+// against exp(u^2) erfc(u) on u in [0, 14] is least (a linear program over its
+// coefficients; 9.5e-6), so the lower tail keeps its digits too.  The
+// exponential is the density's, needed for the derivative anyway.  fp32 results
+// take erfcf.
+// The hardware's own reciprocal and power of two (2^-22 relative, subnormals
+// flushed), for 16-bit results.
+__device__ __forceinline__ float short_rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float short_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
-template <typename T>
-__device__ __forceinline__ float activate(float z, int act, float& d) {
-  switch (act) {
-    case kRelu: d = z > 0.f ? 1.f : 0.f; return z > 0.f || z != z ? z : 0.f;
-    case kCrelu: d = z > 0.f && z < 1.f ? 1.f : 0.f; return z != z ? z : fminf(fmaxf(z, 0.f), 1.f);
-    case kSqrCrelu: {
-      const float c = z != z ? z : fminf(fmaxf(z, 0.f), 1.f);
-      d = z > 0.f && z < 1.f ? 2.f * z : 0.f;
-      return c * c;
+template <typename T, int ACT>
+__device__ __forceinline__ float activate(float z, float& d) {
+  constexpr bool kShort = sizeof(T) == 2;
+  if constexpr (ACT == kRelu) {
+    d = z > 0.f ? 1.f : 0.f;
+    return z > 0.f || z != z ? z : 0.f;
+  } else if constexpr (ACT == kCrelu || ACT == kSqrCrelu) {
+    const float c = z != z ? z : fminf(fmaxf(z, 0.f), 1.f);
+    const bool inside = z > 0.f && z < 1.f;
+    d = inside ? (ACT == kCrelu ? 1.f : 2.f * z) : 0.f;
+    return ACT == kCrelu ? c : c * c;
+  } else if constexpr (ACT == kSilu) {
+    const float s = kShort ? short_rcp(1.f + short_exp2(-1.44269504f * z)) : 1.f / (1.f + expf(-z));
+    d = s * (1.f + z * (1.f - s));
+    return z * s;
+  } else if constexpr (ACT == kGelu) {
+    float phi, bell;
+    if constexpr (kShort) {
+      const float t = short_rcp(fmaf(0.45f * 0.70710678f, fabsf(z), 1.f));
+      bell = short_exp2(-0.72134752f * z * z);
+      float p = fmaf(t, -0.135856772f, 0.292236458f);
+      p = fmaf(t, p, 0.0894653538f);
+      p = fmaf(t, p, 0.248474505f);
+      p = fmaf(t, p, 0.251702836f);
+      p = fmaf(t, p, 0.253968126f);
+      const float tail = 0.5f * t * p * bell;
+      phi = z < 0.f ? tail : 1.f - tail;
+    } else {
+      bell = expf(-0.5f * z * z);
+      phi = 0.5f * erfcf(-0.70710678118654752f * z);
     }
-    case kSilu: {
-      const float s = 1.f / (1.f + exponential<T>(-z));
-      d = s * (1.f + z * (1.f - s));
-      return z * s;
-    }
-    case kGelu: {
-      const float phi = 0.5f * erfcf(-0.70710678118654752f * z);
-      d = phi + z * (0.39894228040143268f * exponential<T>(-0.5f * z * z));
-      return z * phi;
-    }
-    default: d = 1.f; return z;
+    d = fmaf(z * 0.39894228040143268f, bell, phi);
+    return z * phi;
+  } else {
+    d = 1.f;
+    return z;
   }
 }
 
@@ -55,11 +89,13 @@ struct Derivative<bf16> {
   using Code = uint16_t;
   static constexpr float kScale = 28672.f;
   static constexpr int kZero = 4096, kNan = 65535;
+  // Adding 1.5 * 2^23 leaves the rounded integer in the low bits; a NaN result has them all set.
   static __device__ __forceinline__ uint16_t encode(float d) {
-    return d != d ? kNan : (uint16_t)(__float2int_rn(d * kScale) + kZero);
+    return (uint16_t)__float_as_uint(fmaf(d, kScale, 12582912.f + kZero));
   }
   static __device__ __forceinline__ float decode(uint16_t c) {
-    return c == kNan ? __int_as_float(0x7fffffff) : (float)((int)c - kZero) * (1.f / kScale);
+    const float v = (__uint_as_float(0x4b000000u | c) - (8388608.f + kZero)) * (1.f / kScale);
+    return c == kNan ? __int_as_float(0x7fffffff) : v;
   }
 };
 template <>
@@ -76,66 +112,165 @@ struct EpilogueParams {
   bool vec;  // out, residual, act_grad: 16-byte aligned rows
 };
 
-template <typename T>
-struct alignas(16) Vec16 {
-  T v[16 / sizeof(T)];
+template <typename T, int V>
+struct alignas(sizeof(T) * V) VecT {
+  T v[V];
 };
 
-// Writes one 32 x 32 block of sums held in shared memory (row stride 33): rows
-// m0.., columns n0.. below n1.  With `vec` four (16-bit) or eight (fp32)
-// neighbouring lanes share a row and move 16 bytes each; else one lane per
-// column.
-template <typename T>
-__device__ __forceinline__ void store_block(const float* stage, const EpilogueParams& e, int64_t m0, int64_t M,
-                                            int64_t n0, int64_t n1, int64_t N, int lane) {
+template <typename T, int V>
+__device__ __forceinline__ void round_all(const float (&v)[V], VecT<T, V>& out) {
+  if constexpr (sizeof(T) == 2) {  // two per instruction
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      if constexpr (std::is_same<T, bf16>::value)
+        *reinterpret_cast<__nv_bfloat162*>(&out.v[j]) = __floats2bfloat162_rn(v[j], v[j + 1]);
+      else
+        *reinterpret_cast<__half2*>(&out.v[j]) = __floats2half2_rn(v[j], v[j + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out.v[j] = v[j];
+  }
+}
+
+// Calls fn with the activation as a constant.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, const F& fn) {
+  switch (act) {
+    case kRelu: fn(std::integral_constant<int, kRelu>{}); break;
+    case kCrelu: fn(std::integral_constant<int, kCrelu>{}); break;
+    case kSqrCrelu: fn(std::integral_constant<int, kSqrCrelu>{}); break;
+    case kSilu: fn(std::integral_constant<int, kSilu>{}); break;
+    case kGelu: fn(std::integral_constant<int, kGelu>{}); break;
+    default: fn(std::integral_constant<int, kNone>{}); break;
+  }
+}
+
+// A warp's 32 x 32 block of sums on its way from one row per lane to rows
+// shared by neighbouring lanes: 16-byte pieces in shared memory, a row's
+// pieces exchanged by the row's low bits so that neither side meets a bank
+// twice.
+struct Block32 {
+  float4* s;
+  __device__ __forceinline__ void put(const float (&v)[32], int lane) {
+    __syncwarp();  // the previous block has been read
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      s[lane * 8 + (j ^ (lane & 7))] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    __syncwarp();
+  }
+  template <int V>
+  __device__ __forceinline__ void get(int row, int col, float (&v)[V]) const {  // col: a multiple of V >= 4
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      const float4 t = s[row * 8 + ((col / 4 + j) ^ (row & 7))];
+      v[4 * j] = t.x, v[4 * j + 1] = t.y, v[4 * j + 2] = t.z, v[4 * j + 3] = t.w;
+    }
+  }
+  __device__ __forceinline__ float get1(int row, int col) const {
+    return reinterpret_cast<const float*>(s)[row * 32 + (((col >> 2) ^ (row & 7)) << 2) + (col & 3)];
+  }
+};
+
+// Writes one block of sums: the first `rows` rows from m0, columns n0.. below n1.  With `vec` four
+// (16-bit) or eight (fp32) neighbouring lanes share a row and move 16 bytes
+// each; else one lane per column.
+template <typename T, int ACT>
+__device__ __forceinline__ void store_block_act(const Block32& block, const EpilogueParams& e, int64_t m0, int rows,
+                                                int64_t n0, int64_t n1, int64_t N, int lane) {
   using D = Derivative<T>;
   using Code = typename D::Code;
+  constexpr int V = 16 / sizeof(T), kLanes = 32 / V, kRows = 32 / kLanes;
+  const bool with_grad = ACT != kNone && e.act_grad, with_res = e.residual;
   if (e.vec) {
-    constexpr int V = 16 / sizeof(T), kLanes = 32 / V, kRows = 32 / kLanes;
     const int c = (lane % kLanes) * V;
+    int r = lane / kLanes;
     const int64_t n = n0 + c;
-    if (n >= n1) return;
+    if (n >= n1 || r >= rows) return;
+    T* out_p = static_cast<T*>(e.out) + (m0 + r) * N + n;
+    Code* grad_p = static_cast<Code*>(e.act_grad) + (m0 + r) * N + n;
+    const T* res_p = static_cast<const T*>(e.residual) + (m0 + r) * e.ldr + n;
+    VecT<T, V> next;
+    if (with_res) next = *reinterpret_cast<const VecT<T, V>*>(res_p);
     float bias[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) bias[i] = e.bias ? load_mixed<T>(e.bias, n + i, e.bias_f32) : 0.f;
+    for (int j = 0; j < V; ++j) bias[j] = e.bias ? load_mixed<T>(e.bias, n + j, e.bias_f32) : 0.f;
+#pragma unroll 1
+    for (; r < rows; r += kRows) {
+      const VecT<T, V> res = next;
+      res_p += kRows * e.ldr;
+      if (with_res && r + kRows < rows) next = *reinterpret_cast<const VecT<T, V>*>(res_p);  // one step ahead
+      float z[V];
+      block.get<V>(r, c, z);
+      VecT<T, V> out;
+      VecT<Code, V> d;
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += kRows) {
-      const int r = r0 + lane / kLanes;
-      const int64_t m = m0 + r;
-      if (m >= M) return;
-      Vec16<T> res, out;
-      Vec16<Code> d;
-      if (e.residual) res = *reinterpret_cast<const Vec16<T>*>(static_cast<const T*>(e.residual) + m * e.ldr + n);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float dv, o = activate<T>(stage[r * 33 + c + i] + bias[i], e.act, dv);
-        if (e.residual) o += to_f(res.v[i]);
-        out.v[i] = from_f<T>(o);
-        d.v[i] = D::encode(dv);
+      for (int j = 0; j < V; ++j) {
+        float dv;
+        z[j] = activate<T, ACT>(z[j] + bias[j], dv);
+        if (with_res) z[j] += to_f(res.v[j]);
+        d.v[j] = D::encode(dv);
       }
-      *reinterpret_cast<Vec16<T>*>(static_cast<T*>(e.out) + m * N + n) = out;
-      if (e.act_grad) *reinterpret_cast<Vec16<Code>*>(static_cast<Code*>(e.act_grad) + m * N + n) = d;
+      round_all(z, out);
+      *reinterpret_cast<VecT<T, V>*>(out_p) = out;
+      if (with_grad) *reinterpret_cast<VecT<Code, V>*>(grad_p) = d;
+      out_p += kRows * N;
+      grad_p += kRows * N;
     }
   } else {
     const int64_t n = n0 + lane;
     if (n >= n1) return;
     const float bias = e.bias ? load_mixed<T>(e.bias, n, e.bias_f32) : 0.f;
-    for (int r = 0; r < 32 && m0 + r < M; ++r) {
-      const int64_t m = m0 + r;
-      float dv, o = activate<T>(stage[r * 33 + lane] + bias, e.act, dv);
-      if (e.residual) o += to_f(static_cast<const T*>(e.residual)[m * e.ldr + n]);
-      static_cast<T*>(e.out)[m * N + n] = from_f<T>(o);
-      if (e.act_grad) static_cast<Code*>(e.act_grad)[m * N + n] = D::encode(dv);
+    T* out_p = static_cast<T*>(e.out) + m0 * N + n;
+    Code* grad_p = static_cast<Code*>(e.act_grad) + m0 * N + n;
+    const T* res_p = static_cast<const T*>(e.residual) + m0 * e.ldr + n;
+#pragma unroll 1
+    for (int r = 0; r < rows; r += 4) {
+      T res[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (with_res && r + i < rows) res[i] = res_p[i * e.ldr];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float dv, o = activate<T, ACT>(block.get1(r + i, lane) + bias, dv);
+        if (with_res) o += to_f(res[i]);
+        if (r + i < rows) {
+          out_p[i * N] = from_f<T>(o);
+          if (with_grad) grad_p[i * N] = D::encode(dv);
+        }
+      }
+      out_p += 4 * N;
+      grad_p += 4 * N;
+      res_p += 4 * e.ldr;
     }
   }
 }
 
-// The raw sums of one piece of the k range.
-__device__ __forceinline__ void store_partial(const float* stage, float* partial, int64_t m0, int64_t M, int64_t n0,
-                                              int64_t n1, int64_t N, int lane) {
-  const int64_t n = n0 + lane;
-  if (n >= n1) return;
-  for (int r = 0; r < 32 && m0 + r < M; ++r) partial[(m0 + r) * N + n] = stage[r * 33 + lane];
+template <typename T>
+__device__ __forceinline__ void store_block(const Block32& block, const EpilogueParams& e, int64_t m0, int rows,
+                                            int64_t n0, int64_t n1, int64_t N, int lane) {
+  with_activation(e.act,
+                  [&](auto act) { store_block_act<T, decltype(act)::value>(block, e, m0, rows, n0, n1, N, lane); });
+}
+
+// The raw sums of one piece of the k range; vec: N is a multiple of 4.
+__device__ __forceinline__ void store_partial(const Block32& block, float* partial, bool vec, int64_t m0, int rows,
+                                              int64_t n0, int64_t n1, int64_t N, int lane) {
+  if (vec) {
+    const int c = (lane & 7) * 4;
+    if (n0 + c >= n1) return;
+    float* out = partial + m0 * N + n0 + c;
+#pragma unroll
+    for (int r = lane >> 3; r < 32; r += 4) {
+      float z[4];
+      block.get<4>(r, c, z);
+      if (r < rows) *reinterpret_cast<float4*>(out + r * N) = make_float4(z[0], z[1], z[2], z[3]);
+    }
+  } else {
+    if (n0 + lane >= n1) return;
+    float* out = partial + m0 * N + n0 + lane;
+    for (int r = 0; r < rows; ++r) out[r * N] = block.get1(r, lane);
+  }
 }
 
 }  // namespace nnue_ls

@@ -12,7 +12,7 @@
 // One persistent block per SM (or a pair of blocks on two SMs, CG = 2, sharing
 // a 256-row tile: each holds half of A's rows and half of B's, which halves
 // what is read from L2 per product).  Warp 0 copies tiles by TMA into a ring
-// of shared-memory stages, warp 1 issues the products into TMEM, warps 4-11
+// of shared-memory stages, warp 1 issues the products into TMEM, warps 4-19
 // read finished accumulators back while the next tile's products run.
 #pragma once
 
@@ -23,8 +23,9 @@
 
 namespace nnue_ls {
 
-constexpr int kGemmThreads = 384;
-constexpr int kEpilogueWarp0 = 4, kEpilogueWarps = 8;
+constexpr int kEpilogueWarp0 = 4, kEpilogueWarps = 16;
+constexpr int kGemmThreads = 32 * (kEpilogueWarp0 + kEpilogueWarps);
+constexpr int kColumnGroups = kEpilogueWarps / 4;  // a warp reaches a quarter of the accumulators' lanes
 constexpr int kTileM = 128;          // rows of C per block
 constexpr uint64_t kWaitLimitNs = 4000000000ull;
 
@@ -37,8 +38,8 @@ struct GemmShape {
   static constexpr int kRowsB = kMaxBN / CG;                         // rows of B held by one block
   static constexpr int kPlaneA = kTileM * kBK * 2, kPlaneB = kRowsB * kBK * 2;
   static constexpr int kStage = PLANES * (kPlaneA + kPlaneB);
-  static constexpr int kStages = PLANES == 1 ? (CG == 1 ? 4 : 6) : 4;
-  static constexpr int kTranspose = kEpilogueWarps * 32 * 33 * 4;
+  static constexpr int kStages = PLANES == 1 && CG == 2 ? 5 : 3;
+  static constexpr int kTranspose = kEpilogueWarps * 32 * 32 * 4;
   static constexpr int kSmem = 1024 + kStages * kStage + kTranspose + 256;
   // k blocks summed in TMEM before the epilogue warps take the sum into
   // registers.  The tensor cores' running sums lose up to a unit of the last
@@ -48,7 +49,6 @@ struct GemmShape {
 };
 
 struct GemmParams {
-  CUtensorMap a, b;  // [planes][rows][columns], the contiguous direction first
   int64_t M, N;
   int32_t k_blocks, splits;      // k blocks in all; pieces the k range is cut into
   int32_t m_tiles, n_tiles, bn;  // bn: columns of C per tile, a multiple of 16
@@ -96,7 +96,8 @@ __device__ __forceinline__ uint64_t global_ns() {
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
   if (mbar_try(bar, parity)) return true;
   const uint64_t t0 = global_ns();
-  while (!mbar_try(bar, parity)) {
+  for (uint32_t i = 1; !mbar_try(bar, parity); ++i) {
+    if (i % 16) continue;
     if (*gave_up) return false;
     if (global_ns() - t0 > kWaitLimitNs) {
       *gave_up = 1;
@@ -180,21 +181,21 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 __device__ __forceinline__ void tcgen_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 lanes x 32 columns of accumulators: this thread's lane, 32 columns.
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// 32 lanes x 16 columns of accumulators: this thread's lane, 16 columns.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float* v) {
+  uint32_t r[16];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr)
       : "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // Shared-memory operand descriptors.  K-major: rows of BK values, 8-row groups
@@ -209,16 +210,20 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int mn_major) {
   return (uint64_t)((addr & 0x3ffff) >> 4) | (lbo >> 4) << 16 | (sbo >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
 }
 
+// map_a, map_b: [planes][rows][columns], the contiguous direction first.  They are parameters of their own because
+// their address is taken: parameters whose address is not are read as constants.
 // ---- the kernel -----------------------------------------------------------------
 template <typename T, int CG>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const GemmParams p) {
   constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
   using S = GemmShape<PLANES, CG>;
   constexpr int BK = S::kBK;
   extern __shared__ uint8_t smem_raw[];
   // the same offset in both blocks of a pair: the dynamic shared memory starts at the same address there
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  float* transpose = reinterpret_cast<float*>(smem + S::kStages * S::kStage);
+  float4* transpose = reinterpret_cast<float4*>(smem + S::kStages * S::kStage);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStage + S::kTranspose);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S::kStages;
   const uint32_t acc_full0 = empty0 + 8 * S::kStages, acc_empty0 = acc_full0 + 16;
@@ -272,15 +277,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         for (int q = 0; q < PLANES; ++q) {
           if (p.a_mn) {
             for (int i = 0; i < kTileM / 64; ++i)
-              tma_load<CG>(sa + q * S::kPlaneA + i * 64 * BK * 2, &p.a, m0 + 64 * i, k * BK, q, bar);
+              tma_load<CG>(sa + q * S::kPlaneA + i * 64 * BK * 2, &map_a, m0 + 64 * i, k * BK, q, bar);
           } else {
-            tma_load<CG>(sa + q * S::kPlaneA, &p.a, k * BK, m0, q, bar);
+            tma_load<CG>(sa + q * S::kPlaneA, &map_a, k * BK, m0, q, bar);
           }
           if (p.b_mn) {
             for (int i = 0; i < blocks_b; ++i)
-              tma_load<CG>(sb + q * S::kPlaneB + i * 64 * BK * 2, &p.b, n0 + 64 * i, k * BK, q, bar);
+              tma_load<CG>(sb + q * S::kPlaneB + i * 64 * BK * 2, &map_b, n0 + 64 * i, k * BK, q, bar);
           } else {
-            tma_load<CG>(sb + q * S::kPlaneB, &p.b, k * BK, n0, q, bar);
+            tma_load<CG>(sb + q * S::kPlaneB, &map_b, k * BK, n0, q, bar);
           }
         }
         if (++stage == S::kStages) stage = 0, phase ^= 1;
@@ -335,9 +340,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       }
     }
   } else if (warp >= kEpilogueWarp0) {
-    // ---- epilogue: warp's quarter of the lanes, every second block of 32 columns ----
-    const int quarter = warp & 3, half = (warp - kEpilogueWarp0) >> 2;
-    float* stage = transpose + (warp - kEpilogueWarp0) * 32 * 33;
+    // ---- epilogue: warp's quarter of the lanes, every fourth block of 32 columns ----
+    const int quarter = warp & 3, group = (warp - kEpilogueWarp0) >> 2;
+    const int64_t M = p.M, N = p.N;
+    Block32 block{transpose + (warp - kEpilogueWarp0) * 256};
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const int col_blocks = (p.bn + 31) / 32;
     uint32_t chunk = 0;
@@ -346,24 +352,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       const int64_t tile = item % tiles;
       const int split = (int)(item / tiles);
       const int64_t m0 = (tile / p.n_tiles) * (kTileM * CG) + rank * kTileM + quarter * 32;
-      const int64_t n0 = (tile % p.n_tiles) * p.bn, n1 = min(p.N, n0 + p.bn);
-      float* partial = p.splits > 1 ? p.partial + (int64_t)split * p.M * p.N : nullptr;
+      const int64_t n0 = (tile % p.n_tiles) * p.bn, n1 = min(N, n0 + p.bn);
+      const int rows = (int)max((int64_t)0, min((int64_t)32, M - m0));
+      float* partial = p.splits > 1 ? p.partial + (int64_t)split * M * N : nullptr;
       auto finish = [&](int cb, const float (&v)[32]) {
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) stage[lane * 33 + j] = v[j];
-        __syncwarp();
-        if (partial) store_partial(stage, partial, m0, p.M, n0 + cb * 32, n1, p.N, lane);
-        else store_block<T>(stage, p.e, m0, p.M, n0 + cb * 32, n1, p.N, lane);
+        block.put(v, lane);
+        if (partial) store_partial(block, partial, N % 4 == 0, m0, rows, n0 + cb * 32, n1, N, lane);
+        else store_block<T>(block, p.e, m0, rows, n0 + cb * 32, n1, N, lane);
       };
+      if (p.e.residual && !partial && lane < rows) {
+        // the residual's rows come from HBM while the tile's products run
+        const char* r = reinterpret_cast<const char*>(static_cast<const T*>(p.e.residual) + (m0 + lane) * p.e.ldr);
+        for (int cb = group; cb < col_blocks; cb += kColumnGroups)
+          if (n0 + cb * 32 < n1) prefetch_l2(r + (n0 + cb * 32) * sizeof(T));
+      }
       if constexpr (S::kChunk == 0) {
         const uint32_t acc = chunk & 1;
         if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk >> 1) & 1, gave_up))) break;
         tcgen_fence_after();
-        for (int cb = half; cb < col_blocks; cb += 2) {
+        for (int cb = group; cb < col_blocks; cb += kColumnGroups) {
           float v[32];
-          tmem_load32(lanes + acc * 256 + cb * 32, v);
-          if (cb + 2 >= col_blocks) {  // this warp's last read: the accumulator may be written again
+          tmem_load16(lanes + acc * 256 + cb * 32, v);
+          tmem_load16(lanes + acc * 256 + cb * 32 + 16, v + 16);
+          if (cb + kColumnGroups >= col_blocks) {  // this warp's last read: the accumulator may be written again
             tcgen_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -373,13 +384,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           }
           finish(cb, v);
         }
-        if (half >= col_blocks && lane == 0) {  // a narrow tile leaves this warp nothing to read
+        if (group >= col_blocks && lane == 0) {  // a narrow tile leaves this warp nothing to read
           if constexpr (CG == 1) mbar_arrive(acc_empty0 + 8 * acc);
           else mbar_arrive_leader(acc_empty0 + 8 * acc);
         }
         ++chunk;
       } else {
-        constexpr int kMine = S::kMaxBN / 64;  // column blocks of 32 per warp
+        constexpr int kMine = S::kMaxBN / (32 * kColumnGroups);  // column blocks of 32 per warp
         float sum[kMine][32];
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
@@ -393,12 +404,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           tcgen_fence_after();
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
-            const int cb = half + 2 * i;
+            const int cb = group + kColumnGroups * i;
             if (cb < col_blocks) {
-              float v[32];
-              tmem_load32(lanes + acc * 256 + cb * 32, v);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sum[i][j] += v[j];
+              for (int h = 0; h < 32; h += 16) {
+                float v[16];
+                tmem_load16(lanes + acc * 256 + cb * 32 + h, v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sum[i][h + j] += v[j];
+              }
             }
           }
           tcgen_fence_before();
@@ -411,7 +425,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
-          if (half + 2 * i < col_blocks) finish(half + 2 * i, sum[i]);
+          if (group + kColumnGroups * i < col_blocks) finish(group + kColumnGroups * i, sum[i]);
       }
     }
   }

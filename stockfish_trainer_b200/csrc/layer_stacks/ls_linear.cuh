@@ -60,11 +60,6 @@ __device__ __forceinline__ void store_operand(void* dst, int64_t at, int64_t pla
   }
 }
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V) VecT {
-  T v[V];
-};
-
 // [rows, cols] with row stride ld -> rows of ldo (a multiple of 8) values in
 // the products' layout; a thread moves 8 values.
 template <typename T, bool VEC>
@@ -165,7 +160,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / groups, n = (i - m * groups) * V;
     float z[V] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) {
       const auto t = *reinterpret_cast<const VecT<float, V>*>(partial + s * MN + m * N + n);
 #pragma unroll
@@ -174,14 +169,16 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     VecT<T, V> out, res;
     VecT<Code, V> d;
     if (e.residual) res = *reinterpret_cast<const VecT<T, V>*>(static_cast<const T*>(e.residual) + m * e.ldr + n);
+    with_activation(e.act, [&](auto act) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (e.bias) z[j] += load_mixed<T>(e.bias, n + j, e.bias_f32);
-      float dv, o = activate<T>(z[j], e.act, dv);
-      if (e.residual) o += to_f(res.v[j]);
-      out.v[j] = from_f<T>(o);
-      d.v[j] = D::encode(dv);
-    }
+      for (int j = 0; j < V; ++j) {
+        if (e.bias) z[j] += load_mixed<T>(e.bias, n + j, e.bias_f32);
+        float dv, o = activate<T, decltype(act)::value>(z[j], dv);
+        if (e.residual) o += to_f(res.v[j]);
+        out.v[j] = from_f<T>(o);
+        d.v[j] = D::encode(dv);
+      }
+    });
     *reinterpret_cast<VecT<T, V>*>(static_cast<T*>(e.out) + m * N + n) = out;
     if (e.act_grad) *reinterpret_cast<VecT<Code, V>*>(static_cast<Code*>(e.act_grad) + m * N + n) = d;
   }

@@ -109,7 +109,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, int planes) {
 }
 
 template <typename T, int CG>
-int launch_gemm_cg(const GemmParams& p, cudaStream_t s) {
+int launch_gemm_cg(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, cudaStream_t s) {
   using S = GemmShape<sizeof(T) == 4 ? 3 : 1, CG>;
   static std::atomic<uint64_t> ready{0};  // one bit per device: the kernel may use S::kSmem there
   int dev = 0;
@@ -133,7 +133,7 @@ int launch_gemm_cg(const GemmParams& p, cudaStream_t s) {
   cfg.attrs = &cluster;
   cfg.numAttrs = CG == 1 ? 0 : 1;
   count_launch();
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, CG>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, CG>, a, b, p);
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "gemm: %s", cudaGetErrorString(e));
 }
 
@@ -145,8 +145,9 @@ int launch_gemm(const Operand& a, const Operand& b, int64_t M, int64_t N, const 
   constexpr int bk = planes == 1 ? 64 : 32;
   constexpr bool is_f16 = std::is_same<T, f16>::value;
   GemmParams p;
-  if (int rc = make_map(&p.a, a, planes, is_f16, bk, kTileM)) return rc;
-  if (int rc = make_map(&p.b, b, planes, is_f16, bk, t.bn / t.cg)) return rc;
+  CUtensorMap map_a, map_b;
+  if (int rc = make_map(&map_a, a, planes, is_f16, bk, kTileM)) return rc;
+  if (int rc = make_map(&map_b, b, planes, is_f16, bk, t.bn / t.cg)) return rc;
   p.M = M;
   p.N = N;
   p.k_blocks = t.k_blocks;
@@ -165,7 +166,7 @@ int launch_gemm(const Operand& a, const Operand& b, int64_t M, int64_t N, const 
   auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   e.vec = N % V == 0 && aligned(e.out) && aligned(e.act_grad) && aligned(e.residual) && (!e.residual || e.ldr % V == 0);
   p.e = e;
-  if (int rc = t.cg == 1 ? launch_gemm_cg<T, 1>(p, s) : launch_gemm_cg<T, 2>(p, s)) return rc;
+  if (int rc = t.cg == 1 ? launch_gemm_cg<T, 1>(map_a, map_b, p, s) : launch_gemm_cg<T, 2>(map_a, map_b, p, s)) return rc;
   if (t.splits > 1) {
     const int64_t total = e.vec ? M * N / 4 : M * N;
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total, 256), kNumSMs * 16);

@@ -34,7 +34,8 @@ constexpr uint64_t kWaitLimitNs = 4000000000ull;
 template <int PLANES, int CG>
 struct GemmShape {
   static constexpr int kBK = PLANES == 1 ? 64 : 32;
-  static constexpr int kMaxBN = PLANES == 3 && CG == 1 ? 128 : 256;  // columns of C per tile
+  static constexpr int kMaxBN = PLANES == 3 && CG == 1 ? 128 : 256;   // columns of C per tile
+  static constexpr int kAccs = 512 / kMaxBN;                          // accumulators that TMEM holds
   static constexpr int kRowsB = kMaxBN / CG;                         // rows of B held by one block
   static constexpr int kPlaneA = kTileM * kBK * 2, kPlaneB = kRowsB * kBK * 2;
   static constexpr int kStage = PLANES * (kPlaneA + kPlaneB);
@@ -226,9 +227,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   float4* transpose = reinterpret_cast<float4*>(smem + S::kStages * S::kStage);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStage + S::kTranspose);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S::kStages;
-  const uint32_t acc_full0 = empty0 + 8 * S::kStages, acc_empty0 = acc_full0 + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 4);
+  const uint32_t acc_full0 = empty0 + 8 * S::kStages, acc_empty0 = acc_full0 + 8 * S::kAccs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * (S::kStages + S::kAccs));
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  EpilogueParams* epilogue = reinterpret_cast<EpilogueParams*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 1 ? 0 : (int)cluster_rank();
@@ -237,11 +239,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kAccs; ++i) {
       mbar_init(acc_full0 + 8 * i, 1);
       mbar_init(acc_empty0 + 8 * i, kEpilogueWarps * CG);
     }
     *gave_up = 0;
+    *epilogue = p.e;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async;" ::: "memory");
   }
@@ -308,8 +311,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int k0 = (int)((int64_t)p.k_blocks * split / p.splits), k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
       const int per_chunk = S::kChunk ? S::kChunk : k1 - k0;
       for (int kc = k0; kc < k1 && ok; kc += per_chunk, ++chunk) {
-        const uint32_t acc = chunk & 1, d = tmem + acc * 256;
-        if (!(ok = mbar_wait(acc_empty0 + 8 * acc, ((chunk >> 1) & 1) ^ 1, gave_up))) break;
+        const uint32_t acc = chunk % S::kAccs, d = tmem + acc * S::kMaxBN;
+        if (!(ok = mbar_wait(acc_empty0 + 8 * acc, ((chunk / S::kAccs) & 1) ^ 1, gave_up))) break;
         tcgen_fence_after();
         uint32_t accumulate = 0;
         for (int k = kc; k < min(kc + per_chunk, k1); ++k) {
@@ -358,6 +361,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       auto finish = [&](int cb, const float (&v)[32]) {
         block.put(v, lane);
         if (partial) store_partial(block, partial, N % 4 == 0, m0, rows, n0 + cb * 32, n1, N, lane);
+        else if constexpr (PLANES == 3) store_block_f32(block.s, epilogue, m0, rows, n0 + cb * 32, n1, N, lane);
         else store_block<T>(block, p.e, m0, rows, n0 + cb * 32, n1, N, lane);
       };
       if (p.e.residual && !partial && lane < rows) {
@@ -367,13 +371,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           if (n0 + cb * 32 < n1) prefetch_l2(r + (n0 + cb * 32) * sizeof(T));
       }
       if constexpr (S::kChunk == 0) {
-        const uint32_t acc = chunk & 1;
-        if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk >> 1) & 1, gave_up))) break;
+        const uint32_t acc = chunk % S::kAccs;
+        if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
         tcgen_fence_after();
         for (int cb = group; cb < col_blocks; cb += kColumnGroups) {
           float v[32];
-          tmem_load16(lanes + acc * 256 + cb * 32, v);
-          tmem_load16(lanes + acc * 256 + cb * 32 + 16, v + 16);
+          tmem_load16(lanes + acc * S::kMaxBN + cb * 32, v);
+          tmem_load16(lanes + acc * S::kMaxBN + cb * 32 + 16, v + 16);
           if (cb + kColumnGroups >= col_blocks) {  // this warp's last read: the accumulator may be written again
             tcgen_fence_before();
             __syncwarp();
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         ++chunk;
       } else {
-        constexpr int kMine = S::kMaxBN / (32 * kColumnGroups);  // column blocks of 32 per warp
+        constexpr int kMine = S::kMaxBN / (32 * kColumnGroups);  // column blocks per warp
         float sum[kMine][32];
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
@@ -399,8 +403,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int k0 = (int)((int64_t)p.k_blocks * split / p.splits),
                   k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
         for (int kc = k0; kc < k1; kc += S::kChunk, ++chunk) {
-          const uint32_t acc = chunk & 1;
-          if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk >> 1) & 1, gave_up))) break;
+          const uint32_t acc = chunk % S::kAccs;
+          if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
           tcgen_fence_after();
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
               for (int h = 0; h < 32; h += 16) {
                 float v[16];
-                tmem_load16(lanes + acc * 256 + cb * 32 + h, v);
+                tmem_load16(lanes + acc * S::kMaxBN + cb * 32 + h, v);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) sum[i][h + j] += v[j];
               }

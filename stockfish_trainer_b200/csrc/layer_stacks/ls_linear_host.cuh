@@ -213,7 +213,7 @@ template <typename T>
 ForwardPlan plan_forward(const nnue_ls_linear& a) {
   ForwardPlan p{};
   p.tiles = plan_tiles(a.rows, a.outputs, a.inputs, sizeof(T) == 4 ? 3 : 1);
-  p.x = needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+  p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
   p.w = needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
   p.partial = p.tiles.partial_bytes(a.rows, a.outputs);
   p.total = p.x + p.w + p.partial;
@@ -223,7 +223,7 @@ ForwardPlan plan_forward(const nnue_ls_linear& a) {
 template <typename T>
 int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   const ForwardPlan p = plan_forward<T>(a);
-  const Operand x = operand<T>(a.x, a.ldx, a.rows, a.inputs, false, ws, s);
+  const Operand x = operand<T>(a.x, a.ldx, a.rows, a.inputs, false, a.x_packed ? a.x_packed : ws, s);
   const Operand w = operand<T>(a.weight, a.ldw, a.outputs, a.inputs, false, ws + p.x, s);
   EpilogueParams e{a.bias, a.residual, a.out, a.act_grad, a.ldr, a.activation, a.bias_dtype == NNUE_LS_F32, false};
   return launch_gemm<T>(x, w, a.rows, a.outputs, p.tiles, e, ws + p.x + p.w, s);
@@ -250,7 +250,7 @@ BackwardPlan plan_backward(const nnue_ls_linear& a) {
   }
   if (a.grad_weight) {
     p.dw = plan_tiles(a.outputs, a.inputs, a.rows, planes);
-    p.x = needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+    p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
     p.partial = std::max(p.partial, p.dw.partial_bytes(a.outputs, a.inputs));
   }
   p.dz_written = products && (a.activation != NNUE_LS_ACT_NONE || needs_pack<T>(a.grad_out, a.ldg, a.rows));
@@ -306,7 +306,8 @@ int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   }
   if (a.grad_weight) {  // dW = dz^T x: k runs over the rows
     e.out = a.grad_weight;
-    const Operand b = operand<T>(a.x, a.ldx, a.rows, a.inputs, true, x, s);
+    const Operand b = a.x_packed ? Operand{a.x_packed, a.inputs, a.rows, round8(a.inputs), true}
+                                 : operand<T>(a.x, a.ldx, a.rows, a.inputs, true, x, s);
     d.mn_major = true;
     if (int rc = launch_gemm<T>(d, b, a.outputs, a.inputs, p.dw, e, partial, s)) return rc;
   }

@@ -170,6 +170,14 @@ int nnue_ls_device_errors(uint32_t* flags, int clear) {
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
 
+size_t nnue_ls_linear_packed_size(const nnue_ls_linear* a) {
+  if (check_linear("linear_packed_size", a) || a->rows == 0) return 0;
+  return with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    return needs_pack<T>(a->x, a->ldx, a->rows) ? pack_bytes<T>(a->rows, a->inputs) : (size_t)0;
+  });
+}
+
 size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear* a) {
   if (check_linear("linear_forward", a) || a->rows == 0) return 0;
   return with_type(a->dtype, [&](auto t) { return plan_forward<decltype(t)>(*a).total; });
@@ -181,8 +189,12 @@ int nnue_ls_linear_forward(const nnue_ls_linear* a, void* workspace, size_t work
   if (!a->x || !a->weight || !a->out) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: null pointer");
   if (a->ldx < a->inputs || a->ldw < a->inputs || (a->residual && a->ldr < a->outputs))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: row stride below the row length");
+  if (reinterpret_cast<uintptr_t>(a->x_packed) % 256)
+    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed not 256-byte aligned");
   return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
+    if (a->x_packed && !needs_pack<T>(a->x, a->ldx, a->rows))
+      return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed given for an x that is not packed");
     if (int rc = check_workspace("linear_forward", workspace, workspace_bytes, plan_forward<T>(*a).total)) return rc;
     return linear_forward<T>(*a, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
@@ -197,9 +209,9 @@ int nnue_ls_linear_backward(const nnue_ls_linear* a, void* workspace, size_t wor
   if (int rc = check_linear("linear_backward", a)) return rc;
   if (a->rows > 0) {
     if (!a->grad_out || (a->activation != NNUE_LS_ACT_NONE && !a->act_grad) || (a->grad_x && !a->weight) ||
-        (a->grad_weight && !a->x))
+        (a->grad_weight && !a->x && !a->x_packed))
       return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_backward: null pointer");
-    if (a->ldg < a->outputs || (a->grad_x && a->ldw < a->inputs) || (a->grad_weight && a->ldx < a->inputs))
+    if (a->ldg < a->outputs || (a->grad_x && a->ldw < a->inputs) || (a->grad_weight && !a->x_packed && a->ldx < a->inputs))
       return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_backward: row stride below the row length");
   }
   return with_type(a->dtype, [&](auto t) {

@@ -32,16 +32,19 @@ def _args(x, weight, bias, residual, act):
     return a
 
 
-def _forward(x, weight, bias, residual, act, want_act_grad):
+def _forward(x, weight, bias, residual, act, want_act_grad=False, keep_packed=False):
     a = _args(x, weight, bias, residual, act)
     out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
     a.out = out.data_ptr()
-    act_grad = None
+    act_grad = packed = None
     if want_act_grad and act:
         act_grad = torch.empty_like(out)
         a.act_grad = act_grad.data_ptr()
+    if keep_packed:
+        packed = _native.packed_buffer(a, x.device)
+        a.x_packed = _native.ptr(packed)
     _native.run("nnue_ls_linear_forward", a, x.device)
-    return out, act_grad
+    return out, act_grad, packed
 
 
 class LinearActFunction(torch.autograd.Function):
@@ -49,32 +52,45 @@ class LinearActFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        out, act_grad = _forward(x, weight, bias, residual, act, True)
-        ctx.save_for_backward(x, weight, bias, act_grad)
-        ctx.act = act
+        need_w = ctx.needs_input_grad[1]
+        out, act_grad, packed = _forward(x, weight, bias, residual, act, True, need_w)
+        # the packed form serves the backward in x's place
+        ctx.save_for_backward(x if packed is None and need_w else None, packed, weight, bias, act_grad)
+        ctx.meta = (act, x.shape, x.dtype)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        x, weight, bias, act_grad = ctx.saved_tensors
+        x, packed, weight, bias, act_grad = ctx.saved_tensors
+        act, x_shape, dtype = ctx.meta
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         grad_x = grad_w = grad_b = None
         if need_x or need_w or need_b:
             g = _native.rows_of(grad_out)
-            a = _args(x, weight, bias, None, ctx.act)
+            dev = g.device
+            a = _native.Linear()
+            a.rows, a.inputs = x_shape
+            a.outputs = weight.shape[0]
+            a.dtype = _native.DTYPES[dtype]
+            a.bias_dtype = a.dtype if bias is None else _native.DTYPES[bias.dtype]
+            a.activation = act
+            if x is not None:
+                a.x, a.ldx = x.data_ptr(), _native.row_stride(x)
+            a.x_packed = _native.ptr(packed)
+            a.weight, a.ldw = weight.data_ptr(), _native.row_stride(weight)
             a.grad_out, a.ldg = g.data_ptr(), _native.row_stride(g)
             a.act_grad = _native.ptr(act_grad)
             if need_x:
-                grad_x = torch.empty(a.rows, a.inputs, dtype=x.dtype, device=x.device)
+                grad_x = torch.empty(x_shape, dtype=dtype, device=dev)
                 a.grad_x = grad_x.data_ptr()
             if need_w:
-                grad_w = torch.empty(a.outputs, a.inputs, dtype=x.dtype, device=x.device)
+                grad_w = torch.empty(weight.shape, dtype=dtype, device=dev)
                 a.grad_weight = grad_w.data_ptr()
             if need_b:
                 grad_b = torch.empty_like(bias)
                 a.grad_bias = grad_b.data_ptr()
-            _native.run("nnue_ls_linear_backward", a, x.device)
+            _native.run("nnue_ls_linear_backward", a, dev)
         return grad_x, grad_w, grad_b, grad_out if need_r else None, None
 
 
@@ -92,8 +108,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     non-finite fp32 operand may turn an infinite sum into NaN.  Rows may be
     strided; other layouts are copied.
 
-    The backward keeps ``x``, ``weight`` and the activation's derivative (in
-    the output's type); it is differentiable once.
+    For the backward ``x`` (in the form its products read: for fp32 1.5 times
+    its size), ``weight`` and the activation's derivative (as wide as the
+    output) are kept; it is differentiable once.
     """
     _native.check_tensor(x, "x")
     dev, dt = x.device, x.dtype
@@ -123,5 +140,5 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if _native.needs_grad(x, weight, bias, residual):
         out = LinearActFunction.apply(x, weight, bias, residual, _ACT[activation])
     else:
-        out = _forward(x, weight, bias, residual, _ACT[activation], False)[0]
+        out = _forward(x, weight, bias, residual, _ACT[activation])[0]
     return out if len(shape) == 2 else out.view(shape)

@@ -13,10 +13,12 @@ is compiled without it: its sums are not tied to a reference order.
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -50,15 +52,8 @@ def _stale(lib: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _compile(lib: str, sources: list[str], flags: list[str], verbose: bool) -> str:
-    tmp = lib + ".tmp"
-    cmd = [
-        nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", *flags,
-        "-Xcompiler", "-fPIC,-O3,-pthread", "-shared",
-        "-I", INCLUDE,
-        *sources,
-        "-o", tmp, "-lpthread",
-    ]
+def _nvcc(args: list[str], verbose: bool) -> None:
+    cmd = [nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O3,-pthread", "-I", INCLUDE, *args]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -66,22 +61,32 @@ def _compile(lib: str, sources: list[str], flags: list[str], verbose: bool) -> s
         raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
     if verbose:
         sys.stderr.write(res.stderr)
-    os.replace(tmp, lib)
-    return lib
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     deps = [os.path.join(CSRC, d) for d in DEPS] + [os.path.join(INCLUDE, "nnue_ft.h")]
     if not force and not _stale(LIB_PATH, deps):
         return LIB_PATH
-    return _compile(LIB_PATH, [os.path.join(CSRC, s) for s in SOURCES], ["-fmad=false"], verbose)
+    tmp = LIB_PATH + ".tmp"
+    _nvcc(["-fmad=false", "-shared", *(os.path.join(CSRC, s) for s in SOURCES), "-o", tmp, "-lpthread"], verbose)
+    os.replace(tmp, LIB_PATH)
+    return LIB_PATH
 
 
 def build_layer_stacks(force: bool = False, verbose: bool = False) -> str:
     deps = [os.path.join(LS_CSRC, d) for d in sorted(os.listdir(LS_CSRC)) if d.endswith((".cu", ".cuh"))]
     if not force and not _stale(LS_LIB_PATH, deps + [os.path.join(INCLUDE, "nnue_ls.h")]):
         return LS_LIB_PATH
-    return _compile(LS_LIB_PATH, [os.path.join(LS_CSRC, "nnue_ls.cu")], [], verbose)
+    sources = sorted(d for d in os.listdir(LS_CSRC) if d.endswith(".cu"))
+    tmp = LS_LIB_PATH + ".tmp"
+    with tempfile.TemporaryDirectory() as objects:  # one nvcc per source file, side by side
+        outs = [os.path.join(objects, s + ".o") for s in sources]
+        with concurrent.futures.ThreadPoolExecutor(len(sources)) as pool:
+            list(pool.map(lambda so: _nvcc(["-c", os.path.join(LS_CSRC, so[0]), "-o", so[1]], verbose),
+                          zip(sources, outs)))
+        _nvcc(["-shared", *outs, "-o", tmp, "-lpthread"], verbose)
+    os.replace(tmp, LS_LIB_PATH)
+    return LS_LIB_PATH
 
 
 if __name__ == "__main__":

@@ -1,0 +1,12 @@
+// The linear layer on fp32 tensors.
+#include "ls_linear_host.cuh"
+
+namespace nnue_ls {
+template size_t linear_packed_bytes<float>(const nnue_ls_linear&);
+template size_t linear_forward_bytes<float>(const nnue_ls_linear&);
+template int linear_forward<float>(const nnue_ls_linear&, char*, cudaStream_t);
+template size_t linear_backward_bytes<float>(const nnue_ls_linear&);
+template int linear_backward<float>(const nnue_ls_linear&, char*, cudaStream_t);
+template bool linear_packs_x<float>(const nnue_ls_linear&);
+template cudaError_t linear_device_errors<float>(unsigned*, bool);
+}  // namespace nnue_ls

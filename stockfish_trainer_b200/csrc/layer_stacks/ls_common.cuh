@@ -1,5 +1,5 @@
 // Shared helpers of the layer-stack kernels (sm_100a): element types, warp and
-// block sums, the sticky device error word.  One translation unit (nnue_ls.cu).
+// block sums, the sticky device error word (one per source file that uses it).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -13,12 +13,22 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kNumSMs = 148;
 
 // Sticky flags raised by kernels instead of hanging or faulting.
-__device__ unsigned int g_device_errors = 0;
+static __device__ unsigned int g_device_errors = 0;
 enum : unsigned {
   kErrWaitTimeout = 1u,  // a matrix kernel's wait on its own copies or products ran out
   kErrBadIndex = 2u,     // route backward: a chosen index outside [-1, experts) was skipped
 };
 __device__ __forceinline__ void flag_error(unsigned e) { atomicOr(&g_device_errors, e); }
+
+// Adds this file's word to *flags; clears it on demand.  Synchronises.
+static inline cudaError_t read_device_errors(unsigned* flags, bool clear) {
+  unsigned v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_errors, sizeof(v));
+  *flags |= v;
+  const unsigned zero = 0;
+  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(g_device_errors, &zero, sizeof(zero));
+  return e;
+}
 
 using bf16 = __nv_bfloat16;
 using f16 = __half;

@@ -258,7 +258,7 @@ __device__ __forceinline__ void store_block(const Block32& block, const Epilogue
 // inlined, 561 us called).  The 16-bit kernels hold no sums and are faster
 // inlined (143 us called, 133 us inlined).  `shared`: the parameters' copy in
 // shared memory.
-__device__ __noinline__ void store_block_f32(float4* block, const EpilogueParams* shared, int64_t m0, int rows,
+static __device__ __noinline__ void store_block_f32(float4* block, const EpilogueParams* shared, int64_t m0, int rows,
                                              int64_t n0, int64_t n1, int64_t N, int lane) {
   store_block<float>(Block32{block}, *shared, m0, rows, n0, n1, N, lane);
 }

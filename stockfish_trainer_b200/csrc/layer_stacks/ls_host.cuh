@@ -4,40 +4,26 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-#include <cstdarg>
-#include <cstdio>
-
 #include "../../../include/nnue_ls.h"
+#include "ls_common.cuh"
 
 namespace nnue_ls {
-namespace {
 
-thread_local char g_last_error[512];
-std::atomic<unsigned long long> g_launches{0};
-
-inline void count_launch(unsigned n = 1) { g_launches.fetch_add(n, std::memory_order_relaxed); }
-
+// One per library (nnue_ls.cu).
+void count_launch();
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
-  va_end(ap);
-  return code;
-}
+int check_launch(const char* what);  // the last launch's error, if any
 
-int check_launch(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
+namespace {
 
 constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-bool bad_dtype(int t) { return t < NNUE_LS_F32 || t > NNUE_LS_F16; }
+constexpr int64_t kMaxDim = (1 << 30) - 1;
 
-int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
+inline bool bad_dtype(int t) { return t < NNUE_LS_F32 || t > NNUE_LS_F16; }
+
+inline int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
   if (need == 0) return NNUE_LS_OK;
   if (!ws || have < need)
     return fail(NNUE_LS_ERR_WORKSPACE, "%s: workspace has %zu bytes, needs %zu", what, ws ? have : (size_t)0, need);
@@ -55,4 +41,28 @@ auto with_type(int dtype, const F& fn) {
 }
 
 }  // namespace
+
+// The operators' entry points per element type, each compiled in a file of its
+// own (linear_*.cu, norm_*.cu), and the device error words of those files.
+template <typename T>
+size_t linear_packed_bytes(const nnue_ls_linear& a);
+template <typename T>
+size_t linear_forward_bytes(const nnue_ls_linear& a);
+template <typename T>
+int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s);
+template <typename T>
+size_t linear_backward_bytes(const nnue_ls_linear& a);
+template <typename T>
+int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s);
+template <typename T>
+bool linear_packs_x(const nnue_ls_linear& a);
+template <typename T>
+cudaError_t linear_device_errors(unsigned* flags, bool clear);
+template <typename T>
+int norm_forward(const nnue_ls_norm& a, cudaStream_t s);
+template <typename T>
+size_t norm_backward_bytes(const nnue_ls_norm& a);
+template <typename T>
+int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s);
+
 }  // namespace nnue_ls

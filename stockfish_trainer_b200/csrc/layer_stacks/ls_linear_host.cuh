@@ -220,6 +220,23 @@ ForwardPlan plan_forward(const nnue_ls_linear& a) {
   return p;
 }
 
+}  // namespace
+
+template <typename T>
+bool linear_packs_x(const nnue_ls_linear& a) {
+  return needs_pack<T>(a.x, a.ldx, a.rows);
+}
+
+template <typename T>
+size_t linear_packed_bytes(const nnue_ls_linear& a) {
+  return linear_packs_x<T>(a) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+}
+
+template <typename T>
+size_t linear_forward_bytes(const nnue_ls_linear& a) {
+  return plan_forward<T>(a).total;
+}
+
 template <typename T>
 int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   const ForwardPlan p = plan_forward<T>(a);
@@ -230,6 +247,8 @@ int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
 }
 
 // ---- backward --------------------------------------------------------------------
+namespace {
+
 struct BackwardPlan {
   TilePlan dx, dw;
   int64_t parts, rows_per_part;  // the bias sum's row ranges
@@ -267,6 +286,13 @@ BackwardPlan plan_backward(const nnue_ls_linear& a) {
   p.bias = a.grad_bias ? align256((size_t)p.parts * a.outputs * 4) : 0;
   p.total = p.dz + p.x + p.w + p.bias + p.partial;
   return p;
+}
+
+}  // namespace
+
+template <typename T>
+size_t linear_backward_bytes(const nnue_ls_linear& a) {
+  return plan_backward<T>(a).total;
 }
 
 template <typename T>
@@ -314,5 +340,9 @@ int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   return check_launch("linear_backward");
 }
 
-}  // namespace
+template <typename T>
+cudaError_t linear_device_errors(unsigned* flags, bool clear) {
+  return read_device_errors(flags, clear);
+}
+
 }  // namespace nnue_ls

@@ -17,7 +17,7 @@ struct NormParams {
   const void *x, *f, *gate;
   const void *post_weight, *post_bias, *scale, *pre_weight, *pre_bias;  // [width]; null = absent
   void *y, *h;
-  float4* stats;  // per row: mean and 1/std of f, mean and 1/std of y
+  float4* stats;  // per row: mean of f and its variance + eps; the same of y
   const void *grad_y, *grad_h;
   void *grad_x, *grad_f, *grad_gate;
   float* partial;  // backward: [blocks, 5, width] column sums (post_weight, post_bias, scale, pre_weight, pre_bias)
@@ -65,10 +65,10 @@ struct NormRow {
   }
 };
 
-// Mean (layer norm) and 1/std of a row whose element c is value(c).
+// Mean (layer norm) and variance + eps of a row whose element c is value(c).
 template <bool CENTER, typename F>
 __device__ __forceinline__ void row_stats(const F& value, int width, float eps, float* scratch, float& mean,
-                                          float& rstd) {
+                                          float& var) {
   float v[1];
   mean = 0.f;
   if (CENTER) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ void row_stats(const F& value, int width, float eps, 
     v[0] += d * d;
   }
   block_sum(v, scratch);
-  rstd = rsqrtf(v[0] / width + eps);
+  var = v[0] / width + eps;
 }
 
 // One block per row, any width; the row is read again for each pass.
@@ -92,10 +92,12 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
   __shared__ float scratch[32];
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     NormRow<T> r(p, row);
-    float mean_y = 0.f, rstd_y = 1.f;
+    float mean_y = 0.f, var_f = 1.f, var_y = 1.f;
     if (p.f && p.post_weight)
-      row_stats<CENTER>([&](int c) { return to_f(r.f[c]); }, p.width, p.eps, scratch, r.mean_f, r.rstd_f);
-    if (p.pre_weight) row_stats<CENTER>([&](int c) { return r.y(c); }, p.width, p.eps, scratch, mean_y, rstd_y);
+      row_stats<CENTER>([&](int c) { return to_f(r.f[c]); }, p.width, p.eps, scratch, r.mean_f, var_f);
+    r.rstd_f = __frsqrt_rn(var_f);
+    if (p.pre_weight) row_stats<CENTER>([&](int c) { return r.y(c); }, p.width, p.eps, scratch, mean_y, var_y);
+    const float rstd_y = __frsqrt_rn(var_y);
     for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
       const float y = r.y(c);
       if (p.y) static_cast<T*>(p.y)[row * p.width + c] = from_f<T>(y);
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
         static_cast<T*>(p.h)[row * p.width + c] = from_f<T>(h);
       }
     }
-    if (p.stats && threadIdx.x == 0) p.stats[row] = make_float4(r.mean_f, r.rstd_f, mean_y, rstd_y);
+    if (p.stats && threadIdx.x == 0) p.stats[row] = make_float4(r.mean_f, var_f, mean_y, var_y);
   }
 }
 
@@ -115,6 +117,8 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
 //   df = rstd_f * (v - mean(v) - f_hat * mean(v * f_hat)),      v = gate * d * post_weight
 // and, summed over rows: post_weight += gate * d * f_hat, post_bias += gate * d, scale += d * x,
 // pre_weight += dh * y_hat, pre_bias += dh.
+// The products with y_hat and f_hat are formed as (y - mean) * (mean(u * (y - mean)) / (var + eps)): the two terms
+// of a difference that can cancel then share fewer roundings.
 // y is formed again from x, f and the gate: x has to be read for the scale's gradient anyway, and the y that the
 // forward wrote is rounded to 16 bits, which would show in the fp32 sums.
 // Each block owns a slice of `partial` and each thread its columns of it.
@@ -131,26 +135,27 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
     NormRow<T> r(p, row);
     const float4 st = p.stats[row];
     r.mean_f = st.x;
-    r.rstd_f = st.y;
+    r.rstd_f = __frsqrt_rn(st.y);
+    const float rstd_y = __frsqrt_rn(st.w);
     const T* gy = static_cast<const T*>(p.grad_y) + (p.grad_y ? row * W : 0);
     const T* gh = static_cast<const T*>(p.grad_h) + (p.grad_h ? row * W : 0);
     const bool pre = p.grad_h && p.pre_weight;
-    auto y_hat = [&](int c) { return (r.y(c) - st.z) * st.w; };
+    auto y_cen = [&](int c) { return r.y(c) - st.z; };
     float s[2] = {0.f, 0.f};
     if (pre) {
       for (int c = threadIdx.x; c < W; c += blockDim.x) {
         const float u = to_f(gh[c]) * r.param(p.pre_weight, c);
-        s[0] += u * y_hat(c);
+        s[0] += u * y_cen(c);
         if (CENTER) s[1] += u;
       }
       block_sum(s, scratch);
     }
-    const float c1 = s[0] * inv, c2 = s[1] * inv;
+    const float c1 = s[0] * inv / st.w, c2 = s[1] * inv;
     auto d_of = [&](int c) {
       float d = p.grad_y ? to_f(gy[c]) : 0.f;
       if (pre) {
         const float u = to_f(gh[c]) * r.param(p.pre_weight, c);
-        d += st.w * (u - c2 - y_hat(c) * c1);
+        d += rstd_y * (u - c2 - y_cen(c) * c1);
       }
       return d;
     };
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
         const float d = d_of(c);
         if (p.post_weight) {
           const float v = r.gate(c) * d * r.param(p.post_weight, c);
-          q[0] += v * r.f_hat(c);
+          q[0] += v * (to_f(r.f[c]) - st.x);
           if (CENTER) q[1] += v;
         }
         if (p.gate_mode == kGateRow) q[2] += d * r.branch(c);
@@ -173,7 +178,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
       q[1] = t[1];
       q[2] = t2[0];
     }
-    const float c3 = q[0] * inv, c4 = q[1] * inv;
+    const float c3 = q[0] * inv / st.y, c4 = q[1] * inv;
     for (int c = threadIdx.x; c < W; c += blockDim.x) {
       const float d = d_of(c);
       const int64_t o = row * W + c;
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
         gn = gate * d;
         if (p.grad_f) {
           float df = gn;
-          if (p.post_weight) df = r.rstd_f * (gn * r.param(p.post_weight, c) - c4 - r.f_hat(c) * c3);
+          if (p.post_weight) df = r.rstd_f * (gn * r.param(p.post_weight, c) - c4 - (to_f(r.f[c]) - st.x) * c3);
           static_cast<T*>(p.grad_f)[o] = from_f<T>(df);
         }
         if (p.grad_gate && p.gate_mode == kGateFull) {
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
         }
         if (p.f && p.scale) part[2 * W + c] += d * to_f(r.x[c]);
         if (pre) {
-          part[3 * W + c] += to_f(gh[c]) * y_hat(c);
+          part[3 * W + c] += to_f(gh[c]) * (y_cen(c) * rstd_y);
           if (p.pre_bias) part[4 * W + c] += to_f(gh[c]);
         }
       }
@@ -213,24 +218,422 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
   }
 }
 
-// Totals of the backward's column sums over blocks, in block order within each
-// of a block's 8 rows of threads; out[i] null = not wanted.
+// ---- rows held in registers -----------------------------------------------------
+// The kernels above read a row once per pass, for any width.  Up to 2048 columns
+// the ones below read it once: a block works on R rows at a time and a thread
+// keeps NV * V = 4 columns of them in registers (V = 4 neighbouring ones, or 4
+// single ones where rows are not aligned).  A thread's columns are the same in
+// every row, so the parameters are read once and the sums over rows are plain
+// registers until the block's last row; R rows share each barrier, and with
+// PREFETCH the next R rows are on their way meanwhile.
+
+// V values of a row at column c.
+template <typename T, int V>
+struct RowVec {
+  struct alignas(sizeof(T) * V) Raw {
+    T v[V];
+  };
+  Raw raw;
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    raw = *reinterpret_cast<const Raw*>(static_cast<const T*>(base) + at);
+  }
+  __device__ __forceinline__ float operator[](int i) const { return to_f(raw.v[i]); }
+};
+template <typename T, int V>
+__device__ __forceinline__ void store_row(void* base, int64_t at, const float (&v)[V]) {
+  typename RowVec<T, V>::Raw o;
+#pragma unroll
+  for (int i = 0; i < V; ++i) o.v[i] = from_f<T>(v[i]);
+  *reinterpret_cast<typename RowVec<T, V>::Raw*>(static_cast<T*>(base) + at) = o;
+}
+// V values of a parameter; `absent` where there is none.
+template <typename T, int V>
+__device__ __forceinline__ void load_param(const void* p, int c, bool f32, float absent, float (&v)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = absent;
+  } else if (f32) {
+    if constexpr (V >= 4) {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const float4 t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + i));
+        v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = __ldg(static_cast<const float*>(p) + c + i);
+    }
+  } else {
+    RowVec<T, V> t;
+    t.load(p, c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = t[i];
+  }
+}
+
+// Sums K values (a power of two) over the block; every thread gets the totals.
+// Within a warp each step of the exchange halves the number of values a lane
+// carries; between warps the sums meet in shared memory, taken in warp order.
+// Two halves of `scratch` in turn make one barrier enough.
+template <int K>
+struct BlockSum {
+  static constexpr int kSpan = 32 / K;  // neighbouring lanes that end with the same value
+  float* scratch;                       // 2 * 32 * K floats
+  int turn = 0;
+  __device__ __forceinline__ void operator()(float (&v)[K]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int o = 16;
+#pragma unroll
+    for (int n = K; n > 1; n /= 2) {
+#pragma unroll
+      for (int i = 0; i < n / 2; ++i) {
+        const bool upper = lane & o;
+        const float send = upper ? v[i] : v[i + n / 2], keep = upper ? v[i + n / 2] : v[i];
+        v[i] = keep + __shfl_xor_sync(kFull, send, o);
+      }
+      o /= 2;
+    }
+    float sum = v[0];
+#pragma unroll
+    for (int q = kSpan / 2; q > 0; q /= 2) sum += __shfl_xor_sync(kFull, sum, q);
+    if (warps > 1) {
+      float* s = scratch + turn * 32 * K;
+      turn ^= 1;
+      const int k = lane / kSpan, sub = lane % kSpan;
+      if (sub == 0) s[warp * K + k] = sum;
+      __syncthreads();
+      sum = 0.f;
+      for (int w = sub; w < warps; w += kSpan) sum += s[w * K + k];
+#pragma unroll
+      for (int q = kSpan / 2; q > 0; q /= 2) sum += __shfl_xor_sync(kFull, sum, q);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = __shfl_sync(kFull, sum, k * kSpan);
+  }
+};
+
+__host__ __device__ constexpr int pow2_at_least(int n) { return n <= 1 ? 1 : 2 * pow2_at_least((n + 1) / 2); }
+
+// This thread's columns of the rows under work.
+template <typename T, int V>
+struct Columns {
+  static constexpr int kNV = 4 / V;
+  __device__ __forceinline__ static int at(int i) { return ((int)threadIdx.x + i * (int)blockDim.x) * V; }
+  RowVec<T, V> raw[kNV];
+  __device__ __forceinline__ void load(const void* base, int64_t row, int width) {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i)
+      if (at(i) < width) raw[i].load(base, row * width + at(i));
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) raw[i].raw.v[j] = from_f<T>(0.f);
+  }
+  __device__ __forceinline__ float operator[](int k) const { return to_f(raw[k / V].raw.v[k % V]); }
+  __device__ __forceinline__ static void store(void* base, int64_t row, int width, const float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i)
+      if (at(i) < width) {
+        float t[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = v[i * V + j];
+        store_row<T, V>(base, row * width + at(i), t);
+      }
+  }
+  __device__ __forceinline__ static void params(const void* p, int width, bool f32, float absent, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      float t[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[j] = 0.f;
+      if (at(i) < width) load_param<T, V>(p, at(i), f32, absent, t);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i * V + j] = t[j];
+    }
+  }
+};
+
+// The rows of one round: loads skip what the call does not have (then zero).
+template <typename T, int V, bool FULL, bool BACKWARD>
+struct RowIn {
+  Columns<T, V> x, f, g, gy, gh;
+  float4 st;
+  float gate;
+  __device__ __forceinline__ void init() {
+    x.zero(), f.zero(), g.zero(), gy.zero(), gh.zero();
+    st = make_float4(0.f, 1.f, 0.f, 1.f);
+    gate = 0.f;
+  }
+  __device__ __forceinline__ void load(const NormParams& p, int64_t row) {
+    if (row >= p.rows) {  // adds nothing to any sum
+      init();
+      return;
+    }
+    x.load(p.x, row, p.width);
+    if (p.f) f.load(p.f, row, p.width);
+    if (FULL) g.load(p.gate, row, p.width);
+    gate = !p.f ? 0.f : p.gate_mode == kGateRow ? load_mixed<T>(p.gate, row, p.gate_f32) : 1.f;
+    if (BACKWARD) {
+      if (p.grad_y) gy.load(p.grad_y, row, p.width);
+      if (p.grad_h) gh.load(p.grad_h, row, p.width);
+      st = p.stats[row];
+    }
+  }
+  // the row's gate, or this column's
+  __device__ __forceinline__ float gate_at(const NormParams& p, float row_gate, int k) const {
+    if (!FULL) return row_gate;
+    return p.gate_sigmoid ? sigmoid(g[k]) : g[k];
+  }
+  __device__ __forceinline__ float row_gate(const NormParams& p) const {
+    return p.gate_mode == kGateRow && p.gate_sigmoid ? sigmoid(gate) : gate;
+  }
+};
+
+template <typename T, int V, int R, bool CENTER, bool FULL, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(const NormParams p) {
+  using C = Columns<T, V>;
+  __shared__ float scratch[2 * 32 * R];
+  BlockSum<R> total{scratch};
+  const int W = p.width;
+  const float inv = 1.f / W;
+  bool mine[4];  // columns inside the row
+#pragma unroll
+  for (int k = 0; k < 4; ++k) mine[k] = C::at(k / V) < W;
+  float w[4], b[4], sc[4], pw[4], pb[4];
+  C::params(p.post_weight, W, p.params_f32, 1.f, w);
+  C::params(p.post_bias, W, p.params_f32, 0.f, b);
+  C::params(p.scale, W, p.params_f32, p.scale_value, sc);
+  C::params(p.pre_weight, W, p.params_f32, 1.f, pw);
+  C::params(p.pre_bias, W, p.params_f32, 0.f, pb);
+  RowIn<T, V, FULL, false> in[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) in[r].init();
+  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < p.rows; row0 += (int64_t)gridDim.x * R) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) in[r].load(p, row0 + r);
+    float4 st[R];
+    float s[R], y[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) st[r] = make_float4(0.f, 1.f, 0.f, 1.f);
+    if (p.post_weight) {
+      if (CENTER) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = (in[r].f[0] + in[r].f[1]) + (in[r].f[2] + in[r].f[3]);
+        total(s);
+#pragma unroll
+        for (int r = 0; r < R; ++r) st[r].x = s[r] * inv;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        s[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float d = in[r].f[k] - st[r].x;
+          if (mine[k]) s[r] += d * d;
+        }
+      }
+      total(s);
+#pragma unroll
+      for (int r = 0; r < R; ++r) st[r].y = s[r] * inv + p.eps;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float row_gate = in[r].row_gate(p), rstd = __frsqrt_rn(st[r].y);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float n = (in[r].f[k] - st[r].x) * rstd * w[k] + b[k];
+        y[r][k] = p.f ? sc[k] * in[r].x[k] + in[r].gate_at(p, row_gate, k) * n : in[r].x[k];
+      }
+      if (p.f && row0 + r < p.rows) C::store(p.y, row0 + r, W, y[r]);
+    }
+    if (p.h) {
+      if (CENTER) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          s[r] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (mine[k]) s[r] += y[r][k];
+        }
+        total(s);
+#pragma unroll
+        for (int r = 0; r < R; ++r) st[r].z = s[r] * inv;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        s[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float d = y[r][k] - st[r].z;
+          if (mine[k]) s[r] += d * d;
+        }
+      }
+      total(s);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        st[r].w = s[r] * inv + p.eps;
+        const float rstd = __frsqrt_rn(st[r].w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[r][k] = (y[r][k] - st[r].z) * rstd * pw[k] + pb[k];
+        if (row0 + r < p.rows) C::store(p.h, row0 + r, W, y[r]);
+      }
+    }
+    if (p.stats && threadIdx.x == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row0 + r < p.rows) p.stats[row0 + r] = st[r];
+    }
+  }
+}
+
+template <typename T, int V, int R, bool CENTER, bool FULL, bool PREFETCH, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_backward_rows_kernel(const NormParams p) {
+  using C = Columns<T, V>;
+  constexpr int N1 = CENTER ? 2 : 1, N2 = CENTER ? 3 : 2, K1 = R * N1, K2 = pow2_at_least(R * N2);
+  __shared__ float scratch[2 * 32 * (K1 + K2)];
+  BlockSum<K1> total1{scratch};
+  BlockSum<K2> total2{scratch + 2 * 32 * K1};
+  const int W = p.width;
+  const float inv = 1.f / W;
+  const bool pre = p.grad_h && p.pre_weight;
+  float w[4], b[4], sc[4], pw[4], acc[5][4] = {};
+  C::params(p.post_weight, W, p.params_f32, 1.f, w);
+  C::params(p.post_bias, W, p.params_f32, 0.f, b);
+  C::params(p.scale, W, p.params_f32, p.scale_value, sc);
+  C::params(p.pre_weight, W, p.params_f32, 0.f, pw);
+  RowIn<T, V, FULL, true> in[R], next[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    in[r].init();
+    if (PREFETCH) {
+      next[r].init();
+      next[r].load(p, (int64_t)blockIdx.x * R + r);
+    }
+  }
+  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < p.rows; row0 += (int64_t)gridDim.x * R) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (PREFETCH) {
+        in[r] = next[r];
+        next[r].load(p, row0 + (int64_t)gridDim.x * R + r);
+      } else {
+        in[r].load(p, row0 + r);
+      }
+    }
+    float row_gate[R], rstd_f[R], rstd_y[R], d[R][4], s[K1];  // d: y - mean, then the gradient of y
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      row_gate[r] = in[r].row_gate(p);
+      rstd_f[r] = __frsqrt_rn(in[r].st.y);
+      rstd_y[r] = __frsqrt_rn(in[r].st.w);
+    }
+    if (pre) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float y = in[r].x[k];
+          if (p.f) {
+            const float n = (in[r].f[k] - in[r].st.x) * rstd_f[r] * w[k] + b[k];
+            y = sc[k] * y + in[r].gate_at(p, row_gate[r], k) * n;
+          }
+          const float yc = y - in[r].st.z, gh = in[r].gh[k], u = gh * pw[k];
+          d[r][k] = yc;
+          s0 += u * yc;
+          if (CENTER) s1 += u;
+          acc[3][k] += gh * (yc * rstd_y[r]);
+          acc[4][k] += gh;
+        }
+        s[r * N1] = s0;
+        if (CENTER) s[r * N1 + 1] = s1;
+      }
+      total1(s);
+    }
+    float q[K2];
+#pragma unroll
+    for (int i = R * N2; i < K2; ++i) q[i] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float c1 = pre ? s[r * N1] * inv / in[r].st.w : 0.f, c2 = CENTER && pre ? s[r * N1 + CENTER] * inv : 0.f;
+      float dx[4], q0 = 0.f, q1 = 0.f, q2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float v = in[r].gy[k];
+        if (pre) v += rstd_y[r] * (in[r].gh[k] * pw[k] - c2 - d[r][k] * c1);
+        d[r][k] = v;
+        dx[k] = p.f ? sc[k] * v : v;
+        const float gn = in[r].gate_at(p, row_gate[r], k) * v, fc = in[r].f[k] - in[r].st.x, fh = fc * rstd_f[r],
+                    vw = gn * w[k];
+        q0 += vw * fc;
+        if (CENTER) q1 += vw;
+        q2 += v * (fh * w[k] + b[k]);
+        acc[0][k] += gn * fh;
+        acc[1][k] += gn;
+        acc[2][k] += v * in[r].x[k];
+      }
+      q[r * N2] = q0;
+      q[r * N2 + 1] = q2;
+      if (CENTER) q[r * N2 + 2] = q1;
+      if (p.grad_x && row0 + r < p.rows) C::store(p.grad_x, row0 + r, W, dx);
+    }
+    if (!p.f) continue;
+    total2(q);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= p.rows) break;
+      const float c3 = p.post_weight ? q[r * N2] * inv / in[r].st.y : 0.f, c4 = CENTER && p.post_weight ? q[r * N2 + 2 * CENTER] * inv : 0.f;
+      float df[4], dg[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float gate = in[r].gate_at(p, row_gate[r], k), fc = in[r].f[k] - in[r].st.x;
+        df[k] = rstd_f[r] * (gate * d[r][k] * w[k] - c4 - fc * c3);
+        if (FULL) {
+          dg[k] = d[r][k] * (fc * rstd_f[r] * w[k] + b[k]);
+          if (p.gate_sigmoid) dg[k] *= gate * (1.f - gate);
+        }
+      }
+      if (p.grad_f) C::store(p.grad_f, row0 + r, W, df);
+      if (FULL) {
+        if (p.grad_gate) C::store(p.grad_gate, row0 + r, W, dg);
+      } else if (p.grad_gate && threadIdx.x == 0) {
+        const float g = row_gate[r], dq = q[r * N2 + 1];
+        store_mixed<T>(p.grad_gate, row0 + r, p.gate_f32, p.gate_sigmoid ? dq * g * (1.f - g) : dq);
+      }
+    }
+  }
+  if (!p.partial) return;
+  float* part = p.partial + (int64_t)blockIdx.x * 5 * W;
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = C::at(k / V) + k % V;
+      if (C::at(k / V) < W) part[i * W + c] = acc[i][k];
+    }
+}
+
+// Totals of the backward's column sums over blocks: 32 rows of threads take
+// every 32nd block, then their sums are added in turn; out[i] null = not wanted.
 struct NormTotals {
   void* out[5];
 };
 template <typename T>
-__global__ void __launch_bounds__(256) norm_totals_kernel(const float* __restrict__ partial, int blocks, int width,
-                                                          NormTotals t, bool out_f32) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) norm_totals_kernel(const float* __restrict__ partial, int blocks, int width,
+                                                           NormTotals t, bool out_f32) {
+  __shared__ float red[32][33];
   const int which = blockIdx.y, c = blockIdx.x * 32 + threadIdx.x;
   if (!t.out[which]) return;
   float sum = 0.f;
   if (c < width)
-    for (int b = threadIdx.y; b < blocks; b += 8) sum += partial[((int64_t)b * 5 + which) * width + c];
+#pragma unroll 4
+    for (int b = threadIdx.y; b < blocks; b += 32) sum += partial[((int64_t)b * 5 + which) * width + c];
   red[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.y == 0 && c < width) {
-    for (int i = 1; i < 8; ++i) sum += red[i][threadIdx.x];
+    for (int i = 1; i < 32; ++i) sum += red[i][threadIdx.x];
     store_mixed<T>(t.out[which], c, out_f32, sum);
   }
 }

@@ -1,24 +1,43 @@
 // C ABI of the layer-stack operators for B200 (sm_100a).
 // Declarations and contracts: include/nnue_ls.h.
 //
-// One translation unit: the kernels live in the *.cuh files included here.
+// Checks of arguments, and the router; the linear layer and the norms are
+// compiled per element type in files of their own.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
+#include <cstdarg>
+#include <cstdio>
 
 #include "../../../include/nnue_ls.h"
 #include "ls_common.cuh"
 #include "ls_host.cuh"
-#include "ls_linear_host.cuh"
-#include "ls_norm.cuh"
 #include "ls_route.cuh"
 
 namespace nnue_ls {
-namespace {
 
-constexpr int64_t kMaxDim = (1 << 30) - 1;
+static thread_local char g_last_error[512];
+static std::atomic<unsigned long long> g_launches{0};
+
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int check_launch(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+namespace {
 
 // ---- linear ----------------------------------------------------------------
 int check_linear(const char* what, const nnue_ls_linear* a) {
@@ -29,7 +48,7 @@ int check_linear(const char* what, const nnue_ls_linear* a) {
     return fail(NNUE_LS_ERR_UNSUPPORTED, "%s: sizes must be below 2^30", what);
   if (bad_dtype(a->dtype) || (a->bias_dtype != a->dtype && a->bias_dtype != NNUE_LS_F32))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: bad element type", what);
-  if (a->activation < 0 || a->activation >= kActivations)
+  if (a->activation < 0 || a->activation > NNUE_LS_ACT_GELU)
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, a->activation);
   return NNUE_LS_OK;
 }
@@ -45,52 +64,17 @@ int check_norm(const char* what, const nnue_ls_norm* a) {
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: bad element type", what);
   if (a->kind != NNUE_LS_NORM_RMS && a->kind != NNUE_LS_NORM_LAYER)
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: unknown norm kind %d", what, a->kind);
-  if (a->gate_mode < kGateNone || a->gate_mode > kGateFull)
+  if (a->gate_mode < NNUE_LS_GATE_NONE || a->gate_mode > NNUE_LS_GATE_FULL)
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: unknown gate mode %d", what, a->gate_mode);
-  if (a->rows > 0 && !a->f && (a->gate_mode != kGateNone || a->post_weight || a->scale))
+  if (a->rows > 0 && !a->f && (a->gate_mode != NNUE_LS_GATE_NONE || a->post_weight || a->scale))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: a gate, scale or norm after the block needs f", what);
   if ((a->post_bias && !a->post_weight) || (a->pre_bias && !a->pre_weight))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: a norm's bias needs its weight", what);
   if (!(a->eps >= 0.f)) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", what);
-  if (a->rows > 0 && (!a->x || (a->gate_mode != kGateNone && !a->gate)))
+  if (a->rows > 0 && (!a->x || (a->gate_mode != NNUE_LS_GATE_NONE && !a->gate)))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   return NNUE_LS_OK;
 }
-
-NormParams norm_params(const nnue_ls_norm& a) {
-  NormParams p{};
-  p.x = a.x;
-  p.f = a.f;
-  p.gate = a.gate;
-  p.post_weight = a.post_weight;
-  p.post_bias = a.post_bias;
-  p.scale = a.scale;
-  p.pre_weight = a.pre_weight;
-  p.pre_bias = a.pre_bias;
-  p.y = a.y;
-  p.h = a.h;
-  p.stats = reinterpret_cast<float4*>(a.stats);
-  p.grad_y = a.grad_y;
-  p.grad_h = a.grad_h;
-  p.grad_x = a.grad_x;
-  p.grad_f = a.grad_f;
-  p.grad_gate = a.grad_gate;
-  p.rows = a.rows;
-  p.width = a.width;
-  p.scale_value = a.scale_value;
-  p.eps = a.eps;
-  p.gate_mode = a.gate_mode;
-  p.gate_sigmoid = a.gate_sigmoid != 0;
-  p.gate_f32 = a.gate_dtype == NNUE_LS_F32;
-  p.params_f32 = a.params_dtype == NNUE_LS_F32;
-  return p;
-}
-
-bool wants_params(const nnue_ls_norm& a) {
-  return a.grad_post_weight || a.grad_post_bias || a.grad_scale || a.grad_pre_weight || a.grad_pre_bias;
-}
-
-int64_t norm_backward_blocks(const nnue_ls_norm& a) { return std::min<int64_t>(std::max<int64_t>(a.rows, 1), kNumSMs * 4); }
 
 // ---- route -------------------------------------------------------------------
 int check_route(const char* what, const nnue_ls_route* a) {
@@ -164,23 +148,24 @@ uint64_t nnue_ls_launch_count(void) { return g_launches.load(); }
 int nnue_ls_device_errors(uint32_t* flags, int clear) {
   if (!flags) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "device_errors: null pointer");
   cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(flags, g_device_errors, sizeof(*flags));
-  const unsigned zero = 0;
-  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbol(g_device_errors, &zero, sizeof(zero));
+  *flags = 0;
+  if (e == cudaSuccess) e = linear_device_errors<float>(flags, clear != 0);
+  if (e == cudaSuccess) e = linear_device_errors<bf16>(flags, clear != 0);
+  if (e == cudaSuccess) e = linear_device_errors<f16>(flags, clear != 0);
+  if (e == cudaSuccess) e = read_device_errors(flags, clear != 0);
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
 
 size_t nnue_ls_linear_packed_size(const nnue_ls_linear* a) {
   if (check_linear("linear_packed_size", a) || a->rows == 0) return 0;
   return with_type(a->dtype, [&](auto t) {
-    using T = decltype(t);
-    return needs_pack<T>(a->x, a->ldx, a->rows) ? pack_bytes<T>(a->rows, a->inputs) : (size_t)0;
+    return linear_packed_bytes<decltype(t)>(*a);
   });
 }
 
 size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear* a) {
   if (check_linear("linear_forward", a) || a->rows == 0) return 0;
-  return with_type(a->dtype, [&](auto t) { return plan_forward<decltype(t)>(*a).total; });
+  return with_type(a->dtype, [&](auto t) { return linear_forward_bytes<decltype(t)>(*a); });
 }
 
 int nnue_ls_linear_forward(const nnue_ls_linear* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -193,16 +178,16 @@ int nnue_ls_linear_forward(const nnue_ls_linear* a, void* workspace, size_t work
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed not 256-byte aligned");
   return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (a->x_packed && !needs_pack<T>(a->x, a->ldx, a->rows))
+    if (a->x_packed && !linear_packs_x<T>(*a))
       return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed given for an x that is not packed");
-    if (int rc = check_workspace("linear_forward", workspace, workspace_bytes, plan_forward<T>(*a).total)) return rc;
+    if (int rc = check_workspace("linear_forward", workspace, workspace_bytes, linear_forward_bytes<T>(*a))) return rc;
     return linear_forward<T>(*a, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
 }
 
 size_t nnue_ls_linear_backward_workspace_size(const nnue_ls_linear* a) {
   if (check_linear("linear_backward", a)) return 0;
-  return with_type(a->dtype, [&](auto t) { return plan_backward<decltype(t)>(*a).total; });
+  return with_type(a->dtype, [&](auto t) { return linear_backward_bytes<decltype(t)>(*a); });
 }
 
 int nnue_ls_linear_backward(const nnue_ls_linear* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -216,7 +201,7 @@ int nnue_ls_linear_backward(const nnue_ls_linear* a, void* workspace, size_t wor
   }
   return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (int rc = check_workspace("linear_backward", workspace, workspace_bytes, plan_backward<T>(*a).total)) return rc;
+    if (int rc = check_workspace("linear_backward", workspace, workspace_bytes, linear_backward_bytes<T>(*a))) return rc;
     return linear_backward<T>(*a, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
 }
@@ -226,21 +211,13 @@ int nnue_ls_norm_forward(const nnue_ls_norm* a, void* stream) {
   if (a->rows == 0) return NNUE_LS_OK;
   if ((a->f && !a->y) || (a->pre_weight && !a->h) || (a->h && !a->pre_weight))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "norm_forward: null pointer, or h without pre_weight");
-  const NormParams p = norm_params(*a);
-  const unsigned grid = (unsigned)std::min<int64_t>(a->rows, kNumSMs * 8);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  with_type(a->dtype, [&](auto t) {
-    using T = decltype(t);
-    count_launch();
-    if (a->kind == NNUE_LS_NORM_LAYER) norm_forward_kernel<T, true><<<grid, 256, 0, s>>>(p);
-    else norm_forward_kernel<T, false><<<grid, 256, 0, s>>>(p);
-  });
-  return check_launch("norm_forward");
+  return with_type(a->dtype,
+                   [&](auto t) { return norm_forward<decltype(t)>(*a, static_cast<cudaStream_t>(stream)); });
 }
 
 size_t nnue_ls_norm_backward_workspace_size(const nnue_ls_norm* a) {
-  if (check_norm("norm_backward", a) || !wants_params(*a)) return 0;
-  return align256((size_t)norm_backward_blocks(*a) * 5 * a->width * 4);
+  if (check_norm("norm_backward", a)) return 0;
+  return with_type(a->dtype, [&](auto t) { return norm_backward_bytes<decltype(t)>(*a); });
 }
 
 int nnue_ls_norm_backward(const nnue_ls_norm* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -248,26 +225,11 @@ int nnue_ls_norm_backward(const nnue_ls_norm* a, void* workspace, size_t workspa
   if (a->rows > 0 && !a->stats) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "norm_backward: null pointer");
   if (a->rows > 0 && !a->f && (a->grad_f || a->grad_gate || a->grad_post_weight || a->grad_post_bias || a->grad_scale))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "norm_backward: gradients of a branch that is absent");
-  if (int rc = check_workspace("norm_backward", workspace, workspace_bytes, nnue_ls_norm_backward_workspace_size(a)))
-    return rc;
-  NormParams p = norm_params(*a);
-  const bool params = wants_params(*a);
-  p.partial = params ? static_cast<float*>(workspace) : nullptr;
-  const unsigned grid = (unsigned)norm_backward_blocks(*a);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  with_type(a->dtype, [&](auto t) {
+  return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    count_launch();
-    if (a->kind == NNUE_LS_NORM_LAYER) norm_backward_kernel<T, true><<<grid, 256, 0, s>>>(p);
-    else norm_backward_kernel<T, false><<<grid, 256, 0, s>>>(p);
-    if (params) {
-      const NormTotals out{{a->grad_post_weight, a->grad_post_bias, a->grad_scale, a->grad_pre_weight, a->grad_pre_bias}};
-      count_launch();
-      norm_totals_kernel<T><<<dim3((unsigned)ceil_div(a->width, 32), 5), dim3(32, 8), 0, s>>>(
-          p.partial, (int)grid, a->width, out, p.params_f32);
-    }
+    if (int rc = check_workspace("norm_backward", workspace, workspace_bytes, norm_backward_bytes<T>(*a))) return rc;
+    return norm_backward<T>(*a, workspace, static_cast<cudaStream_t>(stream));
   });
-  return check_launch("norm_backward");
 }
 
 size_t nnue_ls_route_forward_workspace_size(const nnue_ls_route* a) {

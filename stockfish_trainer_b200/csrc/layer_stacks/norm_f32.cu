@@ -1,0 +1,8 @@
+// The norms around a residual block on fp32 tensors.
+#include "ls_norm_host.cuh"
+
+namespace nnue_ls {
+template int norm_forward<float>(const nnue_ls_norm&, cudaStream_t);
+template size_t norm_backward_bytes<float>(const nnue_ls_norm&);
+template int norm_backward<float>(const nnue_ls_norm&, void*, cudaStream_t);
+}  // namespace nnue_ls

@@ -43,7 +43,7 @@ auto with_type(int dtype, const F& fn) {
 }  // namespace
 
 // The operators' entry points per element type, each compiled in a file of its
-// own (linear_*.cu, norm_*.cu), and the device error words of those files.
+// own (linear_*.cu, norm_*.cu; route.cu), and the device error words of those files.
 template <typename T>
 size_t linear_packed_bytes(const nnue_ls_linear& a);
 template <typename T>
@@ -64,5 +64,11 @@ template <typename T>
 size_t norm_backward_bytes(const nnue_ls_norm& a);
 template <typename T>
 int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s);
+size_t route_forward_bytes(const nnue_ls_route& a);
+template <typename T>
+int route_forward(const nnue_ls_route& a, void* workspace, cudaStream_t s);
+template <typename T>
+int route_backward(const nnue_ls_route& a, cudaStream_t s);
+cudaError_t route_device_errors(unsigned* flags, bool clear);
 
 }  // namespace nnue_ls

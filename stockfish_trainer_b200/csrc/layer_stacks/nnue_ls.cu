@@ -1,8 +1,7 @@
 // C ABI of the layer-stack operators for B200 (sm_100a).
 // Declarations and contracts: include/nnue_ls.h.
 //
-// Checks of arguments, and the router; the linear layer and the norms are
-// compiled per element type in files of their own.
+// Checks of arguments; the operators are compiled in files of their own.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -15,7 +14,6 @@
 #include "../../../include/nnue_ls.h"
 #include "ls_common.cuh"
 #include "ls_host.cuh"
-#include "ls_route.cuh"
 
 namespace nnue_ls {
 
@@ -90,48 +88,6 @@ int check_route(const char* what, const nnue_ls_route* a) {
   return NNUE_LS_OK;
 }
 
-int64_t route_blocks(const nnue_ls_route& a) {
-  return std::min<int64_t>(std::max<int64_t>(1, ceil_div(a.rows, 8)), kNumSMs * 2);
-}
-
-RouteParams route_params(const nnue_ls_route& a) {
-  RouteParams r{};
-  r.logits = a.logits;
-  r.valid = a.valid;
-  r.indices = a.indices;
-  r.gates = a.gates;
-  r.counts = a.counts;
-  r.loss = a.loss;
-  r.unit = a.loss + 1;
-  r.grad_gates = a.grad_gates;
-  r.grad_loss = a.grad_loss;
-  r.grad_logits = a.grad_logits;
-  r.rows = a.rows;
-  r.ld = a.ld;
-  r.experts = a.experts;
-  r.k = a.k;
-  r.blocks = (int)route_blocks(a);
-  r.renormalize = a.renormalize != 0;
-  return r;
-}
-
-template <typename T>
-void launch_route(const RouteParams& r, bool backward, cudaStream_t s) {
-  count_launch();
-#define NNUE_LS_ROUTE(V)                                                      \
-  if (r.experts <= 32 * V) {                                                  \
-    if (backward) route_backward_kernel<T, V><<<r.blocks, 256, 0, s>>>(r);    \
-    else route_forward_kernel<T, V><<<r.blocks, 256, 0, s>>>(r);              \
-    return;                                                                   \
-  }
-  NNUE_LS_ROUTE(1)
-  NNUE_LS_ROUTE(2)
-  NNUE_LS_ROUTE(4)
-  NNUE_LS_ROUTE(8)
-  NNUE_LS_ROUTE(32)
-#undef NNUE_LS_ROUTE
-}
-
 }  // namespace
 }  // namespace nnue_ls
 
@@ -152,7 +108,7 @@ int nnue_ls_device_errors(uint32_t* flags, int clear) {
   if (e == cudaSuccess) e = linear_device_errors<float>(flags, clear != 0);
   if (e == cudaSuccess) e = linear_device_errors<bf16>(flags, clear != 0);
   if (e == cudaSuccess) e = linear_device_errors<f16>(flags, clear != 0);
-  if (e == cudaSuccess) e = read_device_errors(flags, clear != 0);
+  if (e == cudaSuccess) e = route_device_errors(flags, clear != 0);
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
 
@@ -233,31 +189,22 @@ int nnue_ls_norm_backward(const nnue_ls_norm* a, void* workspace, size_t workspa
 }
 
 size_t nnue_ls_route_forward_workspace_size(const nnue_ls_route* a) {
-  if (check_route("route_forward", a)) return 0;
-  return align256((size_t)route_blocks(*a) * (2 * a->experts + 1) * 4);
+  return check_route("route_forward", a) ? 0 : route_forward_bytes(*a);
 }
 
 int nnue_ls_route_forward(const nnue_ls_route* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_route("route_forward", a)) return rc;
-  if (int rc = check_workspace("route_forward", workspace, workspace_bytes, nnue_ls_route_forward_workspace_size(a)))
-    return rc;
-  RouteParams r = route_params(*a);
-  r.partial_p = static_cast<float*>(workspace);
-  r.partial_count = reinterpret_cast<int32_t*>(r.partial_p + (int64_t)r.blocks * r.experts);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  with_type(a->dtype, [&](auto t) { launch_route<decltype(t)>(r, false, s); });
-  count_launch();
-  route_totals_kernel<<<1, 256, 0, s>>>(r);
-  return check_launch("route_forward");
+  if (int rc = check_workspace("route_forward", workspace, workspace_bytes, route_forward_bytes(*a))) return rc;
+  return with_type(
+      a->dtype, [&](auto t) { return route_forward<decltype(t)>(*a, workspace, static_cast<cudaStream_t>(stream)); });
 }
 
 int nnue_ls_route_backward(const nnue_ls_route* a, void* stream) {
   if (int rc = check_route("route_backward", a)) return rc;
   if (a->rows == 0) return NNUE_LS_OK;
   if (!a->grad_logits) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "route_backward: null pointer");
-  const RouteParams r = route_params(*a);
-  with_type(a->dtype, [&](auto t) { launch_route<decltype(t)>(r, true, static_cast<cudaStream_t>(stream)); });
-  return check_launch("route_backward");
+  return with_type(a->dtype,
+                   [&](auto t) { return route_backward<decltype(t)>(*a, static_cast<cudaStream_t>(stream)); });
 }
 
 }  // extern "C"

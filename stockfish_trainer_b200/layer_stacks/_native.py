@@ -11,6 +11,7 @@ import os
 import threading
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import build as _build
 from .._native import NativeError
@@ -126,23 +127,45 @@ def check(func: str, rc: int) -> None:
         raise NativeError(func, rc, last_error())
 
 
-def run(func: str, args: ctypes.Structure, device: torch.device, sized: bool = True) -> None:
-    """Enqueue ``func(args)`` on the device's current stream; with ``sized`` the
-    call takes a workspace, allocated here from PyTorch's caching allocator."""
-    lib = _lib or load()
-    if device.index != torch.cuda.current_device():
+_calls: dict = {}  # name -> (function, its workspace-size function or None)
+
+
+def _lookup(func: str):
+    lib = load()
+    size = func + "_workspace_size"
+    _calls[func] = found = (getattr(lib, func), getattr(lib, size) if size in _SIGNATURES else None)
+    return found
+
+
+def run(func: str, args: ctypes.Structure, device: torch.device) -> None:
+    """Enqueue ``func(args)`` on the device's current stream.  Where the call
+    takes a workspace, it comes from PyTorch's caching allocator."""
+    index = device.index
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            return run(func, args, device, sized)
+            return run(func, args, device)
+    fn, size = _calls.get(func) or _lookup(func)
     ref = ctypes.byref(args)
-    stream = torch.cuda.current_stream().cuda_stream
-    if not sized:
-        return check(func, getattr(lib, func)(ref, stream))
-    nbytes = getattr(lib, func + "_workspace_size")(ref)
-    if nbytes == 0:
-        return check(func, getattr(lib, func)(ref, None, 0, stream))
-    # the caching allocator returns 512-byte aligned blocks; the ABI needs 256
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    check(func, getattr(lib, func)(ref, ws.data_ptr(), nbytes, stream))
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if size is None:
+        rc = fn(ref, stream)
+    else:
+        nbytes = size(ref)
+        # the caching allocator returns 512-byte aligned blocks; the ABI needs 256
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
+        rc = fn(ref, ws, nbytes, stream)
+    if rc != OK:
+        check(func, rc)
+
+
+def once(backward):
+    """``once_differentiable`` that costs nothing unless a graph of the backward is asked for."""
+    guarded = once_differentiable(backward)
+
+    def wrapper(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return wrapper
 
 
 def packed_buffer(a: Linear, device: torch.device) -> torch.Tensor | None:
@@ -161,18 +184,21 @@ def check_tensor(t: torch.Tensor, name: str, device: torch.device | None = None,
         raise TypeError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if device is None:
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+    elif t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}" if t.is_cuda else
+                         f"{name} must be a CUDA tensor")
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """``t`` as a matrix of its last dimension's rows, with unit column stride
     and rows that do not overlap; copied only where the layout asks for it."""
     m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if (m.stride(1) != 1 and m.shape[1] > 1) or (m.stride(0) < m.shape[1] and m.shape[0] > 1):
-        m = m.contiguous()
+    if not m.is_contiguous():
+        if (m.stride(1) != 1 and m.shape[1] > 1) or (m.stride(0) < m.shape[1] and m.shape[0] > 1):
+            m = m.contiguous()
     return m
 
 

@@ -8,7 +8,6 @@ bias, a (squared) clamp to [0, 1], and a skip term added at the end
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -60,7 +59,7 @@ class LinearActFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_native.once
     def backward(ctx, grad_out):
         x, packed, weight, bias, act_grad = ctx.saved_tensors
         act, x_shape, dtype = ctx.meta

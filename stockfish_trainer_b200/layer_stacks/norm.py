@@ -4,29 +4,30 @@ residual scale, as one kernel each way."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
 _KINDS = {"rms": 0, "layer": 1}
-_PARAMS = ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")
 
 
 def _args(x, f, gate, params, meta):
     a = _native.Norm()
     a.rows, a.width = x.shape
-    a.dtype = _native.DTYPES[x.dtype]
-    a.params_dtype = a.gate_dtype = a.dtype
+    dt = _native.DTYPES[x.dtype]
+    a.dtype = a.params_dtype = a.gate_dtype = dt
     a.kind, a.gate_mode, a.gate_sigmoid, a.scale_value, a.eps = meta
     a.x = x.data_ptr()
     if f is not None:
         a.f = f.data_ptr()
     if gate is not None:
-        a.gate, a.gate_dtype = gate.data_ptr(), _native.DTYPES[gate.dtype]
-    for name, t in zip(_PARAMS, params):
+        a.gate = gate.data_ptr()
+        a.gate_dtype = _native.DTYPES[gate.dtype]
+    ptrs = [None if t is None else t.data_ptr() for t in params]
+    a.post_weight, a.post_bias, a.scale, a.pre_weight, a.pre_bias = ptrs
+    for t in params:
         if t is not None:
-            setattr(a, name, t.data_ptr())
             a.params_dtype = _native.DTYPES[t.dtype]
+            break
     return a
 
 
@@ -42,7 +43,7 @@ def _forward(x, f, gate, params, meta, want_stats):
     if want_stats:
         stats = torch.empty(x.shape[0], 4, dtype=torch.float32, device=x.device)
         a.stats = stats.data_ptr()
-    _native.run("nnue_ls_norm_forward", a, x.device, sized=False)
+    _native.run("nnue_ls_norm_forward", a, x.device)
     return y, h, stats
 
 
@@ -60,7 +61,7 @@ class BlockNormFunction(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
+    @_native.once
     def backward(ctx, grad_y, grad_h):
         x, f, gate, stats, *params = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -68,12 +69,9 @@ class BlockNormFunction(torch.autograd.Function):
         a.stats = stats.data_ptr()
         held = [None if g is None else g.contiguous() for g in (grad_y, grad_h)]
         a.grad_y, a.grad_h = (_native.ptr(g) for g in held)
-        grads = [None] * 8
-        names = ("grad_x", "grad_f", "grad_gate") + tuple("grad_" + n for n in _PARAMS)
-        for i, (name, t) in enumerate(zip(names, (x, f, gate, *params))):
-            if need[i] and t is not None:
-                grads[i] = torch.empty_like(t)
-                setattr(a, name, grads[i].data_ptr())
+        grads = [torch.empty_like(t) if n and t is not None else None for n, t in zip(need, (x, f, gate, *params))]
+        (a.grad_x, a.grad_f, a.grad_gate, a.grad_post_weight, a.grad_post_bias, a.grad_scale, a.grad_pre_weight,
+         a.grad_pre_bias) = [None if g is None else g.data_ptr() for g in grads]
         _native.run("nnue_ls_norm_backward", a, x.device)
         return (*grads, None)
 
@@ -137,28 +135,36 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
                 raise ValueError(f"{name} must have shape ({width},), got {tuple(t.shape)}")
             t = t.contiguous()
         params.append(t)
+    # the common case, matrices, adds no view to the graph
+    flat = len(shape) == 2
     mode = 0
     if gate is not None:
         if gate.shape == shape[:-1] or (gate.shape == shape[:-1] + (1,) and width > 1):
             mode = 1
             _native.check_tensor(gate, "gate", dev, mixed)
-            gate = gate.reshape(-1)
+            if gate.dim() != 1:
+                gate = gate.reshape(-1)
         else:
             mode = 2
             _native.check_tensor(gate, "gate", dev, (dt,))
-            try:
-                gate = gate.expand(shape)
-            except RuntimeError:
-                raise ValueError(f"gate {tuple(gate.shape)} fits neither x's rows nor its shape {tuple(shape)}") \
-                    from None
-            gate = gate.reshape(-1, width)
+            if gate.shape != shape:
+                try:
+                    gate = gate.expand(shape)
+                except RuntimeError:
+                    raise ValueError(f"gate {tuple(gate.shape)} fits neither x's rows nor its shape {tuple(shape)}") \
+                        from None
+            if not flat:
+                gate = gate.reshape(-1, width)
         gate = gate.contiguous()
-    x2 = x.reshape(-1, width).contiguous()
-    f2 = None if f is None else f.reshape(-1, width).contiguous()
+    x2 = (x if flat else x.reshape(-1, width)).contiguous()
+    f2 = None if f is None else (f if flat else f.reshape(-1, width)).contiguous()
     meta = (_KINDS[kind], mode, int(gate_activation == "sigmoid"), scale_value, float(eps))
     if _native.needs_grad(x2, f2, gate, *params):
         y, h = BlockNormFunction.apply(x2, f2, gate, *params, meta)
     else:
         y, h, _ = _forward(x2, f2, gate, params, meta, False)
-    y = x if f is None else y.view(shape)
-    return y, None if h is None else h.view(shape)
+    if f is None:
+        y = x
+    elif not flat:
+        y = y.view(shape)
+    return y, h if h is None or flat else h.view(shape)

@@ -9,7 +9,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -56,7 +55,7 @@ class RouteFunction(torch.autograd.Function):
         return indices, gates, counts, loss[0]
 
     @staticmethod
-    @once_differentiable
+    @_native.once
     def backward(ctx, _indices, grad_gates, _counts, grad_loss):
         logits, valid, indices, gates, counts, loss = ctx.saved_tensors
         a = _args(logits, valid, *ctx.meta, indices, gates, counts, loss)
@@ -64,7 +63,7 @@ class RouteFunction(torch.autograd.Function):
         a.grad_gates, a.grad_loss = (_native.ptr(g) for g in held)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         a.grad_logits = grad.data_ptr()
-        _native.run("nnue_ls_route_backward", a, logits.device, sized=False)
+        _native.run("nnue_ls_route_backward", a, logits.device)
         return grad, None, None, None
 
 

@@ -172,54 +172,72 @@ struct Block32 {
   }
 };
 
-// Writes one block of sums: the first `rows` rows from m0, columns n0.. below n1.  With `vec` four
-// (16-bit) or eight (fp32) neighbouring lanes share a row and move 16 bytes
-// each; else one lane per column.
-template <typename T, int ACT>
-__device__ __forceinline__ void store_block_act(const Block32& block, const EpilogueParams& e, int64_t m0, int rows,
-                                                int64_t n0, int64_t n1, int64_t N, int lane) {
+// One block's writer: the first `rows` rows from m0, columns n0.. below n1.
+// With `vec` four (16-bit) or eight (fp32) neighbouring lanes share a row and
+// move 16 bytes each; else one lane per column.  The first residual is asked
+// for at construction, before the sums are waited for.
+template <typename T>
+struct BlockWriter {
   using D = Derivative<T>;
   using Code = typename D::Code;
-  constexpr int V = 16 / sizeof(T), kLanes = 32 / V, kRows = 32 / kLanes;
-  const bool with_grad = ACT != kNone && e.act_grad, with_res = e.residual;
-  if (e.vec) {
-    const int c = (lane % kLanes) * V;
-    int r = lane / kLanes;
-    const int64_t n = n0 + c;
-    if (n >= n1 || r >= rows) return;
-    T* out_p = static_cast<T*>(e.out) + (m0 + r) * N + n;
-    Code* grad_p = static_cast<Code*>(e.act_grad) + (m0 + r) * N + n;
-    const T* res_p = static_cast<const T*>(e.residual) + (m0 + r) * e.ldr + n;
-    VecT<T, V> next;
-    if (with_res) next = *reinterpret_cast<const VecT<T, V>*>(res_p);
+  static constexpr int V = 16 / sizeof(T), kLanes = 32 / V, kRows = 32 / kLanes;
+  const EpilogueParams& e;
+  int64_t m0, n, N;
+  int rows, lane, row, col;
+  bool inside;
+  VecT<T, V> first;
+
+  __device__ __forceinline__ BlockWriter(const EpilogueParams& e_, int64_t m0_, int rows_, int64_t n0, int64_t n1,
+                                         int64_t N_, int lane_)
+      : e(e_), m0(m0_), N(N_), rows(rows_), lane(lane_) {
+    row = e.vec ? lane / kLanes : 0;
+    col = e.vec ? (lane % kLanes) * V : lane;
+    n = n0 + col;
+    inside = n < n1 && row < rows;
+    if (e.vec && e.residual && inside)
+      first = *reinterpret_cast<const VecT<T, V>*>(static_cast<const T*>(e.residual) + (m0 + row) * e.ldr + n);
+  }
+
+  template <int ACT, bool RES, bool GRAD>
+  __device__ __forceinline__ void write_vec(const Block32& block) const {
+    T* out_p = static_cast<T*>(e.out) + (m0 + row) * N + n;
+    Code* grad_p = static_cast<Code*>(e.act_grad) + (m0 + row) * N + n;
+    const T* res_p = static_cast<const T*>(e.residual) + (m0 + row) * e.ldr + n;
+    VecT<T, V> next = first;
     float bias[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) bias[j] = e.bias ? load_mixed<T>(e.bias, n + j, e.bias_f32) : 0.f;
 #pragma unroll 1
-    for (; r < rows; r += kRows) {
+    for (int r = row; r < rows; r += kRows) {
       const VecT<T, V> res = next;
-      res_p += kRows * e.ldr;
-      if (with_res && r + kRows < rows) next = *reinterpret_cast<const VecT<T, V>*>(res_p);  // one step ahead
+      if (RES) {
+        res_p += kRows * e.ldr;
+        if (r + kRows < rows) next = *reinterpret_cast<const VecT<T, V>*>(res_p);  // one step ahead
+      }
       float z[V];
-      block.get<V>(r, c, z);
+      block.get<V>(r, col, z);
       VecT<T, V> out;
       VecT<Code, V> d;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float dv;
         z[j] = activate<T, ACT>(z[j] + bias[j], dv);
-        if (with_res) z[j] += to_f(res.v[j]);
-        d.v[j] = D::encode(dv);
+        if (RES) z[j] += to_f(res.v[j]);
+        if (GRAD) d.v[j] = D::encode(dv);
       }
       round_all(z, out);
       *reinterpret_cast<VecT<T, V>*>(out_p) = out;
-      if (with_grad) *reinterpret_cast<VecT<Code, V>*>(grad_p) = d;
       out_p += kRows * N;
-      grad_p += kRows * N;
+      if (GRAD) {
+        *reinterpret_cast<VecT<Code, V>*>(grad_p) = d;
+        grad_p += kRows * N;
+      }
     }
-  } else {
-    const int64_t n = n0 + lane;
-    if (n >= n1) return;
+  }
+
+  template <int ACT>
+  __device__ __forceinline__ void write_single(const Block32& block) const {
+    const bool with_res = e.residual, with_grad = ACT != kNone && e.act_grad;
     const float bias = e.bias ? load_mixed<T>(e.bias, n, e.bias_f32) : 0.f;
     T* out_p = static_cast<T*>(e.out) + m0 * N + n;
     Code* grad_p = static_cast<Code*>(e.act_grad) + m0 * N + n;
@@ -244,23 +262,31 @@ __device__ __forceinline__ void store_block_act(const Block32& block, const Epil
       res_p += 4 * e.ldr;
     }
   }
-}
 
-template <typename T>
-__device__ __forceinline__ void store_block(const Block32& block, const EpilogueParams& e, int64_t m0, int rows,
-                                            int64_t n0, int64_t n1, int64_t N, int lane) {
-  with_activation(e.act,
-                  [&](auto act) { store_block_act<T, decltype(act)::value>(block, e, m0, rows, n0, n1, N, lane); });
-}
+  __device__ __forceinline__ void write(const Block32& block) const {
+    if (!inside) return;
+    with_activation(e.act, [&](auto a) {
+      constexpr int ACT = decltype(a)::value;
+      if (!e.vec) {
+        write_single<ACT>(block);
+      } else if (e.act_grad && ACT != kNone) {
+        e.residual ? write_vec<ACT, true, ACT != kNone>(block) : write_vec<ACT, false, ACT != kNone>(block);
+      } else {
+        e.residual ? write_vec<ACT, true, false>(block) : write_vec<ACT, false, false>(block);
+      }
+    });
+  }
+};
 
-// The same as a call, for the fp32 kernel: inlined there, the activations' code
+// Writing a block as a call, for the fp32 kernel: inlined there, the activations' code
 // pushes the running sums out of the registers (65536 x 1024 x 1040: 757 us
 // inlined, 561 us called).  The 16-bit kernels hold no sums and are faster
 // inlined (143 us called, 133 us inlined).  `shared`: the parameters' copy in
 // shared memory.
 static __device__ __noinline__ void store_block_f32(float4* block, const EpilogueParams* shared, int64_t m0, int rows,
                                              int64_t n0, int64_t n1, int64_t N, int lane) {
-  store_block<float>(Block32{block}, *shared, m0, rows, n0, n1, N, lane);
+  const EpilogueParams e = *shared;
+  BlockWriter<float>(e, m0, rows, n0, n1, N, lane).write(Block32{block});
 }
 
 // The raw sums of one piece of the k range; vec: N is a multiple of 4.

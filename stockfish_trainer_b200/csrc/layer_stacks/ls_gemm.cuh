@@ -358,12 +358,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int64_t n0 = (tile % p.n_tiles) * p.bn, n1 = min(N, n0 + p.bn);
       const int rows = (int)max((int64_t)0, min((int64_t)32, M - m0));
       float* partial = p.splits > 1 ? p.partial + (int64_t)split * M * N : nullptr;
-      auto finish = [&](int cb, const float (&v)[32]) {
-        block.put(v, lane);
-        if (partial) store_partial(block, partial, N % 4 == 0, m0, rows, n0 + cb * 32, n1, N, lane);
-        else if constexpr (PLANES == 3) store_block_f32(block.s, epilogue, m0, rows, n0 + cb * 32, n1, N, lane);
-        else store_block<T>(block, p.e, m0, rows, n0 + cb * 32, n1, N, lane);
-      };
       if (p.e.residual && !partial && lane < rows) {
         // the residual's rows come from HBM while the tile's products run
         const char* r = reinterpret_cast<const char*>(static_cast<const T*>(p.e.residual) + (m0 + lane) * p.e.ldr);
@@ -375,6 +369,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
         tcgen_fence_after();
         for (int cb = group; cb < col_blocks; cb += kColumnGroups) {
+          const int64_t n = n0 + cb * 32;
+          BlockWriter<T> writer(p.e, m0, partial ? 0 : rows, n, n1, N, lane);
           float v[32];
           tmem_load16(lanes + acc * S::kMaxBN + cb * 32, v);
           tmem_load16(lanes + acc * S::kMaxBN + cb * 32 + 16, v + 16);
@@ -386,7 +382,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               else mbar_arrive_leader(acc_empty0 + 8 * acc);
             }
           }
-          finish(cb, v);
+          block.put(v, lane);
+          if (partial) store_partial(block, partial, N % 4 == 0, m0, rows, n, n1, N, lane);
+          else writer.write(block);
         }
         if (group >= col_blocks && lane == 0) {  // a narrow tile leaves this warp nothing to read
           if constexpr (CG == 1) mbar_arrive(acc_empty0 + 8 * acc);
@@ -429,7 +427,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < kMine; ++i)
-          if (group + kColumnGroups * i < col_blocks) finish(group + kColumnGroups * i, sum[i]);
+          if (group + kColumnGroups * i < col_blocks) {
+            const int64_t n = n0 + (group + kColumnGroups * i) * 32;
+            block.put(sum[i], lane);
+            if (partial) store_partial(block, partial, N % 4 == 0, m0, rows, n, n1, N, lane);
+            else store_block_f32(block.s, epilogue, m0, rows, n, n1, N, lane);
+          }
       }
     }
   }

@@ -73,7 +73,7 @@ struct TilePlan {
 // bytes from L2 (about 48 per clock and SM), whichever is more; an item adds
 // the fill and drain of the pipeline; pieces add their joining pass (at 3500
 // bytes per clock) and its launch.
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, int planes) {
+TilePlan find_tiles(int64_t M, int64_t N, int64_t K, int planes) {
   const int bk = planes == 1 ? 64 : 32, products = planes == 1 ? 1 : 6;
   TilePlan best{};
   double best_cost = 0;
@@ -106,6 +106,19 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, int planes) {
     }
   }
   return best;
+}
+
+// The plan of a shape, kept for the next call with it: the search takes a few
+// microseconds, and a call asks for its workspace's size first.
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, int planes) {
+  struct Entry {
+    int64_t M = 0, N = 0, K = 0;
+    TilePlan plan{};
+  };
+  static thread_local Entry kept[32];
+  Entry& e = kept[(uint64_t)(M * 31 + N * 7 + K) % 32];
+  if (e.M != M || e.N != N || e.K != K) e = Entry{M, N, K, find_tiles(M, N, K, planes)};
+  return e.plan;
 }
 
 template <typename T, int CG>
@@ -204,6 +217,28 @@ Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_m
 }
 
 // ---- forward -------------------------------------------------------------------
+// Up to 4 rows (fp32: 8, where the other way packs its operands first) go to the
+// kernel without tiles.  1040 x 1040 bf16: 2.6 us for one row, 6.8 for 4, 10.9
+// for 8; on tiles 10.6 for any of them.  1040 x 256 fp32: 2.6 us for one row,
+// 6.1 for 8, 16.4 for 16; on tiles 16.7.
+template <typename T>
+bool few_rows(const nnue_ls_linear& a) {
+  return a.rows <= (sizeof(T) == 4 ? 8 : 4);
+}
+
+template <typename T, int MT>
+void launch_few_rows(const nnue_ls_linear& a, const EpilogueParams& e, cudaStream_t s) {
+  constexpr int64_t V = 16 / sizeof(T);
+  auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool vec = a.inputs % V == 0 && (a.ldx % V == 0 || a.rows == 1) && (a.ldw % V == 0 || a.outputs == 1) &&
+                   aligned(a.x) && aligned(a.weight);
+  const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.weight);
+  const unsigned grid = (unsigned)ceil_div(a.outputs, 8);
+  count_launch();
+  if (vec) few_rows_kernel<T, MT, true><<<grid, 256, 0, s>>>(x, a.ldx, w, a.ldw, (int)a.rows, a.outputs, a.inputs, e);
+  else few_rows_kernel<T, MT, false><<<grid, 256, 0, s>>>(x, a.ldx, w, a.ldw, (int)a.rows, a.outputs, a.inputs, e);
+}
+
 struct ForwardPlan {
   TilePlan tiles;
   size_t x, w, partial, total;
@@ -212,6 +247,7 @@ struct ForwardPlan {
 template <typename T>
 ForwardPlan plan_forward(const nnue_ls_linear& a) {
   ForwardPlan p{};
+  if (few_rows<T>(a)) return p;
   p.tiles = plan_tiles(a.rows, a.outputs, a.inputs, sizeof(T) == 4 ? 3 : 1);
   p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
   p.w = needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
@@ -224,7 +260,7 @@ ForwardPlan plan_forward(const nnue_ls_linear& a) {
 
 template <typename T>
 bool linear_packs_x(const nnue_ls_linear& a) {
-  return needs_pack<T>(a.x, a.ldx, a.rows);
+  return !few_rows<T>(a) && needs_pack<T>(a.x, a.ldx, a.rows);
 }
 
 template <typename T>
@@ -239,10 +275,16 @@ size_t linear_forward_bytes(const nnue_ls_linear& a) {
 
 template <typename T>
 int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
+  EpilogueParams e{a.bias, a.residual, a.out, a.act_grad, a.ldr, a.activation, a.bias_dtype == NNUE_LS_F32, false};
+  if (few_rows<T>(a)) {
+    if (a.rows == 1) launch_few_rows<T, 1>(a, e, s);
+    else if (a.rows <= 4) launch_few_rows<T, 4>(a, e, s);
+    else if constexpr (sizeof(T) == 4) launch_few_rows<T, 8>(a, e, s);
+    return check_launch("linear_forward");
+  }
   const ForwardPlan p = plan_forward<T>(a);
   const Operand x = operand<T>(a.x, a.ldx, a.rows, a.inputs, false, a.x_packed ? a.x_packed : ws, s);
   const Operand w = operand<T>(a.weight, a.ldw, a.outputs, a.inputs, false, ws + p.x, s);
-  EpilogueParams e{a.bias, a.residual, a.out, a.act_grad, a.ldr, a.activation, a.bias_dtype == NNUE_LS_F32, false};
   return launch_gemm<T>(x, w, a.rows, a.outputs, p.tiles, e, ws + p.x + p.w, s);
 }
 

@@ -17,7 +17,7 @@ struct NormParams {
   const void *x, *f, *gate;
   const void *post_weight, *post_bias, *scale, *pre_weight, *pre_bias;  // [width]; null = absent
   void *y, *h;
-  float4* stats;  // per row: mean of f and its variance + eps; the same of y
+  float4* stats;  // per row: mean of f and 1 / its deviation; the same of y
   const void *grad_y, *grad_h;
   void *grad_x, *grad_f, *grad_gate;
   float* partial;  // backward: [blocks, 5, width] column sums (post_weight, post_bias, scale, pre_weight, pre_bias)
@@ -28,7 +28,13 @@ struct NormParams {
   bool gate_sigmoid, gate_f32, params_f32;
 };
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
+// 1 / sqrt(v) to about one unit: the hardware's estimate and a Newton step.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float r = rsqrtf(v), e = fmaf(-v * r, r, 1.f);
+  return v > 0.f && isfinite(r) ? fmaf(0.5f * r, e, r) : r;
+}
 
 // One row of the forward's inputs, element by element; used by every pass.
 template <typename T>
@@ -65,10 +71,10 @@ struct NormRow {
   }
 };
 
-// Mean (layer norm) and variance + eps of a row whose element c is value(c).
+// Mean (layer norm) and 1 / deviation of a row whose element c is value(c).
 template <bool CENTER, typename F>
 __device__ __forceinline__ void row_stats(const F& value, int width, float eps, float* scratch, float& mean,
-                                          float& var) {
+                                          float& rstd) {
   float v[1];
   mean = 0.f;
   if (CENTER) {
@@ -83,7 +89,7 @@ __device__ __forceinline__ void row_stats(const F& value, int width, float eps, 
     v[0] += d * d;
   }
   block_sum(v, scratch);
-  var = v[0] / width + eps;
+  rstd = inv_sqrt(v[0] / width + eps);
 }
 
 // One block per row, any width; the row is read again for each pass.
@@ -92,12 +98,10 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
   __shared__ float scratch[32];
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     NormRow<T> r(p, row);
-    float mean_y = 0.f, var_f = 1.f, var_y = 1.f;
+    float mean_y = 0.f, rstd_y = 1.f;
     if (p.f && p.post_weight)
-      row_stats<CENTER>([&](int c) { return to_f(r.f[c]); }, p.width, p.eps, scratch, r.mean_f, var_f);
-    r.rstd_f = __frsqrt_rn(var_f);
-    if (p.pre_weight) row_stats<CENTER>([&](int c) { return r.y(c); }, p.width, p.eps, scratch, mean_y, var_y);
-    const float rstd_y = __frsqrt_rn(var_y);
+      row_stats<CENTER>([&](int c) { return to_f(r.f[c]); }, p.width, p.eps, scratch, r.mean_f, r.rstd_f);
+    if (p.pre_weight) row_stats<CENTER>([&](int c) { return r.y(c); }, p.width, p.eps, scratch, mean_y, rstd_y);
     for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
       const float y = r.y(c);
       if (p.y) static_cast<T*>(p.y)[row * p.width + c] = from_f<T>(y);
@@ -107,7 +111,7 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
         static_cast<T*>(p.h)[row * p.width + c] = from_f<T>(h);
       }
     }
-    if (p.stats && threadIdx.x == 0) p.stats[row] = make_float4(r.mean_f, var_f, mean_y, var_y);
+    if (p.stats && threadIdx.x == 0) p.stats[row] = make_float4(r.mean_f, r.rstd_f, mean_y, rstd_y);
   }
 }
 
@@ -117,8 +121,8 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
 //   df = rstd_f * (v - mean(v) - f_hat * mean(v * f_hat)),      v = gate * d * post_weight
 // and, summed over rows: post_weight += gate * d * f_hat, post_bias += gate * d, scale += d * x,
 // pre_weight += dh * y_hat, pre_bias += dh.
-// The products with y_hat and f_hat are formed as (y - mean) * (mean(u * (y - mean)) / (var + eps)): the two terms
-// of a difference that can cancel then share fewer roundings.
+// The products with y_hat and f_hat are formed as (y - mean) * (mean(u * (y - mean)) * rstd^2): the two terms of a
+// difference that can cancel then share fewer roundings.
 // y is formed again from x, f and the gate: x has to be read for the scale's gradient anyway, and the y that the
 // forward wrote is rounded to 16 bits, which would show in the fp32 sums.
 // Each block owns a slice of `partial` and each thread its columns of it.
@@ -135,8 +139,8 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
     NormRow<T> r(p, row);
     const float4 st = p.stats[row];
     r.mean_f = st.x;
-    r.rstd_f = __frsqrt_rn(st.y);
-    const float rstd_y = __frsqrt_rn(st.w);
+    r.rstd_f = st.y;
+    const float rstd_y = st.w;
     const T* gy = static_cast<const T*>(p.grad_y) + (p.grad_y ? row * W : 0);
     const T* gh = static_cast<const T*>(p.grad_h) + (p.grad_h ? row * W : 0);
     const bool pre = p.grad_h && p.pre_weight;
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
       }
       block_sum(s, scratch);
     }
-    const float c1 = s[0] * inv / st.w, c2 = s[1] * inv;
+    const float c1 = s[0] * inv * (rstd_y * rstd_y), c2 = s[1] * inv;
     auto d_of = [&](int c) {
       float d = p.grad_y ? to_f(gy[c]) : 0.f;
       if (pre) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
       q[1] = t[1];
       q[2] = t2[0];
     }
-    const float c3 = q[0] * inv / st.y, c4 = q[1] * inv;
+    const float c3 = q[0] * inv * (st.y * st.y), c4 = q[1] * inv;
     for (int c = threadIdx.x; c < W; c += blockDim.x) {
       const float d = d_of(c);
       const int64_t o = row * W + c;
@@ -224,8 +228,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
 // keeps NV * V = 4 columns of them in registers (V = 4 neighbouring ones, or 4
 // single ones where rows are not aligned).  A thread's columns are the same in
 // every row, so the parameters are read once and the sums over rows are plain
-// registers until the block's last row; R rows share each barrier, and with
-// PREFETCH the next R rows are on their way meanwhile.
+// registers until the block's last row; R rows share each barrier.
 
 // V values of a row at column c.
 template <typename T, int V>
@@ -355,48 +358,131 @@ struct Columns {
   }
 };
 
-// The rows of one round: loads skip what the call does not have (then zero).
-template <typename T, int V, bool FULL, bool BACKWARD>
-struct RowIn {
-  Columns<T, V> x, f, g, gy, gh;
-  float4 st;
-  float gate;
-  __device__ __forceinline__ void init() {
-    x.zero(), f.zero(), g.zero(), gy.zero(), gh.zero();
-    st = make_float4(0.f, 1.f, 0.f, 1.f);
-    gate = 0.f;
+// The rows to come, on their way from HBM to shared memory while earlier ones
+// are worked on: STAGES rounds of R rows, a thread's own columns in a slot of
+// its own, so that nobody waits for anybody and every pass over a row reads its
+// slot again instead of holding the row in registers.  Arrays: x, f, grad_y,
+// grad_h, gate.  STAGES == 0 (V == 1: a 2-byte value cannot be copied
+// asynchronously): the rows are loaded when they are needed, into registers.
+enum RowArray : int { kX = 0, kF = 1, kGate = 2, kGradY = 3, kGradH = 4 };
+
+template <typename T, int V, int R, bool FULL, bool BACKWARD, int STAGES>
+struct RowRing {
+  using C = Columns<T, V>;
+  using Raw = typename RowVec<T, 4>::Raw;
+  static constexpr int kArrays = 2 + FULL + 2 * BACKWARD;
+  __host__ __device__ static constexpr int index(int a) { return a <= kGate ? a : a - !FULL; }
+  Raw* slots;
+  const void* base[5];
+  int width, rows, stage = 0;
+  C held[STAGES ? 1 : R][STAGES ? 1 : kArrays];
+
+  __device__ __forceinline__ RowRing(const NormParams& p, void* smem) {
+    slots = static_cast<Raw*>(smem) + threadIdx.x;
+    base[kX] = p.x;
+    base[kF] = p.f;
+    base[kGate] = FULL ? p.gate : nullptr;
+    base[kGradY] = BACKWARD ? p.grad_y : nullptr;
+    base[kGradH] = BACKWARD ? p.grad_h : nullptr;
+    width = p.width;
+    rows = (int)p.rows;
   }
-  __device__ __forceinline__ void load(const NormParams& p, int64_t row) {
-    if (row >= p.rows) {  // adds nothing to any sum
-      init();
-      return;
+  __device__ __forceinline__ Raw* slot(int st, int r, int i) const {
+    return slots + ((st * R + r) * kArrays + i) * (int)blockDim.x;
+  }
+  __device__ __forceinline__ void issue(int row0, int st) const {
+    const int c = (int)threadIdx.x * 4;
+    if (c < width && row0 < rows) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int64_t at = (int64_t)min(row0 + r, rows - 1) * width + c;  // beyond the last row: read, not used
+#pragma unroll
+        for (int a = 0; a < 5; ++a) {
+          if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
+          if (a != kX && !base[a]) continue;
+          const T* src = static_cast<const T*>(base[a]) + at;
+          const unsigned d = (unsigned)__cvta_generic_to_shared(slot(st, r, index(a)));
+          if constexpr (sizeof(Raw) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+        }
+      }
     }
-    x.load(p.x, row, p.width);
-    if (p.f) f.load(p.f, row, p.width);
-    if (FULL) g.load(p.gate, row, p.width);
-    gate = !p.f ? 0.f : p.gate_mode == kGateRow ? load_mixed<T>(p.gate, row, p.gate_f32) : 1.f;
-    if (BACKWARD) {
-      if (p.grad_y) gy.load(p.grad_y, row, p.width);
-      if (p.grad_h) gh.load(p.grad_h, row, p.width);
-      st = p.stats[row];
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void start(int row0, int stride) {
+    if constexpr (STAGES > 0) {
+#pragma unroll
+      for (int i = 0; i < STAGES - 1; ++i) issue(row0 + i * stride, i);
     }
   }
-  // the row's gate, or this column's
-  __device__ __forceinline__ float gate_at(const NormParams& p, float row_gate, int k) const {
-    if (!FULL) return row_gate;
-    return p.gate_sigmoid ? sigmoid(g[k]) : g[k];
+  // The rows from row0 on are there; those of STAGES - 1 rounds later are asked for.
+  __device__ __forceinline__ void next(int row0, int stride) {
+    if constexpr (STAGES > 0) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES > 1 ? STAGES - 2 : 0) : "memory");
+      // the slots written now were last read in the round before, by this thread
+      const int64_t ahead = row0 + (int64_t)(STAGES - 1) * stride;
+      issue(ahead < rows ? (int)ahead : rows, stage == 0 ? STAGES - 1 : stage - 1);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int a = 0; a < 5; ++a) {
+          if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
+          held[r][index(a)].zero();
+          if (base[a]) held[r][index(a)].load(base[a], min(row0 + r, rows - 1), width);
+        }
+    }
   }
-  __device__ __forceinline__ float row_gate(const NormParams& p) const {
-    return p.gate_mode == kGateRow && p.gate_sigmoid ? sigmoid(gate) : gate;
+  __device__ __forceinline__ void done() {
+    if (STAGES > 0 && ++stage == STAGES) stage = 0;
+  }
+  // The thread's four values of array A in row r of the round; zero where there are none.
+  template <int A>
+  __device__ __forceinline__ void get(int r, float (&v)[4]) const {
+    if constexpr (STAGES > 0) {
+      typename RowVec<T, 4>::Raw raw;
+      if ((A == kX || base[A]) && (int)threadIdx.x * 4 < width) raw = *slot(stage, r, index(A));
+      else raw = typename RowVec<T, 4>::Raw{};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = to_f(raw.v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = held[r][index(A)][k];
+    }
   }
 };
 
-template <typename T, int V, int R, bool CENTER, bool FULL, int THREADS, int BLOCKS>
+// The gate of a row's four columns.
+template <bool FULL, typename Ring>
+__device__ __forceinline__ void gates(const NormParams& p, const Ring& ring, int r, float row_gate, float (&g)[4]) {
+  if constexpr (FULL) {
+    ring.template get<kGate>(r, g);
+    if (p.gate_sigmoid) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g[k] = sigmoid(g[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = row_gate;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float load_row_gate(const NormParams& p, int row) {
+  if (p.gate_mode != kGateRow) return 1.f;
+  const float g = load_mixed<T>(p.gate, row, p.gate_f32);
+  return p.gate_sigmoid ? sigmoid(g) : g;
+}
+
+// BOTH: the call has f with its norm and the norm after it; else what is there
+// is looked up.
+template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, int STAGES, int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
+  extern __shared__ float4 norm_ring[];
   __shared__ float scratch[2 * 32 * R];
   BlockSum<R> total{scratch};
-  const int W = p.width;
+  const bool has_f = BOTH || p.f, post = BOTH || p.post_weight, pre = BOTH || p.h;
+  const int W = p.width, rows = (int)p.rows, stride = (int)gridDim.x * R;
   const float inv = 1.f / W;
   bool mine[4];  // columns inside the row
 #pragma unroll
@@ -407,202 +493,238 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
   C::params(p.scale, W, p.params_f32, p.scale_value, sc);
   C::params(p.pre_weight, W, p.params_f32, 1.f, pw);
   C::params(p.pre_bias, W, p.params_f32, 0.f, pb);
-  RowIn<T, V, FULL, false> in[R];
+  RowRing<T, V, R, FULL, false, STAGES> ring(p, norm_ring);
+  ring.start((int)blockIdx.x * R, stride);
+  for (int row0 = (int)blockIdx.x * R; row0 < rows; row0 += stride) {
+    ring.next(row0, stride);
+    float gate[R], mean_f[R], rstd_f[R], mean_y[R], rstd_y[R], s[R], y[R][4], v[4];
 #pragma unroll
-  for (int r = 0; r < R; ++r) in[r].init();
-  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < p.rows; row0 += (int64_t)gridDim.x * R) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) in[r].load(p, row0 + r);
-    float4 st[R];
-    float s[R], y[R][4];
-#pragma unroll
-    for (int r = 0; r < R; ++r) st[r] = make_float4(0.f, 1.f, 0.f, 1.f);
-    if (p.post_weight) {
+    for (int r = 0; r < R; ++r) {
+      gate[r] = FULL ? 1.f : load_row_gate<T>(p, min(row0 + r, rows - 1));
+      mean_f[r] = mean_y[r] = 0.f;
+      rstd_f[r] = rstd_y[r] = 1.f;
+    }
+    if (post) {
       if (CENTER) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = (in[r].f[0] + in[r].f[1]) + (in[r].f[2] + in[r].f[3]);
+        for (int r = 0; r < R; ++r) {
+          ring.template get<kF>(r, v);
+          s[r] = (v[0] + v[1]) + (v[2] + v[3]);
+        }
         total(s);
 #pragma unroll
-        for (int r = 0; r < R; ++r) st[r].x = s[r] * inv;
+        for (int r = 0; r < R; ++r) mean_f[r] = s[r] * inv;
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        ring.template get<kF>(r, v);
         s[r] = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float d = in[r].f[k] - st[r].x;
-          if (mine[k]) s[r] += d * d;
+          const float d = CENTER ? (mine[k] ? v[k] - mean_f[r] : 0.f) : v[k];
+          s[r] = fmaf(d, d, s[r]);
         }
       }
       total(s);
 #pragma unroll
-      for (int r = 0; r < R; ++r) st[r].y = s[r] * inv + p.eps;
+      for (int r = 0; r < R; ++r) rstd_f[r] = inv_sqrt(s[r] * inv + p.eps);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float row_gate = in[r].row_gate(p), rstd = __frsqrt_rn(st[r].y);
+      ring.template get<kX>(r, y[r]);
+      if (has_f) {
+        float g[4];
+        gates<FULL>(p, ring, r, gate[r], g);
+        ring.template get<kF>(r, v);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float n = (in[r].f[k] - st[r].x) * rstd * w[k] + b[k];
-        y[r][k] = p.f ? sc[k] * in[r].x[k] + in[r].gate_at(p, row_gate, k) * n : in[r].x[k];
+        for (int k = 0; k < 4; ++k)
+          y[r][k] = sc[k] * y[r][k] + g[k] * fmaf((v[k] - mean_f[r]) * rstd_f[r], w[k], b[k]);
+        if (row0 + r < rows) C::store(p.y, row0 + r, W, y[r]);
       }
-      if (p.f && row0 + r < p.rows) C::store(p.y, row0 + r, W, y[r]);
     }
-    if (p.h) {
+    if (pre) {
       if (CENTER) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           s[r] = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (mine[k]) s[r] += y[r][k];
+          for (int k = 0; k < 4; ++k) s[r] += mine[k] ? y[r][k] : 0.f;
         }
         total(s);
 #pragma unroll
-        for (int r = 0; r < R; ++r) st[r].z = s[r] * inv;
+        for (int r = 0; r < R; ++r) mean_y[r] = s[r] * inv;
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         s[r] = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float d = y[r][k] - st[r].z;
-          if (mine[k]) s[r] += d * d;
+          const float d = mine[k] ? y[r][k] - mean_y[r] : 0.f;
+          s[r] = fmaf(d, d, s[r]);
         }
       }
       total(s);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        st[r].w = s[r] * inv + p.eps;
-        const float rstd = __frsqrt_rn(st[r].w);
+        rstd_y[r] = inv_sqrt(s[r] * inv + p.eps);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[r][k] = (y[r][k] - st[r].z) * rstd * pw[k] + pb[k];
-        if (row0 + r < p.rows) C::store(p.h, row0 + r, W, y[r]);
+        for (int k = 0; k < 4; ++k) y[r][k] = fmaf((y[r][k] - mean_y[r]) * rstd_y[r], pw[k], pb[k]);
+        if (row0 + r < rows) C::store(p.h, row0 + r, W, y[r]);
       }
     }
     if (p.stats && threadIdx.x == 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (row0 + r < p.rows) p.stats[row0 + r] = st[r];
+        if (row0 + r < rows) p.stats[row0 + r] = make_float4(mean_f[r], rstd_f[r], mean_y[r], rstd_y[r]);
     }
+    ring.done();
   }
 }
 
-template <typename T, int V, int R, bool CENTER, bool FULL, bool PREFETCH, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_backward_rows_kernel(const NormParams p) {
+template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, int STAGES, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
   constexpr int N1 = CENTER ? 2 : 1, N2 = CENTER ? 3 : 2, K1 = R * N1, K2 = pow2_at_least(R * N2);
+  extern __shared__ float4 norm_ring[];
   __shared__ float scratch[2 * 32 * (K1 + K2)];
   BlockSum<K1> total1{scratch};
   BlockSum<K2> total2{scratch + 2 * 32 * K1};
-  const int W = p.width;
+  const bool has_f = BOTH || p.f, post = BOTH || p.post_weight, pre = BOTH || (p.grad_h && p.pre_weight);
+  const int W = p.width, rows = (int)p.rows, stride = (int)gridDim.x * R;
   const float inv = 1.f / W;
-  const bool pre = p.grad_h && p.pre_weight;
   float w[4], b[4], sc[4], pw[4], acc[5][4] = {};
   C::params(p.post_weight, W, p.params_f32, 1.f, w);
   C::params(p.post_bias, W, p.params_f32, 0.f, b);
   C::params(p.scale, W, p.params_f32, p.scale_value, sc);
   C::params(p.pre_weight, W, p.params_f32, 0.f, pw);
-  RowIn<T, V, FULL, true> in[R], next[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    in[r].init();
-    if (PREFETCH) {
-      next[r].init();
-      next[r].load(p, (int64_t)blockIdx.x * R + r);
-    }
-  }
-  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < p.rows; row0 += (int64_t)gridDim.x * R) {
+  RowRing<T, V, R, FULL, true, STAGES> ring(p, norm_ring);
+  ring.start((int)blockIdx.x * R, stride);
+  // the rows' statistics and gates come a round ahead, in registers
+  float4 st[R], st_next[R];
+  float gate[R], gate_next[R];
+  auto ahead = [&](int row0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (PREFETCH) {
-        in[r] = next[r];
-        next[r].load(p, row0 + (int64_t)gridDim.x * R + r);
-      } else {
-        in[r].load(p, row0 + r);
-      }
+      const int row = min(row0 + r, rows - 1);
+      st_next[r] = __ldg(p.stats + row);
+      gate_next[r] = FULL ? 1.f : load_row_gate<T>(p, row);
     }
-    float row_gate[R], rstd_f[R], rstd_y[R], d[R][4], s[K1];  // d: y - mean, then the gradient of y
+  };
+  if ((int)blockIdx.x * R < rows) ahead((int)blockIdx.x * R);
+  for (int row0 = (int)blockIdx.x * R; row0 < rows; row0 += stride) {
+    ring.next(row0, stride);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      row_gate[r] = in[r].row_gate(p);
-      rstd_f[r] = __frsqrt_rn(in[r].st.y);
-      rstd_y[r] = __frsqrt_rn(in[r].st.w);
+      st[r] = st_next[r];
+      gate[r] = gate_next[r];
     }
+    ahead(min(row0 + stride, rows - 1));
+    float d[R][4], s[K1], q[K2];  // d: y - mean, then the gradient of y
     if (pre) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        const bool live = row0 + r < rows;
+        float gh[4], v[4], g[4];
+        ring.template get<kX>(r, d[r]);
+        ring.template get<kGradH>(r, gh);
+        if (has_f) {
+          ring.template get<kF>(r, v);
+          gates<FULL>(p, ring, r, gate[r], g);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            d[r][k] = sc[k] * d[r][k] + g[k] * fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]);
+        }
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float y = in[r].x[k];
-          if (p.f) {
-            const float n = (in[r].f[k] - in[r].st.x) * rstd_f[r] * w[k] + b[k];
-            y = sc[k] * y + in[r].gate_at(p, row_gate[r], k) * n;
-          }
-          const float yc = y - in[r].st.z, gh = in[r].gh[k], u = gh * pw[k];
-          d[r][k] = yc;
-          s0 += u * yc;
+          d[r][k] -= st[r].z;
+          const float u = gh[k] * pw[k];
+          s0 = fmaf(u, d[r][k], s0);
           if (CENTER) s1 += u;
-          acc[3][k] += gh * (yc * rstd_y[r]);
-          acc[4][k] += gh;
         }
         s[r * N1] = s0;
         if (CENTER) s[r * N1 + 1] = s1;
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            acc[3][k] = fmaf(gh[k], d[r][k] * st[r].w, acc[3][k]);
+            acc[4][k] += gh[k];
+          }
+        }
       }
       total1(s);
     }
-    float q[K2];
 #pragma unroll
     for (int i = R * N2; i < K2; ++i) q[i] = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float c1 = pre ? s[r * N1] * inv / in[r].st.w : 0.f, c2 = CENTER && pre ? s[r * N1 + CENTER] * inv : 0.f;
-      float dx[4], q0 = 0.f, q1 = 0.f, q2 = 0.f;
+      const bool live = row0 + r < rows;
+      float gy[4], v[4], g[4], dx[4], q0 = 0.f, q1 = 0.f, q2 = 0.f;
+      ring.template get<kGradY>(r, gy);
+      if (pre) {
+        const float c1 = s[r * N1] * inv * (st[r].w * st[r].w), c2 = CENTER ? s[r * N1 + CENTER] * inv : 0.f;
+        ring.template get<kGradH>(r, v);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v = in[r].gy[k];
-        if (pre) v += rstd_y[r] * (in[r].gh[k] * pw[k] - c2 - d[r][k] * c1);
-        d[r][k] = v;
-        dx[k] = p.f ? sc[k] * v : v;
-        const float gn = in[r].gate_at(p, row_gate[r], k) * v, fc = in[r].f[k] - in[r].st.x, fh = fc * rstd_f[r],
-                    vw = gn * w[k];
-        q0 += vw * fc;
-        if (CENTER) q1 += vw;
-        q2 += v * (fh * w[k] + b[k]);
-        acc[0][k] += gn * fh;
-        acc[1][k] += gn;
-        acc[2][k] += v * in[r].x[k];
+        for (int k = 0; k < 4; ++k) gy[k] = fmaf(st[r].w, fmaf(-d[r][k], c1, fmaf(v[k], pw[k], -c2)), gy[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[r][k] = gy[k], dx[k] = sc[k] * gy[k];
+      if (p.grad_x && live) C::store(p.grad_x, row0 + r, W, dx);
+      if (has_f) {
+        float x[4];
+        ring.template get<kF>(r, v);
+        ring.template get<kX>(r, x);
+        gates<FULL>(p, ring, r, gate[r], g);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float gn = g[k] * d[r][k], fc = v[k] - st[r].x, fh = fc * st[r].y, vw = gn * w[k];
+          q0 = fmaf(vw, fc, q0);
+          if (CENTER) q1 += vw;
+          if (!FULL) q2 = fmaf(d[r][k], fmaf(fh, w[k], b[k]), q2);
+          if (live) {
+            acc[0][k] = fmaf(gn, fh, acc[0][k]);
+            acc[1][k] += gn;
+            acc[2][k] = fmaf(d[r][k], x[k], acc[2][k]);
+          }
+        }
       }
       q[r * N2] = q0;
       q[r * N2 + 1] = q2;
-      if (CENTER) q[r * N2 + 2] = q1;
-      if (p.grad_x && row0 + r < p.rows) C::store(p.grad_x, row0 + r, W, dx);
+      if (CENTER) q[r * N2 + 2 * CENTER] = q1;
     }
-    if (!p.f) continue;
-    total2(q);
+    if (has_f) {
+      total2(q);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (row0 + r >= p.rows) break;
-      const float c3 = p.post_weight ? q[r * N2] * inv / in[r].st.y : 0.f, c4 = CENTER && p.post_weight ? q[r * N2 + 2 * CENTER] * inv : 0.f;
-      float df[4], dg[4];
+      for (int r = 0; r < R; ++r) {
+        if (row0 + r < rows) {
+          const float c3 = post ? q[r * N2] * inv * (st[r].y * st[r].y) : 0.f,
+                      c4 = CENTER && post ? q[r * N2 + 2 * CENTER] * inv : 0.f;
+          float v[4], g[4], df[4];
+          ring.template get<kF>(r, v);
+          gates<FULL>(p, ring, r, gate[r], g);
+          if (p.grad_f) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float gate = in[r].gate_at(p, row_gate[r], k), fc = in[r].f[k] - in[r].st.x;
-        df[k] = rstd_f[r] * (gate * d[r][k] * w[k] - c4 - fc * c3);
-        if (FULL) {
-          dg[k] = d[r][k] * (fc * rstd_f[r] * w[k] + b[k]);
-          if (p.gate_sigmoid) dg[k] *= gate * (1.f - gate);
+            for (int k = 0; k < 4; ++k)
+              df[k] = st[r].y * fmaf(-(v[k] - st[r].x), c3, fmaf(g[k] * d[r][k], w[k], -c4));
+            C::store(p.grad_f, row0 + r, W, df);
+          }
+          if (FULL) {
+            if (p.grad_gate) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                df[k] = d[r][k] * fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]);
+                if (p.gate_sigmoid) df[k] *= g[k] * (1.f - g[k]);
+              }
+              C::store(p.grad_gate, row0 + r, W, df);
+            }
+          } else if (p.grad_gate && threadIdx.x == 0) {
+            const float gr = gate[r], dq = q[r * N2 + 1];
+            store_mixed<T>(p.grad_gate, row0 + r, p.gate_f32, p.gate_sigmoid ? dq * gr * (1.f - gr) : dq);
+          }
         }
       }
-      if (p.grad_f) C::store(p.grad_f, row0 + r, W, df);
-      if (FULL) {
-        if (p.grad_gate) C::store(p.grad_gate, row0 + r, W, dg);
-      } else if (p.grad_gate && threadIdx.x == 0) {
-        const float g = row_gate[r], dq = q[r * N2 + 1];
-        store_mixed<T>(p.grad_gate, row0 + r, p.gate_f32, p.gate_sigmoid ? dq * g * (1.f - g) : dq);
-      }
     }
+    ring.done();
   }
   if (!p.partial) return;
   float* part = p.partial + (int64_t)blockIdx.x * 5 * W;

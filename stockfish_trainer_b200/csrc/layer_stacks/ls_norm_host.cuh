@@ -64,7 +64,6 @@ struct RowPlan {
   int threads;  // 0: the kernel for any width
   bool narrow() const { return vec && threads <= 288; }
 };
-constexpr int kRowsForward = 4;
 
 template <typename T>
 RowPlan plan_norm(const nnue_ls_norm& a) {
@@ -73,25 +72,49 @@ RowPlan plan_norm(const nnue_ls_norm& a) {
   if (threads <= 512) r.threads = (int)threads;
   return r;
 }
-// rows at a time: what 168 registers a thread hold twice over (narrow) or 128 once
-template <typename T>
-constexpr int rows_backward(bool narrow, bool full) { return narrow && sizeof(T) == 2 && !full ? 4 : 2; }
+
+// Rows at a time, rounds in flight, and blocks per SM, so that registers and
+// 227 KB of shared memory hold them.
+template <typename T, bool NARROW, bool FULL, bool BACKWARD>
+struct RowShape {
+  static constexpr int kThreads = NARROW ? 288 : 512;
+  static constexpr int kRows = BACKWARD ? (NARROW && sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 2 || !FULL ? 4 : 2;
+  static constexpr int kSlot = (int)sizeof(T) * 4 * kRows * (2 + FULL + 2 * BACKWARD);  // bytes per thread and round
+  static constexpr int kBlocks = NARROW ? 2 : 1;
+  static constexpr int kFit = 220 * 1024 / kBlocks / (kSlot * kThreads);
+  static constexpr int kStages = kFit > 4 ? 4 : kFit;
+  static_assert(kStages >= 2, "a round on its way while one is worked on");
+};
+
+int norm_blocks_per_sm(const RowPlan& r) { return std::min(16, std::max(1, (r.narrow() ? 576 : 512) / r.threads)); }
 
 template <typename T>
 int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
   const int64_t rows = std::max<int64_t>(a.rows, 1);
   if (!r.threads) return std::min<int64_t>(rows, kNumSMs * 4);
-  const int per_sm = (r.narrow() ? 288 : 512) / r.threads;  // as the registers allow
-  return std::min<int64_t>(ceil_div(rows, rows_backward<T>(r.narrow(), a.gate_mode == kGateFull)), (int64_t)kNumSMs * std::min(per_sm, 8));
+  const int at_once = r.narrow() ? RowShape<T, true, false, true>::kRows : RowShape<T, false, false, true>::kRows;
+  return std::min<int64_t>(ceil_div(rows, at_once), (int64_t)kNumSMs * norm_blocks_per_sm(r));
 }
 
-// fn(center, full) with both as constants.
+// Launches with the ring's shared memory, `slots` of them per thread.
+template <typename K>
+int launch_norm_rows(K kernel, unsigned grid, const RowPlan& r, size_t slot_bytes, const NormParams& p, cudaStream_t s) {
+  const size_t smem = slot_bytes * r.threads;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "norm: %s", cudaGetErrorString(e));
+  }
+  kernel<<<grid, r.threads, smem, s>>>(p);
+  return NNUE_LS_OK;
+}
+
+// fn(center, full, both) with all as constants.
 template <typename F>
-void with_flags(bool center, bool full, const F& fn) {
-  using Yes = std::true_type;
-  using No = std::false_type;
-  if (center) full ? fn(Yes{}, Yes{}) : fn(Yes{}, No{});
-  else full ? fn(No{}, Yes{}) : fn(No{}, No{});
+int with_flags(bool center, bool full, bool both, const F& fn) {
+  auto pick = [](bool v, const auto& next) { return v ? next(std::true_type{}) : next(std::false_type{}); };
+  return pick(center, [&](auto c) {
+    return pick(full, [&](auto f) { return pick(both, [&](auto b) { return fn(c, f, b); }); });
+  });
 }
 
 }  // namespace
@@ -109,15 +132,23 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
     return check_launch("norm_forward");
   }
   // as many blocks as stay on the SMs together, each looping over rows
-  const int per_sm = std::min(16, 576 / r.threads);
-  const unsigned grid =
-      (unsigned)std::min<int64_t>(ceil_div(a.rows, kRowsForward), (int64_t)kNumSMs * std::max(1, per_sm));
-  with_flags(center, a.gate_mode == kGateFull, [&](auto c, auto f) {
-    constexpr bool C = decltype(c)::value, F = decltype(f)::value;
-    if (r.narrow()) norm_forward_rows_kernel<T, 4, kRowsForward, C, F, 288, 2><<<grid, r.threads, 0, s>>>(p);
-    else if (r.vec) norm_forward_rows_kernel<T, 4, kRowsForward, C, F, 512, 1><<<grid, r.threads, 0, s>>>(p);
-    else norm_forward_rows_kernel<T, 1, kRowsForward, C, F, 512, 1><<<grid, r.threads, 0, s>>>(p);
+  auto blocks = [&](int at_once) {
+    return (unsigned)std::min<int64_t>(ceil_div(a.rows, at_once), (int64_t)kNumSMs * norm_blocks_per_sm(r));
+  };
+  const bool both = a.f && a.post_weight && a.h;
+  const int rc = with_flags(center, a.gate_mode == kGateFull, both, [&](auto c, auto f, auto b2) {
+    constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b2)::value;
+    using N = RowShape<T, true, F, false>;
+    using W = RowShape<T, false, F, false>;
+    if (r.narrow())
+      return launch_norm_rows(norm_forward_rows_kernel<T, 4, N::kRows, C, F, B, N::kStages, 288, 2>,
+                              blocks(N::kRows), r, N::kSlot * N::kStages, p, s);
+    if (r.vec)
+      return launch_norm_rows(norm_forward_rows_kernel<T, 4, W::kRows, C, F, B, W::kStages, 512, 1>,
+                              blocks(W::kRows), r, W::kSlot * W::kStages, p, s);
+    return launch_norm_rows(norm_forward_rows_kernel<T, 1, 4, C, F, B, 0, 512, 1>, blocks(4), r, 0, p, s);
   });
+  if (rc) return rc;
   return check_launch("norm_forward");
 }
 
@@ -138,12 +169,20 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
     if (center) norm_backward_kernel<T, true><<<grid, 256, 0, s>>>(p);
     else norm_backward_kernel<T, false><<<grid, 256, 0, s>>>(p);
   } else {
-    with_flags(center, a.gate_mode == kGateFull, [&](auto c, auto f) {
-      constexpr bool C = decltype(c)::value, F = decltype(f)::value;
-      if (r.narrow()) norm_backward_rows_kernel<T, 4, rows_backward<T>(true, F), C, F, true, 288><<<grid, r.threads, 0, s>>>(p);
-      else if (r.vec) norm_backward_rows_kernel<T, 4, 2, C, F, false, 512><<<grid, r.threads, 0, s>>>(p);
-      else norm_backward_rows_kernel<T, 1, 2, C, F, false, 512><<<grid, r.threads, 0, s>>>(p);
+    const bool both = a.f && a.post_weight && a.pre_weight && a.grad_h;
+    const int rc = with_flags(center, a.gate_mode == kGateFull, both, [&](auto c, auto f, auto b2) {
+      constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b2)::value;
+      using N = RowShape<T, true, F, true>;
+      using W = RowShape<T, false, F, true>;
+      if (r.narrow())
+        return launch_norm_rows(norm_backward_rows_kernel<T, 4, N::kRows, C, F, B, N::kStages, 288, 2>, grid, r,
+                                N::kSlot * N::kStages, p, s);
+      if (r.vec)
+        return launch_norm_rows(norm_backward_rows_kernel<T, 4, W::kRows, C, F, B, W::kStages, 512, 1>, grid, r,
+                                W::kSlot * W::kStages, p, s);
+      return launch_norm_rows(norm_backward_rows_kernel<T, 1, 2, C, F, B, 0, 512, 1>, grid, r, 0, p, s);
     });
+    if (rc) return rc;
   }
   if (params) {
     const NormTotals out{{a.grad_post_weight, a.grad_post_bias, a.grad_scale, a.grad_pre_weight, a.grad_pre_bias}};

@@ -102,11 +102,11 @@ struct RouteRow {
 // Warps of a forward block: their sums meet in shared memory.
 __host__ __device__ constexpr int route_warps(int v, int g) { return v * g > 256 ? 4 : 8; }
 
-// Totals over `parts` partial sums; then the loss.  One block of up to eight
-// warps, a part per warp and 32 experts at a time, parts in a fixed order.
+// Totals over `parts` partial sums; then the loss.  One block, a part per warp
+// and 32 experts at a time, parts in a fixed order.
 __device__ __forceinline__ void route_totals(const RouteParams& r, int parts) {
-  __shared__ float sp[8][33];
-  __shared__ long long sc[8][33];
+  __shared__ float sp[32][33];
+  __shared__ long long sc[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, rows = blockDim.x >> 5;
   float weighted = 0.f;  // thread y == 0: its experts' counts * p
   for (int e0 = 0; e0 < r.experts + 1; e0 += 32) {  // the last "expert" is the number of rows
@@ -114,7 +114,7 @@ __device__ __forceinline__ void route_totals(const RouteParams& r, int parts) {
     float p = 0.f;
     long long c = 0;
     if (e <= r.experts) {
-#pragma unroll 4
+#pragma unroll 10
       for (int b = y; b < parts; b += rows) {
         if (e < r.experts) p += r.partial_p[(int64_t)b * r.experts + e];
         c += r.partial_count[(int64_t)b * (r.experts + 1) + e];
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) route_forward_kernel(const RouteParams r)
   }
 }
 
-__global__ void __launch_bounds__(256) route_totals_kernel(const RouteParams r) { route_totals(r, r.blocks); }
+__global__ void __launch_bounds__(1024) route_totals_kernel(const RouteParams r) { route_totals(r, r.blocks); }
 
 // d logits = unit * dloss * p * (counts - sum_e counts_e p_e) + the gates' part:
 // renormalised, on chosen entries g * (dg - sum g dg); else on chosen entries

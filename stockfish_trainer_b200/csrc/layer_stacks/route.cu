@@ -85,7 +85,7 @@ int route_forward(const nnue_ls_route& a, void* workspace, cudaStream_t s) {
   launch_route<T>(r, false, s);
   if (r.blocks > 1) {
     count_launch();
-    route_totals_kernel<<<1, 256, 0, s>>>(r);
+    route_totals_kernel<<<1, 1024, 0, s>>>(r);
   }
   return check_launch("route_forward");
 }

@@ -76,15 +76,17 @@ typedef struct {
   void *act_grad; /* act'(z) in a form of the library's own, [rows, outputs] values as wide as dtype:
                      written by the forward when not null, read by the backward, which needs it for every
                      activation but NNUE_LS_ACT_NONE */
-  void *x_packed; /* null, or nnue_ls_linear_packed_size() bytes, 256-byte aligned: the forward leaves x there in
-                     the form its products read (fp32: 1.5 times x), the backward then reads it instead of x */
+  void *x_packed, *weight_packed; /* null, or nnue_ls_linear_packed_size() bytes, 256-byte aligned: the forward
+                                     leaves x and weight there in the form its products read (fp32: 1.5 times
+                                     their size), the backward then reads that instead */
   const void *grad_out; /* backward */
   int64_t ldg;
   void *grad_x, *grad_weight, *grad_bias; /* contiguous; null = not wanted */
 } nnue_ls_linear;
 
-/* Bytes of x_packed; 0 when x is read as it lies and x_packed has to be null. */
-size_t nnue_ls_linear_packed_size(const nnue_ls_linear *a);
+/* Bytes of x_packed (weight_packed with weight != 0); 0 when the operand is
+ * read as it lies and the buffer has to be null. */
+size_t nnue_ls_linear_packed_size(const nnue_ls_linear *a, int32_t weight);
 size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear *a);
 int nnue_ls_linear_forward(const nnue_ls_linear *a, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -45,7 +45,7 @@ auto with_type(int dtype, const F& fn) {
 // The operators' entry points per element type, each compiled in a file of its
 // own (linear_*.cu, norm_*.cu; route.cu), and the device error words of those files.
 template <typename T>
-size_t linear_packed_bytes(const nnue_ls_linear& a);
+size_t linear_packed_bytes(const nnue_ls_linear& a, bool weight);
 template <typename T>
 size_t linear_forward_bytes(const nnue_ls_linear& a);
 template <typename T>
@@ -54,8 +54,6 @@ template <typename T>
 size_t linear_backward_bytes(const nnue_ls_linear& a);
 template <typename T>
 int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s);
-template <typename T>
-bool linear_packs_x(const nnue_ls_linear& a);
 template <typename T>
 cudaError_t linear_device_errors(unsigned* flags, bool clear);
 template <typename T>

@@ -60,28 +60,41 @@ __device__ __forceinline__ void store_operand(void* dst, int64_t at, int64_t pla
   }
 }
 
-// [rows, cols] with row stride ld -> rows of ldo (a multiple of 8) values in
-// the products' layout; a thread moves 8 values.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
-                                                   void* __restrict__ dst, int64_t ldo) {
-  const int64_t groups = ldo / 8, total = rows * groups;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+// Up to two matrices brought into the products' layout by one launch: [rows,
+// cols] with row stride ld -> rows of ldo (a multiple of 8) values; a thread
+// moves 8 values.  vec: rows start on 16-byte boundaries.
+struct PackJob {
+  const void* src;
+  void* dst;
+  int64_t ld, rows, cols, ldo;
+  bool vec;
+};
+struct PackJobs {
+  PackJob job[2];
+  int64_t end[2];  // threads' work items up to each job's end
+};
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const PackJobs jobs) {
+  for (int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x; item < jobs.end[1]; item += (int64_t)gridDim.x * 256) {
+    const bool second = item >= jobs.end[0];
+    const PackJob& j = second ? jobs.job[1] : jobs.job[0];
+    const int64_t i = second ? item - jobs.end[0] : item, groups = j.ldo / 8;
     const int64_t r = i / groups, c = (i - r * groups) * 8;
+    const T* src = static_cast<const T*>(j.src) + r * j.ld + c;
     float v[8];
-    if (VEC && c + 8 <= cols) {
+    if (j.vec && c + 8 <= j.cols) {
       constexpr int W = 16 / sizeof(T);
 #pragma unroll
-      for (int j = 0; j < 8; j += W) {
-        const auto t = *reinterpret_cast<const VecT<T, W>*>(src + r * ld + c + j);
+      for (int k = 0; k < 8; k += W) {
+        const auto t = *reinterpret_cast<const VecT<T, W>*>(src + k);
 #pragma unroll
-        for (int k = 0; k < W; ++k) v[j + k] = to_f(t.v[k]);
+        for (int q = 0; q < W; ++q) v[k + q] = to_f(t.v[q]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f(src[r * ld + c + j]) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? to_f(src[k]) : 0.f;
     }
-    store_operand<T, 8>(dst, r * ldo + c, rows * ldo, v);
+    store_operand<T, 8>(j.dst, r * j.ldo + c, j.rows * j.ldo, v);
   }
 }
 
@@ -140,7 +153,8 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* __restrict__ x, 
 
 // dz = g * act'(z), written in the products' layout when dst is given, and per
 // block the fp32 column sums of the unrounded dz over a range of rows.
-// A block is `tx` groups of V columns wide and 256 / tx rows high.
+// A block is `tx` groups of V columns wide and 256 / tx rows high (its last few
+// threads may have nothing to do).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ g, int64_t ldg,
                                                  const typename Derivative<T>::Code* __restrict__ act_grad,
@@ -153,7 +167,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ g, int64_
   const int64_t n = ((int64_t)blockIdx.x * tx + x) * V;
   const int64_t m1 = min(M, ((int64_t)blockIdx.y + 1) * rows_per_block);
   float sum[V] = {};
-  if (n < N) {
+  if (n < N && y < ty) {
 #pragma unroll 4
     for (int64_t m = (int64_t)blockIdx.y * rows_per_block + y; m < m1; m += ty) {
       const auto t = *reinterpret_cast<const VecT<T, V>*>(g + m * ldg + n);

@@ -203,18 +203,30 @@ size_t pack_bytes(int64_t rows, int64_t cols) {
   return align256((size_t)rows * round8(cols) * (sizeof(T) == 4 ? 6 : 2));
 }
 
-// The matrix as an operand, packed into `buffer` where it has to be.
+// Matrices that still have to be packed before a product, in one launch.
 template <typename T>
-Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_major, void* buffer, cudaStream_t s) {
-  if (!needs_pack<T>(p, ld, rows)) return Operand{p, cols, rows, round8(ld), mn_major};
-  const int64_t ldo = round8(cols);
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows * (ldo / 8), 256), kNumSMs * 16);
-  const bool vec = reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / sizeof(T)) == 0;
-  count_launch();
-  if (vec) pack_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const T*>(p), ld, rows, cols, buffer, ldo);
-  else pack_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const T*>(p), ld, rows, cols, buffer, ldo);
-  return Operand{buffer, cols, rows, ldo, mn_major};
-}
+struct Packer {
+  PackJobs jobs{};
+  int count = 0;
+
+  // The matrix as an operand; packed into `buffer` where it cannot be read as it lies.
+  Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_major, void* buffer) {
+    if (!needs_pack<T>(p, ld, rows)) return Operand{p, cols, rows, round8(ld), mn_major};
+    const bool vec = reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / (int64_t)sizeof(T)) == 0;
+    jobs.job[count++] = PackJob{p, buffer, ld, rows, cols, round8(cols), vec};
+    return Operand{buffer, cols, rows, round8(cols), mn_major};
+  }
+  void launch(cudaStream_t s) {
+    if (count == 0) return;
+    int64_t total = 0;
+    for (int i = 0; i < 2; ++i) {
+      if (i < count) total += jobs.job[i].rows * (jobs.job[i].ldo / 8);
+      jobs.end[i] = total;
+    }
+    count_launch();
+    pack_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(total, 256), kNumSMs * 16), 256, 0, s>>>(jobs);
+  }
+};
 
 // ---- forward -------------------------------------------------------------------
 // Up to 4 rows (fp32: 8, where the other way packs its operands first) go to the
@@ -250,7 +262,7 @@ ForwardPlan plan_forward(const nnue_ls_linear& a) {
   if (few_rows<T>(a)) return p;
   p.tiles = plan_tiles(a.rows, a.outputs, a.inputs, sizeof(T) == 4 ? 3 : 1);
   p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
-  p.w = needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
+  p.w = !a.weight_packed && needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
   p.partial = p.tiles.partial_bytes(a.rows, a.outputs);
   p.total = p.x + p.w + p.partial;
   return p;
@@ -259,13 +271,10 @@ ForwardPlan plan_forward(const nnue_ls_linear& a) {
 }  // namespace
 
 template <typename T>
-bool linear_packs_x(const nnue_ls_linear& a) {
-  return !few_rows<T>(a) && needs_pack<T>(a.x, a.ldx, a.rows);
-}
-
-template <typename T>
-size_t linear_packed_bytes(const nnue_ls_linear& a) {
-  return linear_packs_x<T>(a) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+size_t linear_packed_bytes(const nnue_ls_linear& a, bool weight) {
+  if (few_rows<T>(a)) return 0;
+  if (weight) return needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
+  return needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
 }
 
 template <typename T>
@@ -283,8 +292,11 @@ int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
     return check_launch("linear_forward");
   }
   const ForwardPlan p = plan_forward<T>(a);
-  const Operand x = operand<T>(a.x, a.ldx, a.rows, a.inputs, false, a.x_packed ? a.x_packed : ws, s);
-  const Operand w = operand<T>(a.weight, a.ldw, a.outputs, a.inputs, false, ws + p.x, s);
+  Packer<T> pack;
+  const Operand x = pack.operand(a.x, a.ldx, a.rows, a.inputs, false, a.x_packed ? a.x_packed : ws);
+  const Operand w =
+      pack.operand(a.weight, a.ldw, a.outputs, a.inputs, false, a.weight_packed ? a.weight_packed : ws + p.x);
+  pack.launch(s);
   return launch_gemm<T>(x, w, a.rows, a.outputs, p.tiles, e, ws + p.x + p.w, s);
 }
 
@@ -306,7 +318,7 @@ BackwardPlan plan_backward(const nnue_ls_linear& a) {
   const bool products = a.grad_x || a.grad_weight;
   if (a.grad_x) {
     p.dx = plan_tiles(a.rows, a.inputs, a.outputs, planes);
-    p.w = needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
+    p.w = !a.weight_packed && needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
     p.partial = p.dx.partial_bytes(a.rows, a.inputs);
   }
   if (a.grad_weight) {
@@ -320,9 +332,10 @@ BackwardPlan plan_backward(const nnue_ls_linear& a) {
   auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   p.v = a.outputs % V == 0 && a.ldg % V == 0 && aligned(a.grad_out) && aligned(a.act_grad) ? (int)V : 1;
   const int64_t groups = ceil_div(a.outputs, p.v);
-  p.tx = 1;
-  while (p.tx < 32 && p.tx < groups) p.tx *= 2;
-  const int64_t wide = ceil_div(groups, p.tx), high = 256 / p.tx;
+  // no more than 32 groups across, spread evenly: 130 groups are five times 26, not four times 32 and one of 2
+  const int64_t wide = ceil_div(groups, 32);
+  p.tx = (int)ceil_div(groups, wide);
+  const int64_t high = 256 / p.tx;
   p.parts = std::max<int64_t>(1, std::min(ceil_div(a.rows, high * 4), ceil_div(kNumSMs * 8, wide)));
   p.rows_per_part = std::max<int64_t>(1, ceil_div(a.rows, p.parts));
   p.bias = a.grad_bias ? align256((size_t)p.parts * a.outputs * 4) : 0;
@@ -366,18 +379,25 @@ int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
       return check_launch("linear_backward");
     return check_launch("linear_backward");
   }
+  // what the forward left packed is read from there
+  Packer<T> pack;
+  Operand bw{}, bx{};
+  if (a.grad_x)
+    bw = a.weight_packed ? Operand{a.weight_packed, a.inputs, a.outputs, round8(a.inputs), true}
+                         : pack.operand(a.weight, a.ldw, a.outputs, a.inputs, true, w);
+  if (a.grad_weight)
+    bx = a.x_packed ? Operand{a.x_packed, a.inputs, a.rows, round8(a.inputs), true}
+                    : pack.operand(a.x, a.ldx, a.rows, a.inputs, true, x);
+  pack.launch(s);
   EpilogueParams e{};
   if (a.grad_x) {  // dx = dz W: k runs over the outputs
     e.out = a.grad_x;
-    const Operand b = operand<T>(a.weight, a.ldw, a.outputs, a.inputs, true, w, s);
-    if (int rc = launch_gemm<T>(d, b, a.rows, a.inputs, p.dx, e, partial, s)) return rc;
+    if (int rc = launch_gemm<T>(d, bw, a.rows, a.inputs, p.dx, e, partial, s)) return rc;
   }
   if (a.grad_weight) {  // dW = dz^T x: k runs over the rows
     e.out = a.grad_weight;
-    const Operand b = a.x_packed ? Operand{a.x_packed, a.inputs, a.rows, round8(a.inputs), true}
-                                 : operand<T>(a.x, a.ldx, a.rows, a.inputs, true, x, s);
     d.mn_major = true;
-    if (int rc = launch_gemm<T>(d, b, a.outputs, a.inputs, p.dw, e, partial, s)) return rc;
+    if (int rc = launch_gemm<T>(d, bx, a.outputs, a.inputs, p.dw, e, partial, s)) return rc;
   }
   return check_launch("linear_backward");
 }

@@ -112,11 +112,9 @@ int nnue_ls_device_errors(uint32_t* flags, int clear) {
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
 
-size_t nnue_ls_linear_packed_size(const nnue_ls_linear* a) {
+size_t nnue_ls_linear_packed_size(const nnue_ls_linear* a, int32_t weight) {
   if (check_linear("linear_packed_size", a) || a->rows == 0) return 0;
-  return with_type(a->dtype, [&](auto t) {
-    return linear_packed_bytes<decltype(t)>(*a);
-  });
+  return with_type(a->dtype, [&](auto t) { return linear_packed_bytes<decltype(t)>(*a, weight != 0); });
 }
 
 size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear* a) {
@@ -130,12 +128,12 @@ int nnue_ls_linear_forward(const nnue_ls_linear* a, void* workspace, size_t work
   if (!a->x || !a->weight || !a->out) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: null pointer");
   if (a->ldx < a->inputs || a->ldw < a->inputs || (a->residual && a->ldr < a->outputs))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: row stride below the row length");
-  if (reinterpret_cast<uintptr_t>(a->x_packed) % 256)
-    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed not 256-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a->x_packed) | reinterpret_cast<uintptr_t>(a->weight_packed)) % 256)
+    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed or weight_packed not 256-byte aligned");
   return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    if (a->x_packed && !linear_packs_x<T>(*a))
-      return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed given for an x that is not packed");
+    if ((a->x_packed && !linear_packed_bytes<T>(*a, false)) || (a->weight_packed && !linear_packed_bytes<T>(*a, true)))
+      return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: a buffer for an operand that is read as it lies");
     if (int rc = check_workspace("linear_forward", workspace, workspace_bytes, linear_forward_bytes<T>(*a))) return rc;
     return linear_forward<T>(*a, static_cast<char*>(workspace), static_cast<cudaStream_t>(stream));
   });
@@ -149,10 +147,10 @@ size_t nnue_ls_linear_backward_workspace_size(const nnue_ls_linear* a) {
 int nnue_ls_linear_backward(const nnue_ls_linear* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_linear("linear_backward", a)) return rc;
   if (a->rows > 0) {
-    if (!a->grad_out || (a->activation != NNUE_LS_ACT_NONE && !a->act_grad) || (a->grad_x && !a->weight) ||
+    if (!a->grad_out || (a->activation != NNUE_LS_ACT_NONE && !a->act_grad) || (a->grad_x && !a->weight && !a->weight_packed) ||
         (a->grad_weight && !a->x && !a->x_packed))
       return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_backward: null pointer");
-    if (a->ldg < a->outputs || (a->grad_x && a->ldw < a->inputs) || (a->grad_weight && !a->x_packed && a->ldx < a->inputs))
+    if (a->ldg < a->outputs || (a->grad_x && !a->weight_packed && a->ldw < a->inputs) || (a->grad_weight && !a->x_packed && a->ldx < a->inputs))
       return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_backward: row stride below the row length");
   }
   return with_type(a->dtype, [&](auto t) {

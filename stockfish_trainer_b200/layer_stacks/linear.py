@@ -31,19 +31,22 @@ def _args(x, weight, bias, residual, act):
     return a
 
 
-def _forward(x, weight, bias, residual, act, want_act_grad=False, keep_packed=False):
+def _forward(x, weight, bias, residual, act, want_act_grad=False, keep_x=False, keep_weight=False):
+    """out, act'(z), and x and the weight as the products read them (None: as they are)."""
     a = _args(x, weight, bias, residual, act)
     out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
     a.out = out.data_ptr()
-    act_grad = packed = None
+    act_grad = x_packed = w_packed = None
     if want_act_grad and act:
         act_grad = torch.empty_like(out)
         a.act_grad = act_grad.data_ptr()
-    if keep_packed:
-        packed = _native.packed_buffer(a, x.device)
-        a.x_packed = _native.ptr(packed)
+    if keep_x:
+        x_packed = _native.packed_buffer(a, False, x.device)
+    if keep_weight:
+        w_packed = _native.packed_buffer(a, True, x.device)
+    a.x_packed, a.weight_packed = _native.ptr(x_packed), _native.ptr(w_packed)
     _native.run("nnue_ls_linear_forward", a, x.device)
-    return out, act_grad, packed
+    return out, act_grad, x_packed, w_packed
 
 
 class LinearActFunction(torch.autograd.Function):
@@ -51,18 +54,19 @@ class LinearActFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        need_w = ctx.needs_input_grad[1]
-        out, act_grad, packed = _forward(x, weight, bias, residual, act, True, need_w)
-        # the packed form serves the backward in x's place
-        ctx.save_for_backward(x if packed is None and need_w else None, packed, weight, bias, act_grad)
-        ctx.meta = (act, x.shape, x.dtype)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        out, act_grad, x_packed, w_packed = _forward(x, weight, bias, residual, act, True, need_w, need_x)
+        # a packed form serves the backward in its original's place
+        ctx.save_for_backward(x if need_w and x_packed is None else None, x_packed,
+                              weight if need_x and w_packed is None else None, w_packed, act_grad)
+        ctx.meta = (act, x.shape, weight.shape, x.dtype, None if bias is None else bias.dtype)
         return out
 
     @staticmethod
     @_native.once
     def backward(ctx, grad_out):
-        x, packed, weight, bias, act_grad = ctx.saved_tensors
-        act, x_shape, dtype = ctx.meta
+        x, x_packed, weight, w_packed, act_grad = ctx.saved_tensors
+        act, x_shape, w_shape, dtype, bias_dtype = ctx.meta
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         grad_x = grad_w = grad_b = None
         if need_x or need_w or need_b:
@@ -70,24 +74,24 @@ class LinearActFunction(torch.autograd.Function):
             dev = g.device
             a = _native.Linear()
             a.rows, a.inputs = x_shape
-            a.outputs = weight.shape[0]
+            a.outputs = w_shape[0]
             a.dtype = _native.DTYPES[dtype]
-            a.bias_dtype = a.dtype if bias is None else _native.DTYPES[bias.dtype]
+            a.bias_dtype = a.dtype if bias_dtype is None else _native.DTYPES[bias_dtype]
             a.activation = act
             if x is not None:
                 a.x, a.ldx = x.data_ptr(), _native.row_stride(x)
-            a.x_packed = _native.ptr(packed)
-            a.weight, a.ldw = weight.data_ptr(), _native.row_stride(weight)
+            if weight is not None:
+                a.weight, a.ldw = weight.data_ptr(), _native.row_stride(weight)
+            a.x_packed, a.weight_packed, a.act_grad = (_native.ptr(t) for t in (x_packed, w_packed, act_grad))
             a.grad_out, a.ldg = g.data_ptr(), _native.row_stride(g)
-            a.act_grad = _native.ptr(act_grad)
             if need_x:
                 grad_x = torch.empty(x_shape, dtype=dtype, device=dev)
                 a.grad_x = grad_x.data_ptr()
             if need_w:
-                grad_w = torch.empty(weight.shape, dtype=dtype, device=dev)
+                grad_w = torch.empty(w_shape, dtype=dtype, device=dev)
                 a.grad_weight = grad_w.data_ptr()
             if need_b:
-                grad_b = torch.empty_like(bias)
+                grad_b = torch.empty(w_shape[0], dtype=bias_dtype, device=dev)
                 a.grad_bias = grad_b.data_ptr()
             _native.run("nnue_ls_linear_backward", a, dev)
         return grad_x, grad_w, grad_b, grad_out if need_r else None, None
@@ -107,8 +111,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     non-finite fp32 operand may turn an infinite sum into NaN.  Rows may be
     strided; other layouts are copied.
 
-    For the backward ``x`` (in the form its products read: for fp32 1.5 times
-    its size), ``weight`` and the activation's derivative (as wide as the
+    For the backward ``x`` and ``weight`` (in the form their products read: for
+    fp32 1.5 times their size) and the activation's derivative (as wide as the
     output) are kept; it is differentiable once.
     """
     _native.check_tensor(x, "x")

@@ -7,9 +7,10 @@ hand-written CUDA kernels behind a C ABI (include/nnue_ft.h).
 
 Submodules
   feature_transformer  autograd functions, kernel factories, tensor ops
+  layer_stacks         the dense layers behind the FT: fused linear layer, block norms, router
   positions            seeded synthetic positions + feature-index encoder
   ddp                  torchrun data-parallel step with the FT gradient allreduce
-  build                in-tree build of libnnue_ft.so
+  build                in-tree build of libnnue_ft.so and libnnue_ls.so
 """
 
 from .feature_transformer import (

@@ -7,10 +7,13 @@ and backward as hand-written kernels (include/nnue_ls.h):
   gate and residual scale;
 * ``route``       a router's top-k choice with per-expert counts and the balance
   loss.
+
+``RoutedLayerStacks`` puts them together.
 """
 
 from .linear import ACTIVATIONS, linear_act
 from .norm import block_norm
 from .router import Routing, route
+from .stacks import ResidualBlock, RoutedLayerStacks
 
-__all__ = ["ACTIVATIONS", "linear_act", "block_norm", "route", "Routing"]
+__all__ = ["ACTIVATIONS", "linear_act", "block_norm", "route", "Routing", "ResidualBlock", "RoutedLayerStacks"]

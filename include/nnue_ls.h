@@ -73,20 +73,19 @@ typedef struct {
   const void *x, *weight, *bias, *residual;
   int64_t ldx, ldw, ldr;
   void *out;      /* forward; row stride outputs */
-  void *act_grad; /* act'(z) in a form of the library's own, [rows, outputs] values as wide as dtype:
-                     written by the forward when not null, read by the backward, which needs it for every
-                     activation but NNUE_LS_ACT_NONE */
-  void *x_packed, *weight_packed; /* null, or nnue_ls_linear_packed_size() bytes, 256-byte aligned: the forward
-                                     leaves x and weight there in the form its products read (fp32: 1.5 times
-                                     their size), the backward then reads that instead */
+  /* Kept from the forward for the backward, each null or placed as nnue_ls_linear_saved_layout() says: act'(z) in a
+     form of the library's own (the backward needs it for every activation but NNUE_LS_ACT_NONE), and x and weight
+     in the form their products read, which the backward then reads instead. */
+  void *act_grad, *x_packed, *weight_packed;
   const void *grad_out; /* backward */
   int64_t ldg;
   void *grad_x, *grad_weight, *grad_bias; /* contiguous; null = not wanted */
 } nnue_ls_linear;
 
-/* Bytes of x_packed (weight_packed with weight != 0); 0 when the operand is
- * read as it lies and the buffer has to be null. */
-size_t nnue_ls_linear_packed_size(const nnue_ls_linear *a, int32_t weight);
+/* Where act_grad, x_packed and weight_packed lie in one 256-byte aligned buffer
+ * of the returned size; parts: 1, 2 and 4 ask for each.  An offset of -1: not
+ * asked for, or the operand is read as it lies and its pointer has to be null. */
+size_t nnue_ls_linear_saved_layout(const nnue_ls_linear *a, int32_t parts, int64_t offsets[3]);
 size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear *a);
 int nnue_ls_linear_forward(const nnue_ls_linear *a, void *workspace, size_t workspace_bytes, void *stream);
 

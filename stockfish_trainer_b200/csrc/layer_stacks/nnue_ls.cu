@@ -112,9 +112,23 @@ int nnue_ls_device_errors(uint32_t* flags, int clear) {
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
 
-size_t nnue_ls_linear_packed_size(const nnue_ls_linear* a, int32_t weight) {
-  if (check_linear("linear_packed_size", a) || a->rows == 0) return 0;
-  return with_type(a->dtype, [&](auto t) { return linear_packed_bytes<decltype(t)>(*a, weight != 0); });
+size_t nnue_ls_linear_saved_layout(const nnue_ls_linear* a, int32_t parts, int64_t offsets[3]) {
+  if (!offsets) return 0;
+  offsets[0] = offsets[1] = offsets[2] = -1;
+  if (check_linear("linear_saved_layout", a) || a->rows == 0) return 0;
+  return with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    const size_t bytes[3] = {
+        parts & 1 && a->activation != NNUE_LS_ACT_NONE ? (size_t)a->rows * a->outputs * sizeof(T) : 0,
+        parts & 2 ? linear_packed_bytes<T>(*a, false) : 0, parts & 4 ? linear_packed_bytes<T>(*a, true) : 0};
+    size_t total = 0;
+    for (int i = 0; i < 3; ++i) {
+      if (!bytes[i]) continue;
+      offsets[i] = (int64_t)total;
+      total += align256(bytes[i]);
+    }
+    return total;
+  });
 }
 
 size_t nnue_ls_linear_forward_workspace_size(const nnue_ls_linear* a) {

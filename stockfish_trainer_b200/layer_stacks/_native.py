@@ -35,8 +35,8 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 class Linear(ctypes.Structure):
     _fields_ = [("rows", _I64), ("inputs", _I64), ("outputs", _I64), ("dtype", _I32), ("bias_dtype", _I32),
                 ("activation", _I32), ("reserved", _I32), ("x", _P), ("weight", _P), ("bias", _P), ("residual", _P),
-                ("ldx", _I64), ("ldw", _I64), ("ldr", _I64), ("out", _P), ("act_grad", _P), ("x_packed", _P), ("weight_packed", _P),
-                ("grad_out", _P),
+                ("ldx", _I64), ("ldw", _I64), ("ldr", _I64), ("out", _P), ("act_grad", _P), ("x_packed", _P),
+                ("weight_packed", _P), ("grad_out", _P),
                 ("ldg", _I64), ("grad_x", _P), ("grad_weight", _P), ("grad_bias", _P)]
 
 
@@ -61,7 +61,7 @@ _SIGNATURES = {
     "nnue_ls_last_error": (ctypes.c_char_p, []),
     "nnue_ls_launch_count": (_U64, []),
     "nnue_ls_device_errors": (_I32, [ctypes.POINTER(ctypes.c_uint32), _I32]),
-    "nnue_ls_linear_packed_size": (_SZ, [ctypes.POINTER(Linear), _I32]),
+    "nnue_ls_linear_saved_layout": (_SZ, [ctypes.POINTER(Linear), _I32, ctypes.POINTER(_I64)]),
     "nnue_ls_linear_forward_workspace_size": (_SZ, [ctypes.POINTER(Linear)]),
     "nnue_ls_linear_forward": (_I32, [ctypes.POINTER(Linear), _P, _SZ, _P]),
     "nnue_ls_linear_backward_workspace_size": (_SZ, [ctypes.POINTER(Linear)]),
@@ -169,11 +169,22 @@ def once(backward):
     return wrapper
 
 
-def packed_buffer(a: Linear, weight: bool, device: torch.device) -> torch.Tensor | None:
-    """The buffer in which a linear forward leaves x (or the weight) packed for
-    its backward, or None where it is read as it lies."""
-    nbytes = (_lib or load()).nnue_ls_linear_packed_size(ctypes.byref(a), weight)
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def linear_saved(a: Linear, parts: int, device: torch.device) -> tuple[torch.Tensor | None, tuple]:
+    """The buffer a linear forward keeps for its backward (parts: 1 act'(z), 2 x,
+    4 weight), entered in ``a``, and the parts' offsets in it; None if it needs none."""
+    offsets = (_I64 * 3)()
+    nbytes = (_lib or load()).nnue_ls_linear_saved_layout(ctypes.byref(a), parts, offsets)
+    offsets = tuple(offsets)
+    if not nbytes:
+        return None, offsets
+    saved = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    place_saved(a, saved, offsets)
+    return saved, offsets
+
+
+def place_saved(a: Linear, saved: torch.Tensor, offsets) -> None:
+    base = saved.data_ptr()
+    a.act_grad, a.x_packed, a.weight_packed = [base + o if o >= 0 else None for o in offsets]
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -16,37 +16,20 @@ _ACT = {name: i for i, name in enumerate(ACTIVATIONS)}
 
 
 def _args(x, weight, bias, residual, act):
-    a = _native.Linear()
-    a.rows, a.inputs = x.shape
-    a.outputs = weight.shape[0]
-    a.dtype = _native.DTYPES[x.dtype]
-    a.bias_dtype = a.dtype if bias is None else _native.DTYPES[bias.dtype]
-    a.activation = act
-    a.x, a.ldx = x.data_ptr(), _native.row_stride(x)
-    a.weight, a.ldw = weight.data_ptr(), _native.row_stride(weight)
-    if bias is not None:
-        a.bias = bias.data_ptr()
-    if residual is not None:
-        a.residual, a.ldr = residual.data_ptr(), _native.row_stride(residual)
-    return a
+    dt = _native.DTYPES[x.dtype]
+    rows, inputs = x.shape
+    return _native.Linear(
+        rows, inputs, weight.shape[0], dt, dt if bias is None else _native.DTYPES[bias.dtype], act, 0, x.data_ptr(),
+        weight.data_ptr(), None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+        max(x.stride(0), inputs), max(weight.stride(0), inputs), 0 if residual is None else _native.row_stride(residual))
 
 
-def _forward(x, weight, bias, residual, act, want_act_grad=False, keep_x=False, keep_weight=False):
-    """out, act'(z), and x and the weight as the products read them (None: as they are)."""
+def _forward(x, weight, bias, residual, act):
     a = _args(x, weight, bias, residual, act)
     out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
     a.out = out.data_ptr()
-    act_grad = x_packed = w_packed = None
-    if want_act_grad and act:
-        act_grad = torch.empty_like(out)
-        a.act_grad = act_grad.data_ptr()
-    if keep_x:
-        x_packed = _native.packed_buffer(a, False, x.device)
-    if keep_weight:
-        w_packed = _native.packed_buffer(a, True, x.device)
-    a.x_packed, a.weight_packed = _native.ptr(x_packed), _native.ptr(w_packed)
     _native.run("nnue_ls_linear_forward", a, x.device)
-    return out, act_grad, x_packed, w_packed
+    return out
 
 
 class LinearActFunction(torch.autograd.Function):
@@ -55,34 +38,36 @@ class LinearActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         need_x, need_w = ctx.needs_input_grad[:2]
-        out, act_grad, x_packed, w_packed = _forward(x, weight, bias, residual, act, True, need_w, need_x)
+        a = _args(x, weight, bias, residual, act)
+        out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
+        a.out = out.data_ptr()
+        saved, offsets = _native.linear_saved(a, 1 | 2 * need_w | 4 * need_x, x.device)
+        _native.run("nnue_ls_linear_forward", a, x.device)
         # a packed form serves the backward in its original's place
-        ctx.save_for_backward(x if need_w and x_packed is None else None, x_packed,
-                              weight if need_x and w_packed is None else None, w_packed, act_grad)
-        ctx.meta = (act, x.shape, weight.shape, x.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(x if need_w and offsets[1] < 0 else None, weight if need_x and offsets[2] < 0 else None,
+                              saved)
+        ctx.meta = (act, x.shape, weight.shape, x.dtype, None if bias is None else bias.dtype, offsets)
         return out
 
     @staticmethod
     @_native.once
     def backward(ctx, grad_out):
-        x, x_packed, weight, w_packed, act_grad = ctx.saved_tensors
-        act, x_shape, w_shape, dtype, bias_dtype = ctx.meta
+        x, weight, saved = ctx.saved_tensors
+        act, x_shape, w_shape, dtype, bias_dtype, offsets = ctx.meta
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         grad_x = grad_w = grad_b = None
         if need_x or need_w or need_b:
             g = _native.rows_of(grad_out)
             dev = g.device
-            a = _native.Linear()
-            a.rows, a.inputs = x_shape
-            a.outputs = w_shape[0]
-            a.dtype = _native.DTYPES[dtype]
-            a.bias_dtype = a.dtype if bias_dtype is None else _native.DTYPES[bias_dtype]
-            a.activation = act
+            dt = _native.DTYPES[dtype]
+            a = _native.Linear(x_shape[0], x_shape[1], w_shape[0], dt,
+                               dt if bias_dtype is None else _native.DTYPES[bias_dtype], act)
             if x is not None:
                 a.x, a.ldx = x.data_ptr(), _native.row_stride(x)
             if weight is not None:
                 a.weight, a.ldw = weight.data_ptr(), _native.row_stride(weight)
-            a.x_packed, a.weight_packed, a.act_grad = (_native.ptr(t) for t in (x_packed, w_packed, act_grad))
+            if saved is not None:
+                _native.place_saved(a, saved, offsets)
             a.grad_out, a.ldg = g.data_ptr(), _native.row_stride(g)
             if need_x:
                 grad_x = torch.empty(x_shape, dtype=dtype, device=dev)
@@ -143,5 +128,5 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if _native.needs_grad(x, weight, bias, residual):
         out = LinearActFunction.apply(x, weight, bias, residual, _ACT[activation])
     else:
-        out = _forward(x, weight, bias, residual, _ACT[activation])[0]
+        out = _forward(x, weight, bias, residual, _ACT[activation])
     return out if len(shape) == 2 else out.view(shape)

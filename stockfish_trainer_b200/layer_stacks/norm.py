@@ -11,24 +11,12 @@ _KINDS = {"rms": 0, "layer": 1}
 
 
 def _args(x, f, gate, params, meta):
-    a = _native.Norm()
-    a.rows, a.width = x.shape
     dt = _native.DTYPES[x.dtype]
-    a.dtype = a.params_dtype = a.gate_dtype = dt
-    a.kind, a.gate_mode, a.gate_sigmoid, a.scale_value, a.eps = meta
-    a.x = x.data_ptr()
-    if f is not None:
-        a.f = f.data_ptr()
-    if gate is not None:
-        a.gate = gate.data_ptr()
-        a.gate_dtype = _native.DTYPES[gate.dtype]
-    ptrs = [None if t is None else t.data_ptr() for t in params]
-    a.post_weight, a.post_bias, a.scale, a.pre_weight, a.pre_bias = ptrs
-    for t in params:
-        if t is not None:
-            a.params_dtype = _native.DTYPES[t.dtype]
-            break
-    return a
+    kind, gate_mode, gate_sigmoid, scale_value, eps, params_dtype, gate_dtype = meta
+    rows, width = x.shape
+    return _native.Norm(rows, width, dt, params_dtype, gate_dtype, kind, gate_mode, gate_sigmoid, scale_value, eps, 0,
+                        x.data_ptr(), None if f is None else f.data_ptr(), None if gate is None else gate.data_ptr(),
+                        *[None if t is None else t.data_ptr() for t in params])
 
 
 def _forward(x, f, gate, params, meta, want_stats):
@@ -67,8 +55,12 @@ class BlockNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         a = _args(x, f, gate, params, ctx.meta)
         a.stats = stats.data_ptr()
-        held = [None if g is None else g.contiguous() for g in (grad_y, grad_h)]
-        a.grad_y, a.grad_h = (_native.ptr(g) for g in held)
+        if grad_y is not None:
+            grad_y = grad_y.contiguous()
+            a.grad_y = grad_y.data_ptr()
+        if grad_h is not None:
+            grad_h = grad_h.contiguous()
+            a.grad_h = grad_h.data_ptr()
         grads = [torch.empty_like(t) if n and t is not None else None for n, t in zip(need, (x, f, gate, *params))]
         (a.grad_x, a.grad_f, a.grad_gate, a.grad_post_weight, a.grad_post_bias, a.grad_scale, a.grad_pre_weight,
          a.grad_pre_bias) = [None if g is None else g.data_ptr() for g in grads]
@@ -158,7 +150,8 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
         gate = gate.contiguous()
     x2 = (x if flat else x.reshape(-1, width)).contiguous()
     f2 = None if f is None else (f if flat else f.reshape(-1, width)).contiguous()
-    meta = (_KINDS[kind], mode, int(gate_activation == "sigmoid"), scale_value, float(eps))
+    meta = (_KINDS[kind], mode, gate_activation == "sigmoid", scale_value, float(eps),
+            _native.DTYPES[params_dtype or dt], _native.DTYPES[dt if gate is None else gate.dtype])
     if _native.needs_grad(x2, f2, gate, *params):
         y, h = BlockNormFunction.apply(x2, f2, gate, *params, meta)
     else:

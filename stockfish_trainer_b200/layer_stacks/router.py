@@ -24,13 +24,10 @@ class Routing(NamedTuple):
 
 
 def _args(logits, valid, k, renormalize, indices, gates, counts, loss):
-    a = _native.Route()
-    a.rows, a.experts = logits.shape
-    a.k, a.dtype, a.renormalize = k, _native.DTYPES[logits.dtype], renormalize
-    a.logits, a.ld = logits.data_ptr(), _native.row_stride(logits)
-    a.valid = _native.ptr(valid)
-    a.indices, a.gates, a.counts, a.loss = indices.data_ptr(), gates.data_ptr(), counts.data_ptr(), loss.data_ptr()
-    return a
+    rows, experts = logits.shape
+    return _native.Route(rows, experts, k, _native.DTYPES[logits.dtype], renormalize, logits.data_ptr(),
+                         max(logits.stride(0), experts), None if valid is None else valid.data_ptr(),
+                         indices.data_ptr(), gates.data_ptr(), counts.data_ptr(), loss.data_ptr())
 
 
 def _forward(logits, valid, k, renormalize):
@@ -59,8 +56,12 @@ class RouteFunction(torch.autograd.Function):
     def backward(ctx, _indices, grad_gates, _counts, grad_loss):
         logits, valid, indices, gates, counts, loss = ctx.saved_tensors
         a = _args(logits, valid, *ctx.meta, indices, gates, counts, loss)
-        held = [None if g is None else g.contiguous() for g in (grad_gates, grad_loss)]
-        a.grad_gates, a.grad_loss = (_native.ptr(g) for g in held)
+        if grad_gates is not None:
+            grad_gates = grad_gates.contiguous()
+            a.grad_gates = grad_gates.data_ptr()
+        if grad_loss is not None:
+            grad_loss = grad_loss.contiguous()
+            a.grad_loss = grad_loss.data_ptr()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         a.grad_logits = grad.data_ptr()
         _native.run("nnue_ls_route_backward", a, logits.device)

@@ -74,6 +74,27 @@ def test_linear_refusals():
     assert lib.nnue_ls_linear_backward(ctypes.byref(a), some + 8, need, None) == _native.ERR_WORKSPACE
 
 
+def test_linear_saved_layout():
+    """act'(z), x and the weight in one buffer: only what is asked for and needed, 256-byte aligned, no overlap."""
+    lib = _native.load()
+    off = (ctypes.c_int64 * 3)()
+    a = _linear(rows=100, inputs=40, outputs=24, ldx=40, ldw=40, x=4096, weight=4096, activation=4)
+    total = lib.nnue_ls_linear_saved_layout(ctypes.byref(a), 7, off)  # fp32: all three
+    assert list(off) == [0, 9728, 9728 + 24064] and total == 9728 + 24064 + 5888
+    assert lib.nnue_ls_linear_saved_layout(ctypes.byref(a), 2, off) == 24064 and list(off) == [-1, 0, -1]
+    a.dtype = a.bias_dtype = 1  # aligned 16-bit operands are read as they lie
+    assert lib.nnue_ls_linear_saved_layout(ctypes.byref(a), 7, off) == 4864 and list(off) == [0, -1, -1]
+    a.ldx = 41
+    assert lib.nnue_ls_linear_saved_layout(ctypes.byref(a), 6, off) == 8192 and list(off) == [-1, 0, -1]
+    a.activation = 0
+    assert lib.nnue_ls_linear_saved_layout(ctypes.byref(a), 1, off) == 0
+    a.x_packed = 4096 + 8
+    a.out = 4096
+    assert lib.nnue_ls_linear_forward(ctypes.byref(a), None, 0, None) == _native.ERR_INVALID_ARGUMENT
+    a.x_packed, a.ldx = 4096, 40  # a buffer for an x that is not packed
+    assert lib.nnue_ls_linear_forward(ctypes.byref(a), None, 0, None) == _native.ERR_INVALID_ARGUMENT
+
+
 def test_norm_refusals():
     lib = _native.load()
     some = 4096

@@ -254,6 +254,28 @@ def test_gradient_against_differences(cuda):
             assert abs(num - ana) <= 2e-3 * float((g.double() * d).abs().sum()) + 1e-3, name
 
 
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 elements: the last rows equal those of a call on them alone, bit for bit."""
+    rows, width = 2_100_037, 1032
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, width, generator=g, device=cuda, dtype=torch.bfloat16)
+    f = torch.randn(rows, width, generator=g, device=cuda, dtype=torch.bfloat16)
+    w = torch.rand(width, device=cuda) + 0.5
+    y, h = block_norm(x, f, post_weight=w, pre_weight=w)
+    for part in (slice(rows - 64, rows), slice(0, 64)):
+        y2, h2 = block_norm(x[part], f[part], post_weight=w, pre_weight=w)
+        assert torch.equal(y[part], y2) and torch.equal(h[part], h2)
+    del y, h
+    xx, ff = x.requires_grad_(), f.requires_grad_()
+    out = block_norm(xx, ff, post_weight=w, pre_weight=w)[1]
+    dx, df = torch.autograd.grad(out, [xx, ff], out.detach())
+    part = slice(rows - 64, rows)
+    xs, fs = x[part].detach().requires_grad_(), f[part].detach().requires_grad_()
+    o2 = block_norm(xs, fs, post_weight=w, pre_weight=w)[1]
+    for a, b in zip((dx, df), torch.autograd.grad(o2, [xs, fs], out[part].detach())):
+        assert torch.equal(a[part], b)
+
+
 def test_nan_stays_in_its_row(cuda):
     t, gy, gh = _make(20, 136, torch.bfloat16, 7, gate="row")
     dev = {k: v.cuda() for k, v in t.items()}

@@ -259,6 +259,27 @@ def test_infinities_and_nan_reach_their_own_rows_only(cuda):
         assert out[3].isnan().all() and not out[131].isfinite().any()
 
 
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 elements of the output and its gradient; x, being narrow, holds whole numbers, so that the sums
+    over two million rows are exact."""
+    M, K, N = 2_100_037, 8, 1032
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(-1, 2, (M, K), generator=g, device=cuda).bfloat16()
+    w = (torch.randint(-2, 3, (N, K), generator=g, device=cuda) / 4).bfloat16()
+    xx, ww = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = linear_act(xx, ww)
+    assert out.numel() > 2**31
+    for rows in (slice(0, 300), slice(M - 300, M), slice(M // 2, M // 2 + 300)):
+        assert torch.equal(out[rows], (x[rows].double() @ w.double().t()).bfloat16())
+    go = torch.zeros(M, N, device=cuda, dtype=torch.bfloat16)
+    go[-5000:] = 1
+    go[:5000] = -1
+    dx, dw = torch.autograd.grad(out, [xx, ww], go)
+    assert torch.equal(dx[-5000:], w.double().sum(0).bfloat16().expand(5000, K)) and (dx[5000:-5000] == 0).all()
+    want = x[-5000:].double().sum(0) - x[:5000].double().sum(0)
+    assert torch.equal(dw, want.bfloat16().expand(N, K))
+
+
 def test_other_stream_and_graph(cuda):
     x, w, b, r, go = _make(300, 64, 48, torch.bfloat16, seed=7)
     want = linear_act(x, w, b, residual=r, activation="gelu")

@@ -154,6 +154,25 @@ def test_many_rows(cuda):
     assert abs(float(r.balance_loss) - float(loss)) < 1e-5
 
 
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 logits: the last rows' choices, gates and gradients equal those of a call on them alone."""
+    rows, experts = 33_600_001, 64
+    l = torch.empty(rows, experts, device=cuda, dtype=torch.bfloat16)
+    l[:] = torch.randn(1, experts, device=cuda).bfloat16()
+    tail = torch.randn(1000, experts, generator=torch.Generator().manual_seed(2)).bfloat16().to(cuda)
+    l[-1000:] = tail
+    ll = l.requires_grad_()
+    r = route(ll, 1)
+    want = route(tail, 1)
+    assert torch.equal(r.indices[-1000:], want.indices) and torch.equal(r.gates[-1000:], want.gates)
+    assert int(r.counts.sum()) == rows
+    dl, = torch.autograd.grad(r.gates, ll, torch.ones_like(r.gates))
+    t2 = tail.clone().requires_grad_()
+    r2 = route(t2, 1)
+    d2, = torch.autograd.grad(r2.gates, t2, torch.ones_like(r2.gates))
+    assert torch.equal(dl[-1000:], d2)
+
+
 def test_no_rows(cuda):
     l = torch.empty(0, 8, device=cuda, requires_grad=True)
     r = route(l, 2)

@@ -138,13 +138,13 @@ def _lookup(func: str):
     return found
 
 
-def run(func: str, args: ctypes.Structure, device: torch.device) -> None:
-    """Enqueue ``func(args)`` on the device's current stream.  Where the call
-    takes a workspace, it comes from PyTorch's caching allocator."""
-    index = device.index
+def run(func: str, args: ctypes.Structure, like: torch.Tensor) -> None:
+    """Enqueue ``func(args)`` on the current stream of ``like``'s device.  Where
+    the call takes a workspace, it comes from PyTorch's caching allocator."""
+    index = like.get_device()
     if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
-            return run(func, args, device)
+        with torch.cuda.device(index):
+            return run(func, args, like)
     fn, size = _calls.get(func) or _lookup(func)
     ref = ctypes.byref(args)
     stream = torch._C._cuda_getCurrentRawStream(index)
@@ -153,8 +153,8 @@ def run(func: str, args: ctypes.Structure, device: torch.device) -> None:
     else:
         nbytes = size(ref)
         # the caching allocator returns 512-byte aligned blocks; the ABI needs 256
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
-        rc = fn(ref, ws, nbytes, stream)
+        ws = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        rc = fn(ref, None if ws is None else ws.data_ptr(), nbytes, stream)
     if rc != OK:
         check(func, rc)
 
@@ -169,7 +169,7 @@ def once(backward):
     return wrapper
 
 
-def linear_saved(a: Linear, parts: int, device: torch.device) -> tuple[torch.Tensor | None, tuple]:
+def linear_saved(a: Linear, parts: int, like: torch.Tensor) -> tuple[torch.Tensor | None, tuple]:
     """The buffer a linear forward keeps for its backward (parts: 1 act'(z), 2 x,
     4 weight), entered in ``a``, and the parts' offsets in it; None if it needs none."""
     offsets = (_I64 * 3)()
@@ -177,7 +177,7 @@ def linear_saved(a: Linear, parts: int, device: torch.device) -> tuple[torch.Ten
     offsets = tuple(offsets)
     if not nbytes:
         return None, offsets
-    saved = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    saved = like.new_empty(nbytes, dtype=torch.uint8)
     place_saved(a, saved, offsets)
     return saved, offsets
 
@@ -191,32 +191,35 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def check_tensor(t: torch.Tensor, name: str, device: torch.device | None = None, dtypes=tuple(DTYPES)) -> None:
+def check_tensor(t: torch.Tensor, name: str, dtypes=DTYPES, index: int | None = None) -> int:
+    """Refuses what is not a CUDA tensor of one of ``dtypes`` (on GPU ``index``); returns its GPU's index."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if device is None:
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-    elif t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}" if t.is_cuda else
-                         f"{name} must be a CUDA tensor")
+    at = t.get_device()
+    if at < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if index is not None and at != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    return at
+
+
+# a type alone, and beside fp32: what parameters may have next to 16-bit tensors
+ALONE = {dt: (dt,) for dt in DTYPES}
+OR_F32 = {dt: (dt,) if dt == torch.float32 else (dt, torch.float32) for dt in DTYPES}
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """``t`` as a matrix of its last dimension's rows, with unit column stride
     and rows that do not overlap; copied only where the layout asks for it."""
     m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if not m.is_contiguous():
-        if (m.stride(1) != 1 and m.shape[1] > 1) or (m.stride(0) < m.shape[1] and m.shape[0] > 1):
-            m = m.contiguous()
+    if m.is_contiguous():
+        return m
+    if (m.stride(1) != 1 and m.shape[1] > 1) or (m.stride(0) < m.shape[1] and m.shape[0] > 1):
+        return m.contiguous()
     return m
 
 
 def row_stride(m: torch.Tensor) -> int:
     return max(m.stride(0), m.shape[1])
-
-
-def needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

@@ -26,9 +26,9 @@ def _args(x, weight, bias, residual, act):
 
 def _forward(x, weight, bias, residual, act):
     a = _args(x, weight, bias, residual, act)
-    out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
+    out = x.new_empty((a.rows, a.outputs))
     a.out = out.data_ptr()
-    _native.run("nnue_ls_linear_forward", a, x.device)
+    _native.run("nnue_ls_linear_forward", a, x)
     return out
 
 
@@ -39,10 +39,10 @@ class LinearActFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         need_x, need_w = ctx.needs_input_grad[:2]
         a = _args(x, weight, bias, residual, act)
-        out = torch.empty(a.rows, a.outputs, dtype=x.dtype, device=x.device)
+        out = x.new_empty((a.rows, a.outputs))
         a.out = out.data_ptr()
-        saved, offsets = _native.linear_saved(a, 1 | 2 * need_w | 4 * need_x, x.device)
-        _native.run("nnue_ls_linear_forward", a, x.device)
+        saved, offsets = _native.linear_saved(a, 1 | 2 * need_w | 4 * need_x, x)
+        _native.run("nnue_ls_linear_forward", a, x)
         # a packed form serves the backward in its original's place
         ctx.save_for_backward(x if need_w and offsets[1] < 0 else None, weight if need_x and offsets[2] < 0 else None,
                               saved)
@@ -58,7 +58,6 @@ class LinearActFunction(torch.autograd.Function):
         grad_x = grad_w = grad_b = None
         if need_x or need_w or need_b:
             g = _native.rows_of(grad_out)
-            dev = g.device
             dt = _native.DTYPES[dtype]
             a = _native.Linear(x_shape[0], x_shape[1], w_shape[0], dt,
                                dt if bias_dtype is None else _native.DTYPES[bias_dtype], act)
@@ -70,15 +69,15 @@ class LinearActFunction(torch.autograd.Function):
                 _native.place_saved(a, saved, offsets)
             a.grad_out, a.ldg = g.data_ptr(), _native.row_stride(g)
             if need_x:
-                grad_x = torch.empty(x_shape, dtype=dtype, device=dev)
+                grad_x = g.new_empty(x_shape)
                 a.grad_x = grad_x.data_ptr()
             if need_w:
-                grad_w = torch.empty(w_shape, dtype=dtype, device=dev)
+                grad_w = g.new_empty(w_shape)
                 a.grad_weight = grad_w.data_ptr()
             if need_b:
-                grad_b = torch.empty(w_shape[0], dtype=bias_dtype, device=dev)
+                grad_b = g.new_empty(w_shape[0], dtype=bias_dtype)
                 a.grad_bias = grad_b.data_ptr()
-            _native.run("nnue_ls_linear_backward", a, dev)
+            _native.run("nnue_ls_linear_backward", a, g)
         return grad_x, grad_w, grad_b, grad_out if need_r else None, None
 
 
@@ -100,33 +99,40 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     fp32 1.5 times their size) and the activation's derivative (as wide as the
     output) are kept; it is differentiable once.
     """
-    _native.check_tensor(x, "x")
-    dev, dt = x.device, x.dtype
-    _native.check_tensor(weight, "weight", dev, (dt,))
-    if activation not in _ACT:
+    act = _ACT.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
-    n = weight.shape[0]
-    if n < 1 or weight.shape[1] < 1:
+    check = _native.check_tensor
+    gpu = check(x, "x")
+    dt = x.dtype
+    alone = _native.ALONE[dt]
+    check(weight, "weight", alone, gpu)
+    x_shape, w_shape = x.shape, weight.shape
+    if len(x_shape) < 1 or len(w_shape) != 2 or x_shape[-1] != w_shape[1]:
+        raise ValueError(f"x {tuple(x_shape)} and weight {tuple(w_shape)} do not match")
+    n = w_shape[0]
+    if n < 1 or w_shape[1] < 1:
         raise ValueError("weight must not be empty")
-    shape = x.shape[:-1] + (n,)
+    grad = x.requires_grad or weight.requires_grad
     if bias is not None:
-        _native.check_tensor(bias, "bias", dev, (dt,) if dt == torch.float32 else (dt, torch.float32))
+        check(bias, "bias", _native.OR_F32[dt], gpu)
         if bias.dim() != 1 or bias.shape[0] != n:
             raise ValueError(f"bias must have shape ({n},), got {tuple(bias.shape)}")
         bias = bias.contiguous()
+        grad = grad or bias.requires_grad
+    shape = x_shape[:-1] + (n,)
     if residual is not None:
-        _native.check_tensor(residual, "residual", dev, (dt,))
+        check(residual, "residual", alone, gpu)
         if residual.shape != shape:
             try:
                 residual = residual.expand(shape)
             except RuntimeError:
                 raise ValueError(f"residual {tuple(residual.shape)} does not broadcast to {tuple(shape)}") from None
         residual = _native.rows_of(residual)
+        grad = grad or residual.requires_grad
     x, weight = _native.rows_of(x), _native.rows_of(weight)
-    if _native.needs_grad(x, weight, bias, residual):
-        out = LinearActFunction.apply(x, weight, bias, residual, _ACT[activation])
+    if grad and torch.is_grad_enabled():
+        out = LinearActFunction.apply(x, weight, bias, residual, act)
     else:
-        out = _forward(x, weight, bias, residual, _ACT[activation])
+        out = _forward(x, weight, bias, residual, act)
     return out if len(shape) == 2 else out.view(shape)

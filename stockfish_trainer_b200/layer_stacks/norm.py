@@ -8,6 +8,7 @@ import torch
 from . import _native
 
 _KINDS = {"rms": 0, "layer": 1}
+_PARAMS = ("post_weight", "post_bias", "residual_scale", "pre_weight", "pre_bias")
 
 
 def _args(x, f, gate, params, meta):
@@ -29,9 +30,9 @@ def _forward(x, f, gate, params, meta, want_stats):
         h = torch.empty_like(x)
         a.h = h.data_ptr()
     if want_stats:
-        stats = torch.empty(x.shape[0], 4, dtype=torch.float32, device=x.device)
+        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
         a.stats = stats.data_ptr()
-    _native.run("nnue_ls_norm_forward", a, x.device)
+    _native.run("nnue_ls_norm_forward", a, x)
     return y, h, stats
 
 
@@ -64,7 +65,7 @@ class BlockNormFunction(torch.autograd.Function):
         grads = [torch.empty_like(t) if n and t is not None else None for n, t in zip(need, (x, f, gate, *params))]
         (a.grad_x, a.grad_f, a.grad_gate, a.grad_post_weight, a.grad_post_bias, a.grad_scale, a.grad_pre_weight,
          a.grad_pre_bias) = [None if g is None else g.data_ptr() for g in grads]
-        _native.run("nnue_ls_norm_backward", a, x.device)
+        _native.run("nnue_ls_norm_backward", a, x)
         return (*grads, None)
 
 
@@ -89,18 +90,21 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
     are held in fp32, h is normalised from the unrounded y, and each output is
     rounded once.  Differentiable once, in every tensor argument.
     """
-    _native.check_tensor(x, "x")
-    dev, dt = x.device, x.dtype
-    mixed = (dt,) if dt == torch.float32 else (dt, torch.float32)
+    check = _native.check_tensor
+    gpu = check(x, "x")
+    dt = x.dtype
+    alone, mixed = _native.ALONE[dt], _native.OR_F32[dt]
     if kind not in _KINDS:
         raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
     if gate_activation not in ("none", "sigmoid"):
         raise ValueError(f"gate_activation must be 'none' or 'sigmoid', got {gate_activation!r}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= _native.NORM_MAX_WIDTH:
-        raise ValueError(f"x must be [..., width] with 1 <= width <= {_native.NORM_MAX_WIDTH}, got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) < 1 or not 1 <= shape[-1] <= _native.NORM_MAX_WIDTH:
+        raise ValueError(f"x must be [..., width] with 1 <= width <= {_native.NORM_MAX_WIDTH}, got {tuple(shape)}")
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    shape, width = x.shape, x.shape[-1]
+    width = shape[-1]
+    grad = x.requires_grad
     scale, scale_value = None, 1.0
     if isinstance(residual_scale, torch.Tensor):
         scale = residual_scale
@@ -112,33 +116,34 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
         if pre_weight is None:
             raise ValueError("nothing to do: give f, pre_weight or both")
     else:
-        _native.check_tensor(f, "f", dev, (dt,))
+        check(f, "f", alone, gpu)
         if f.shape != shape:
             raise ValueError(f"f {tuple(f.shape)} must have x's shape {tuple(shape)}")
+        grad = grad or f.requires_grad
     if (post_bias is not None and post_weight is None) or (pre_bias is not None and pre_weight is None):
         raise ValueError("a norm's bias needs its weight")
-    params, params_dtype = [], None
-    for name, t in zip(("post_weight", "post_bias", "residual_scale", "pre_weight", "pre_bias"),
-                       (post_weight, post_bias, scale, pre_weight, pre_bias)):
+    params, params_dtype = [post_weight, post_bias, scale, pre_weight, pre_bias], None
+    for i, t in enumerate(params):
         if t is not None:
-            _native.check_tensor(t, name, dev, mixed if params_dtype is None else (params_dtype,))
+            name = _PARAMS[i]
+            check(t, name, mixed if params_dtype is None else _native.ALONE[params_dtype], gpu)
             params_dtype = t.dtype
             if t.dim() != 1 or t.shape[0] != width:
                 raise ValueError(f"{name} must have shape ({width},), got {tuple(t.shape)}")
-            t = t.contiguous()
-        params.append(t)
+            params[i] = t.contiguous()
+            grad = grad or t.requires_grad
     # the common case, matrices, adds no view to the graph
     flat = len(shape) == 2
     mode = 0
     if gate is not None:
         if gate.shape == shape[:-1] or (gate.shape == shape[:-1] + (1,) and width > 1):
             mode = 1
-            _native.check_tensor(gate, "gate", dev, mixed)
+            check(gate, "gate", mixed, gpu)
             if gate.dim() != 1:
                 gate = gate.reshape(-1)
         else:
             mode = 2
-            _native.check_tensor(gate, "gate", dev, (dt,))
+            check(gate, "gate", alone, gpu)
             if gate.shape != shape:
                 try:
                     gate = gate.expand(shape)
@@ -148,11 +153,12 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
             if not flat:
                 gate = gate.reshape(-1, width)
         gate = gate.contiguous()
+        grad = grad or gate.requires_grad
     x2 = (x if flat else x.reshape(-1, width)).contiguous()
     f2 = None if f is None else (f if flat else f.reshape(-1, width)).contiguous()
     meta = (_KINDS[kind], mode, gate_activation == "sigmoid", scale_value, float(eps),
             _native.DTYPES[params_dtype or dt], _native.DTYPES[dt if gate is None else gate.dtype])
-    if _native.needs_grad(x2, f2, gate, *params):
+    if grad and torch.is_grad_enabled():
         y, h = BlockNormFunction.apply(x2, f2, gate, *params, meta)
     else:
         y, h, _ = _forward(x2, f2, gate, params, meta, False)

@@ -32,12 +32,11 @@ def _args(logits, valid, k, renormalize, indices, gates, counts, loss):
 
 def _forward(logits, valid, k, renormalize):
     rows, experts = logits.shape
-    dev = logits.device
-    indices = torch.empty(rows, k, dtype=torch.int64, device=dev)
-    gates = torch.empty(rows, k, dtype=torch.float32, device=dev)
-    counts = torch.empty(experts, dtype=torch.int64, device=dev)
-    loss = torch.empty(2, dtype=torch.float32, device=dev)
-    _native.run("nnue_ls_route_forward", _args(logits, valid, k, renormalize, indices, gates, counts, loss), dev)
+    indices = logits.new_empty((rows, k), dtype=torch.int64)
+    gates = logits.new_empty((rows, k), dtype=torch.float32)
+    counts = logits.new_empty(experts, dtype=torch.int64)
+    loss = logits.new_empty(2, dtype=torch.float32)
+    _native.run("nnue_ls_route_forward", _args(logits, valid, k, renormalize, indices, gates, counts, loss), logits)
     return indices, gates, counts, loss
 
 
@@ -62,9 +61,9 @@ class RouteFunction(torch.autograd.Function):
         if grad_loss is not None:
             grad_loss = grad_loss.contiguous()
             a.grad_loss = grad_loss.data_ptr()
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = logits.new_empty(logits.shape)
         a.grad_logits = grad.data_ptr()
-        _native.run("nnue_ls_route_backward", a, logits.device)
+        _native.run("nnue_ls_route_backward", a, logits)
         return grad, None, None, None
 
 
@@ -87,21 +86,22 @@ def route(logits: torch.Tensor, k: int, *, valid: torch.Tensor | None = None, re
     the counts enter them as constants.  Probabilities, gates and sums are held
     in fp32.
     """
-    _native.check_tensor(logits, "logits")
-    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= _native.MAX_EXPERTS:
+    gpu = _native.check_tensor(logits, "logits")
+    shape = logits.shape
+    if len(shape) < 1 or not 1 <= shape[-1] <= _native.MAX_EXPERTS:
         raise ValueError(f"logits must be [..., experts] with 1 <= experts <= {_native.MAX_EXPERTS}, "
-                         f"got {tuple(logits.shape)}")
+                         f"got {tuple(shape)}")
     k = int(k)
-    if not 1 <= k <= logits.shape[-1]:
-        raise ValueError(f"k must be in [1, {logits.shape[-1]}], got {k}")
-    shape = logits.shape[:-1]
+    if not 1 <= k <= shape[-1]:
+        raise ValueError(f"k must be in [1, {shape[-1]}], got {k}")
+    shape = shape[:-1]
     if valid is not None:
-        _native.check_tensor(valid, "valid", logits.device, (torch.bool,))
+        _native.check_tensor(valid, "valid", (torch.bool,), gpu)
         if valid.shape != shape:
             raise ValueError(f"valid must have shape {tuple(shape)}, got {tuple(valid.shape)}")
         valid = valid.reshape(-1).contiguous()
     rows = _native.rows_of(logits)
-    if _native.needs_grad(rows):
+    if logits.requires_grad and torch.is_grad_enabled():
         indices, gates, counts, loss = RouteFunction.apply(rows, valid, k, bool(renormalize))
     else:
         indices, gates, counts, loss = _forward(rows, valid, k, bool(renormalize))

@@ -5,12 +5,9 @@
 // K-major, the input gradient reads W MN-major, the weight gradient reads dz
 // and x MN-major, so no operand is ever transposed in memory.
 //
-// fp32 operands become three bf16 planes whose sum is the value (8 + 8 + 8
+// fp32 operands come as three bf16 planes whose sum is the value (8 + 8 + 8
 // bits, exact); six of the nine plane products are formed, the three left out
-// are below 2^-23 of the product.  The large operand x is split on its way
-// through shared memory (RAW): warps 2 and 3 turn each fp32 tile into planes
-// while the products of the tile before run, so x is read once, as fp32; the
-// other operand (a weight, or dz, whose own pass writes it) comes as planes.
+// are below 2^-23 of the product.
 //
 // One persistent block per SM (or a pair of blocks on two SMs, CG = 2, sharing
 // a 256-row tile: each holds half of A's rows and half of B's, which halves
@@ -34,9 +31,7 @@ constexpr uint64_t kWaitLimitNs = 4000000000ull;
 
 // Shared memory: stages of A and B tiles, one transpose buffer per epilogue
 // warp, barriers.  Planes = 1: 64 k values per stage; 3: 32.
-enum Raw : int { kNoRaw = 0, kRawA = 1, kRawB = 2 };  // which operand arrives as fp32: A K-major, B MN-major
-
-template <int PLANES, int CG, int RAW>
+template <int PLANES, int CG>
 struct GemmShape {
   static constexpr int kBK = PLANES == 1 ? 64 : 32;
   static constexpr int kMaxBN = PLANES == 3 && CG == 1 ? 128 : 256;   // columns of C per tile
@@ -44,10 +39,9 @@ struct GemmShape {
   static constexpr int kRowsB = kMaxBN / CG;                         // rows of B held by one block
   static constexpr int kPlaneA = kTileM * kBK * 2, kPlaneB = kRowsB * kBK * 2;
   static constexpr int kStage = PLANES * (kPlaneA + kPlaneB);
-  static constexpr int kStages = RAW ? 2 : PLANES == 1 && CG == 2 ? 5 : 3;
-  static constexpr int kRawTile = RAW ? 128 * 32 * 4 : 0, kRawStages = RAW ? 3 : 0;  // fp32 tiles on their way
+  static constexpr int kStages = PLANES == 1 && CG == 2 ? 5 : 3;
   static constexpr int kTranspose = kEpilogueWarps * 32 * 32 * 4;
-  static constexpr int kSmem = 1024 + kStages * kStage + kRawStages * kRawTile + kTranspose + 256;
+  static constexpr int kSmem = 1024 + kStages * kStage + kTranspose + 256;
   // k blocks summed in TMEM before the epilogue warps take the sum into
   // registers.  The tensor cores' running sums lose up to a unit of the last
   // place per instruction; with fp32 operands that would show, so there a
@@ -81,21 +75,13 @@ __device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
       " mbarrier.arrive.shared::cluster.b64 _, [ra];\n}" ::"r"(bar)
       : "memory");
 }
-// The same, with this thread's writes before it seen by who waits there.
-__device__ __forceinline__ void mbar_release_leader(uint32_t bar) {
-  asm volatile(
-      "{\n .reg .b32 ra;\n mapa.shared::cluster.u32 ra, %0, 0;\n"
-      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n}" ::"r"(bar)
-      : "memory");
-}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
       : "r"(bar), "r"(parity)
       : "memory");
@@ -227,79 +213,22 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int mn_major) {
 
 // map_a, map_b: [planes][rows][columns], the contiguous direction first.  They are parameters of their own because
 // their address is taken: parameters whose address is not are read as constants.
-// ---- fp32 tiles ------------------------------------------------------------------
-// Eight fp32 values (two 16-byte pieces) as a 16-byte piece of each plane: each
-// plane takes the leading 8 bits of what is left.  An infinity leaves NaN in
-// the second plane, so its sums become NaN.
-__device__ __forceinline__ void split8(const float4& lo, const float4& hi, uint4 (&plane)[3]) {
-  const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  uint32_t q[3][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    q[0][i] = __float_as_uint(v[i]);
-    const float r1 = v[i] - __uint_as_float(q[0][i] & 0xffff0000u);
-    q[1][i] = __float_as_uint(r1);
-    q[2][i] = __float_as_uint(r1 - __uint_as_float(q[1][i] & 0xffff0000u));
-  }
-#pragma unroll
-  for (int k = 0; k < 3; ++k)
-    plane[k] = make_uint4(__byte_perm(q[k][0], q[k][1], 0x7632), __byte_perm(q[k][2], q[k][3], 0x7632),
-                          __byte_perm(q[k][4], q[k][5], 0x7632), __byte_perm(q[k][6], q[k][7], 0x7632));
-}
-
-// One warp's half of a tile.  Both sides are swizzled as TMA and the products
-// expect; the lanes' order keeps eight neighbours on different banks.
-// A, K-major: 128 rows of 32 values; fp32 rows of 128 bytes, plane rows of 64.
-__device__ __forceinline__ void split_tile_a(const uint8_t* raw, uint8_t* planes, int plane_bytes, int half, int lane) {
-#pragma unroll 2
-  for (int it = 0; it < 8; ++it) {
-    const int i = it * 64 + half * 32 + lane, r = i >> 2, c = i & 3, x = r & 7;
-    const float4 lo = *reinterpret_cast<const float4*>(raw + r * 128 + ((2 * c ^ x) << 4));
-    const float4 hi = *reinterpret_cast<const float4*>(raw + r * 128 + (((2 * c + 1) ^ x) << 4));
-    uint4 q[3];
-    split8(lo, hi, q);
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-      *reinterpret_cast<uint4*>(planes + k * plane_bytes + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = q[k];
-  }
-}
-// B, MN-major: per 64 columns, 32 rows (one per k) of 64 values; fp32 as two
-// boxes of 32 columns, 128 bytes a row, plane rows of 128 bytes.
-__device__ __forceinline__ void split_tile_b(const uint8_t* raw, uint8_t* planes, int plane_bytes, int blocks, int half,
-                                             int lane) {
-#pragma unroll 2
-  for (int it = 0; it < blocks * 4; ++it) {
-    const int i = it * 64 + half * 32 + lane, b = i >> 8, j = i & 255;
-    const int r = (j >> 2) & 31, h = j >> 7, c = (j & 3), x = r & 7;
-    const uint8_t* src = raw + (b * 2 + h) * 4096 + r * 128;
-    const float4 lo = *reinterpret_cast<const float4*>(src + ((2 * c ^ x) << 4));
-    const float4 hi = *reinterpret_cast<const float4*>(src + (((2 * c + 1) ^ x) << 4));
-    uint4 q[3];
-    split8(lo, hi, q);
-#pragma unroll
-    for (int k = 0; k < 3; ++k)
-      *reinterpret_cast<uint4*>(planes + k * plane_bytes + b * 4096 + r * 128 + (((c + 4 * h) ^ x) << 4)) = q[k];
-  }
-}
-
 // ---- the kernel -----------------------------------------------------------------
-template <typename T, int CG, int RAW>
+template <typename T, int CG>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const GemmParams p) {
   constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
-  using S = GemmShape<PLANES, CG, RAW>;
+  using S = GemmShape<PLANES, CG>;
   constexpr int BK = S::kBK;
   extern __shared__ uint8_t smem_raw[];
   // the same offset in both blocks of a pair: the dynamic shared memory starts at the same address there
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* raw_tiles = smem + S::kStages * S::kStage;
-  float4* transpose = reinterpret_cast<float4*>(raw_tiles + S::kRawStages * S::kRawTile);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(raw_tiles + S::kRawStages * S::kRawTile + S::kTranspose);
+  float4* transpose = reinterpret_cast<float4*>(smem + S::kStages * S::kStage);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStage + S::kTranspose);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * S::kStages;
   const uint32_t acc_full0 = empty0 + 8 * S::kStages, acc_empty0 = acc_full0 + 8 * S::kAccs;
-  const uint32_t raw_full0 = acc_empty0 + 8 * S::kAccs, raw_empty0 = raw_full0 + 8 * S::kRawStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * (S::kStages + S::kAccs + S::kRawStages));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * (S::kStages + S::kAccs));
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   EpilogueParams* epilogue = reinterpret_cast<EpilogueParams*>(tmem_slot + 2);
 
@@ -307,12 +236,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int rank = CG == 1 ? 0 : (int)cluster_rank();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(full0 + 8 * i, RAW ? 1 + 2 * CG : 1);  // the copies' bytes, and each splitting warp
+      mbar_init(full0 + 8 * i, 1);
       mbar_init(empty0 + 8 * i, 1);
-    }
-    for (int i = 0; i < S::kRawStages; ++i) {
-      mbar_init(raw_full0 + 8 * i, 1);
-      mbar_init(raw_empty0 + 8 * i, 2);
     }
     for (int i = 0; i < S::kAccs; ++i) {
       mbar_init(acc_full0 + 8 * i, 1);
@@ -337,77 +262,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   if (warp == 0 && lane == 0) {
     // ---- copies ----
-    const uint32_t bytes = CG * PLANES * ((RAW == kRawA ? 0 : S::kPlaneA) +
-                                          (RAW == kRawB ? 0 : p.b_mn ? blocks_b * 64 * BK * 2 : rows_b * BK * 2));
-    // where a k block of this block's work lies
-    struct Place {
-      int64_t item;
-      int k, k1, m0, n0;
-    };
-    auto enter = [&](Place& q) {  // the first k block of q.item
-      const int64_t tile = q.item % tiles;
-      const int split = (int)(q.item / tiles);
-      q.m0 = (int)(tile / p.n_tiles) * (kTileM * CG) + rank * kTileM;
-      q.n0 = (int)(tile % p.n_tiles) * p.bn + rank * rows_b;
-      q.k = (int)((int64_t)p.k_blocks * split / p.splits);
-      q.k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
-    };
-    auto step = [&](Place& q) {
-      if (++q.k < q.k1) return;
-      q.item += workers;
-      if (q.item < items) enter(q);
-    };
-    uint32_t stage = 0, phase = 0, raw_stage = 0, raw_phase = 0;
+    const uint32_t bytes =
+        CG * PLANES * (S::kPlaneA + (p.b_mn ? blocks_b * 64 * BK * 2 : rows_b * BK * 2));
+    uint32_t stage = 0, phase = 0;
     bool ok = true;
-    Place at{worker}, ahead;  // fp32 tiles are asked for ahead of the planes
-    enter(at);
-    ahead = at;
-    auto load_raw = [&]() {
-      if (!(ok = mbar_wait(raw_empty0 + 8 * raw_stage, raw_phase ^ 1, gave_up))) return;
-      const uint32_t bar = raw_full0 + 8 * raw_stage, dst = smem_u32(raw_tiles + raw_stage * S::kRawTile);
-      if (RAW == kRawA) {
-        mbar_expect(bar, S::kRawTile);
-        tma_load<1>(dst, &map_a, ahead.k * BK, ahead.m0, 0, bar);
-      } else {
-        mbar_expect(bar, blocks_b * 8192);
-        for (int i = 0; i < 2 * blocks_b; ++i)
-          tma_load<1>(dst + i * 4096, &map_b, ahead.n0 + 32 * i, ahead.k * BK, 0, bar);
-      }
-      if (++raw_stage == S::kRawStages) raw_stage = 0, raw_phase ^= 1;
-      step(ahead);
-    };
-    if constexpr (RAW != kNoRaw) {
-      for (int i = 0; i < S::kRawStages - 1 && ahead.item < items && ok; ++i) load_raw();
-    }
-    while (at.item < items && ok) {
-      if constexpr (RAW != kNoRaw) {
-        if (ahead.item < items) load_raw();
-        if (!ok) break;
-      }
-      if (!(ok = mbar_wait(empty0 + 8 * stage, phase ^ 1, gave_up))) break;
-      const uint32_t bar = full0 + 8 * stage;
-      if (rank == 0) mbar_expect(bar, bytes);
-      const uint32_t sa = smem_u32(smem + stage * S::kStage), sb = sa + PLANES * S::kPlaneA;
-      for (int q = 0; q < PLANES; ++q) {
-        if constexpr (RAW != kRawA) {
+    for (int64_t item = worker; item < items && ok; item += workers) {
+      const int64_t tile = item % tiles;
+      const int split = (int)(item / tiles);
+      const int m0 = (int)(tile / p.n_tiles) * (kTileM * CG) + rank * kTileM;
+      const int n0 = (int)(tile % p.n_tiles) * p.bn + rank * rows_b;
+      const int k0 = (int)((int64_t)p.k_blocks * split / p.splits), k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
+      for (int k = k0; k < k1; ++k) {
+        if (!(ok = mbar_wait(empty0 + 8 * stage, phase ^ 1, gave_up))) break;
+        const uint32_t bar = full0 + 8 * stage;
+        if (rank == 0) mbar_expect(bar, bytes);
+        const uint32_t sa = smem_u32(smem + stage * S::kStage), sb = sa + PLANES * S::kPlaneA;
+        for (int q = 0; q < PLANES; ++q) {
           if (p.a_mn) {
             for (int i = 0; i < kTileM / 64; ++i)
-              tma_load<CG>(sa + q * S::kPlaneA + i * 64 * BK * 2, &map_a, at.m0 + 64 * i, at.k * BK, q, bar);
+              tma_load<CG>(sa + q * S::kPlaneA + i * 64 * BK * 2, &map_a, m0 + 64 * i, k * BK, q, bar);
           } else {
-            tma_load<CG>(sa + q * S::kPlaneA, &map_a, at.k * BK, at.m0, q, bar);
+            tma_load<CG>(sa + q * S::kPlaneA, &map_a, k * BK, m0, q, bar);
           }
-        }
-        if constexpr (RAW != kRawB) {
           if (p.b_mn) {
             for (int i = 0; i < blocks_b; ++i)
-              tma_load<CG>(sb + q * S::kPlaneB + i * 64 * BK * 2, &map_b, at.n0 + 64 * i, at.k * BK, q, bar);
+              tma_load<CG>(sb + q * S::kPlaneB + i * 64 * BK * 2, &map_b, n0 + 64 * i, k * BK, q, bar);
           } else {
-            tma_load<CG>(sb + q * S::kPlaneB, &map_b, at.k * BK, at.n0, q, bar);
+            tma_load<CG>(sb + q * S::kPlaneB, &map_b, k * BK, n0, q, bar);
           }
         }
+        if (++stage == S::kStages) stage = 0, phase ^= 1;
       }
-      if (++stage == S::kStages) stage = 0, phase ^= 1;
-      step(at);
     }
     // the last copies and products have to land before the block ends: wait for every stage to be free again
     for (int i = 0; i < S::kStages; ++i) {
@@ -415,34 +300,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       while (!mbar_try(empty0 + 8 * stage, phase ^ 1) && global_ns() - t0 < (ok ? kWaitLimitNs : kWaitLimitNs / 16)) {
       }
       if (++stage == S::kStages) stage = 0, phase ^= 1;
-    }
-  } else if (RAW != kNoRaw && (warp == 2 || warp == 3)) {
-    // ---- fp32 tiles into planes ----
-    uint32_t stage = 0, phase = 0, raw_stage = 0, raw_phase = 0;
-    bool ok = true;
-    for (int64_t item = worker; item < items && ok; item += workers) {
-      const int split = (int)(item / tiles);
-      const int k0 = (int)((int64_t)p.k_blocks * split / p.splits), k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
-      for (int k = k0; k < k1; ++k) {
-        ok = mbar_wait(raw_full0 + 8 * raw_stage, raw_phase, gave_up) &&
-             mbar_wait(empty0 + 8 * stage, phase ^ 1, gave_up);
-        if (!__all_sync(kFull, ok)) {
-          ok = false;
-          break;
-        }
-        const uint8_t* raw = raw_tiles + raw_stage * S::kRawTile;
-        uint8_t* planes = smem + stage * S::kStage;
-        if (RAW == kRawA) split_tile_a(raw, planes, S::kPlaneA, warp - 2, lane);
-        else split_tile_b(raw, planes + PLANES * S::kPlaneA, S::kPlaneB, blocks_b, warp - 2, lane);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the products read what was just written
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(raw_empty0 + 8 * raw_stage);
-          mbar_release_leader(full0 + 8 * stage);
-        }
-        if (++raw_stage == S::kRawStages) raw_stage = 0, raw_phase ^= 1;
-        if (++stage == S::kStages) stage = 0, phase ^= 1;
-      }
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
     // ---- products ----

@@ -9,13 +9,19 @@
 namespace nnue_ls {
 
 // The three bf16 planes of V fp32 values: each takes the leading 8 bits of
-// what is left, so their sum is the value.  An infinity leaves NaN in the
-// second plane, so its sums become NaN.
+// what is left, so their sum is the value.  An infinity or NaN stays in the
+// first plane.
 template <int V>
 __device__ __forceinline__ void split_planes(const float (&v)[V], uint16_t (&q)[3][V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float r = v[i];
+    const bool finite = (__float_as_uint(r) & 0x7f800000u) != 0x7f800000u;
+    if (!finite) {
+      q[0][i] = r != r ? 0x7fff : (uint16_t)(__float_as_uint(r) >> 16);
+      q[1][i] = q[2][i] = 0;
+      continue;
+    }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       const uint32_t top = __float_as_uint(r) & 0xffff0000u;

@@ -34,30 +34,24 @@ EncodeTiled encode_tiled() {
 }
 
 // An operand in the products' layout: [planes][outer][inner] 16-bit values,
-// inner contiguous; or fp32 as it lies (raw).  base and ld times the element
-// size are multiples of 16 bytes.
+// inner contiguous.  base and ld * 2 are multiples of 16 bytes.
 struct Operand {
   const void* base;
   int64_t inner, outer, ld;
   bool mn_major;  // inner runs along m or n rather than k
-  bool raw;
 };
 
 int make_map(CUtensorMap* map, const Operand& o, int planes, bool is_f16, int bk, int tile_rows) {
   EncodeTiled fn = encode_tiled();
   if (!fn) return fail(NNUE_LS_ERR_CUDA, "gemm: the driver has no cuTensorMapEncodeTiled");
-  const int element = o.raw ? 4 : 2;
-  const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.outer, (cuuint64_t)(o.raw ? 1 : planes)};
-  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * element, (cuuint64_t)o.ld * element * (cuuint64_t)o.outer};
-  // 128 bytes (32 fp32 or 64 16-bit values) of the inner direction, or one k block of it
-  const cuuint32_t box[3] = {(cuuint32_t)(o.mn_major ? 128 / element : bk), (cuuint32_t)(o.mn_major ? bk : tile_rows), 1};
+  const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.outer, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)o.ld * 2 * (cuuint64_t)o.outer};
+  const cuuint32_t box[3] = {(cuuint32_t)(o.mn_major ? 64 : bk), (cuuint32_t)(o.mn_major ? bk : tile_rows), 1};
   const cuuint32_t one[3] = {1, 1, 1};
-  const CUtensorMapDataType type = o.raw    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : is_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   auto encode = [&] {
-    return fn(map, type, 3, const_cast<void*>(o.base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              box[0] * element == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+    return fn(map, is_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+              const_cast<void*>(o.base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              o.mn_major || bk == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = encode();
@@ -127,15 +121,15 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, int planes) {
   return e.plan;
 }
 
-template <typename T, int CG, int RAW>
+template <typename T, int CG>
 int launch_gemm_cg(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, cudaStream_t s) {
-  using S = GemmShape<sizeof(T) == 4 ? 3 : 1, CG, RAW>;
+  using S = GemmShape<sizeof(T) == 4 ? 3 : 1, CG>;
   static std::atomic<uint64_t> ready{0};  // one bit per device: the kernel may use S::kSmem there
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("gemm");
   if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
     const cudaError_t e =
-        cudaFuncSetAttribute(gemm_kernel<T, CG, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        cudaFuncSetAttribute(gemm_kernel<T, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "gemm: %s", cudaGetErrorString(e));
     if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
   }
@@ -152,7 +146,7 @@ int launch_gemm_cg(const CUtensorMap& a, const CUtensorMap& b, const GemmParams&
   cfg.attrs = &cluster;
   cfg.numAttrs = CG == 1 ? 0 : 1;
   count_launch();
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, CG, RAW>, a, b, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<T, CG>, a, b, p);
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "gemm: %s", cudaGetErrorString(e));
 }
 
@@ -185,19 +179,7 @@ int launch_gemm(const Operand& a, const Operand& b, int64_t M, int64_t N, const 
   auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   e.vec = N % V == 0 && aligned(e.out) && aligned(e.act_grad) && aligned(e.residual) && (!e.residual || e.ldr % V == 0);
   p.e = e;
-  auto launch = [&](auto raw) {
-    constexpr int RAW = decltype(raw)::value;
-    return t.cg == 1 ? launch_gemm_cg<T, 1, RAW>(map_a, map_b, p, s) : launch_gemm_cg<T, 2, RAW>(map_a, map_b, p, s);
-  };
-  int rc = NNUE_LS_OK;
-  if constexpr (sizeof(T) == 4) {
-    if (a.raw) rc = launch(std::integral_constant<int, kRawA>{});
-    else if (b.raw) rc = launch(std::integral_constant<int, kRawB>{});
-    else rc = launch(std::integral_constant<int, kNoRaw>{});
-  } else {
-    rc = launch(std::integral_constant<int, kNoRaw>{});
-  }
-  if (rc) return rc;
+  if (int rc = t.cg == 1 ? launch_gemm_cg<T, 1>(map_a, map_b, p, s) : launch_gemm_cg<T, 2>(map_a, map_b, p, s)) return rc;
   if (t.splits > 1) {
     const int64_t total = e.vec ? M * N / 4 : M * N;
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total, 256), kNumSMs * 16);
@@ -209,22 +191,13 @@ int launch_gemm(const Operand& a, const Operand& b, int64_t M, int64_t N, const 
 }
 
 // ---- operands ----------------------------------------------------------------
-// fp32 weights are always brought into planes; other operands are packed only
-// when a row starts off a 16-byte boundary, where TMA cannot copy it.
+// fp32 values are always brought into planes; 16-bit ones only when a row
+// starts off a 16-byte boundary, where TMA cannot copy it.
 template <typename T>
 bool needs_pack(const void* p, int64_t ld, int64_t rows) {
   return sizeof(T) == 4 || reinterpret_cast<uintptr_t>(p) % 16 != 0 || (ld % 8 != 0 && rows > 1);
 }
 constexpr int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
-// Whether an fp32 x can be read as it lies, and split on the way.
-template <typename T>
-bool reads_raw(const void* p, int64_t ld, int64_t rows) {
-  return sizeof(T) == 4 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld % 4 == 0 || rows <= 1);
-}
-template <typename T>
-bool packs_x(const nnue_ls_linear& a) {
-  return needs_pack<T>(a.x, a.ldx, a.rows) && !reads_raw<T>(a.x, a.ldx, a.rows);
-}
 template <typename T>
 size_t pack_bytes(int64_t rows, int64_t cols) {
   return align256((size_t)rows * round8(cols) * (sizeof(T) == 4 ? 6 : 2));
@@ -238,14 +211,10 @@ struct Packer {
 
   // The matrix as an operand; packed into `buffer` where it cannot be read as it lies.
   Operand operand(const void* p, int64_t ld, int64_t rows, int64_t cols, bool mn_major, void* buffer) {
-    if (!needs_pack<T>(p, ld, rows)) return Operand{p, cols, rows, round8(ld), mn_major, false};
+    if (!needs_pack<T>(p, ld, rows)) return Operand{p, cols, rows, round8(ld), mn_major};
     const bool vec = reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (16 / (int64_t)sizeof(T)) == 0;
     jobs.job[count++] = PackJob{p, buffer, ld, rows, cols, round8(cols), vec};
-    return Operand{buffer, cols, rows, round8(cols), mn_major, false};
-  }
-  Operand operand_x(const nnue_ls_linear& a, bool mn_major, void* buffer) {
-    if (reads_raw<T>(a.x, a.ldx, a.rows)) return Operand{a.x, a.inputs, a.rows, (a.ldx + 3) / 4 * 4, mn_major, true};
-    return operand(a.x, a.ldx, a.rows, a.inputs, mn_major, buffer);
+    return Operand{buffer, cols, rows, round8(cols), mn_major};
   }
   void launch(cudaStream_t s) {
     if (count == 0) return;
@@ -292,7 +261,7 @@ ForwardPlan plan_forward(const nnue_ls_linear& a) {
   ForwardPlan p{};
   if (few_rows<T>(a)) return p;
   p.tiles = plan_tiles(a.rows, a.outputs, a.inputs, sizeof(T) == 4 ? 3 : 1);
-  p.x = !a.x_packed && packs_x<T>(a) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+  p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
   p.w = !a.weight_packed && needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
   p.partial = p.tiles.partial_bytes(a.rows, a.outputs);
   p.total = p.x + p.w + p.partial;
@@ -305,7 +274,7 @@ template <typename T>
 size_t linear_packed_bytes(const nnue_ls_linear& a, bool weight) {
   if (few_rows<T>(a)) return 0;
   if (weight) return needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
-  return packs_x<T>(a) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+  return needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
 }
 
 template <typename T>
@@ -324,7 +293,7 @@ int linear_forward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   }
   const ForwardPlan p = plan_forward<T>(a);
   Packer<T> pack;
-  const Operand x = pack.operand_x(a, false, a.x_packed ? a.x_packed : ws);
+  const Operand x = pack.operand(a.x, a.ldx, a.rows, a.inputs, false, a.x_packed ? a.x_packed : ws);
   const Operand w =
       pack.operand(a.weight, a.ldw, a.outputs, a.inputs, false, a.weight_packed ? a.weight_packed : ws + p.x);
   pack.launch(s);
@@ -354,7 +323,7 @@ BackwardPlan plan_backward(const nnue_ls_linear& a) {
   }
   if (a.grad_weight) {
     p.dw = plan_tiles(a.outputs, a.inputs, a.rows, planes);
-    p.x = !a.x_packed && packs_x<T>(a) ? pack_bytes<T>(a.rows, a.inputs) : 0;
+    p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
     p.partial = std::max(p.partial, p.dw.partial_bytes(a.outputs, a.inputs));
   }
   p.dz_written = products && (a.activation != NNUE_LS_ACT_NONE || needs_pack<T>(a.grad_out, a.ldg, a.rows));
@@ -386,7 +355,7 @@ int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   const BackwardPlan p = plan_backward<T>(a);
   using Code = typename Derivative<T>::Code;
   char *dz = ws, *x = dz + p.dz, *w = x + p.x, *bias = w + p.w, *partial = bias + p.bias;
-  Operand d{a.grad_out, a.outputs, a.rows, round8(a.ldg), false, false};
+  Operand d{a.grad_out, a.outputs, a.rows, round8(a.ldg), false};
   if (p.dz_written || p.bias) {
     const T* g = static_cast<const T*>(a.grad_out);
     const Code* ag = a.activation == NNUE_LS_ACT_NONE ? nullptr : static_cast<const Code*>(a.act_grad);
@@ -397,7 +366,7 @@ int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
     count_launch();
     if (p.v > 1) dz_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, s>>>(g, a.ldg, ag, out, ldo, sums, a.rows, a.outputs, p.rows_per_part, p.tx);
     else dz_kernel<T, 1><<<grid, 256, 0, s>>>(g, a.ldg, ag, out, ldo, sums, a.rows, a.outputs, p.rows_per_part, p.tx);
-    if (p.dz_written) d = Operand{dz, a.outputs, a.rows, ldo, false, false};
+    if (p.dz_written) d = Operand{dz, a.outputs, a.rows, ldo, false};
     if (sums) {
       count_launch();
       column_total_kernel<T><<<(unsigned)ceil_div(a.outputs, 32), dim3(32, 8), 0, s>>>(
@@ -414,11 +383,11 @@ int linear_backward(const nnue_ls_linear& a, char* ws, cudaStream_t s) {
   Packer<T> pack;
   Operand bw{}, bx{};
   if (a.grad_x)
-    bw = a.weight_packed ? Operand{a.weight_packed, a.inputs, a.outputs, round8(a.inputs), true, false}
+    bw = a.weight_packed ? Operand{a.weight_packed, a.inputs, a.outputs, round8(a.inputs), true}
                          : pack.operand(a.weight, a.ldw, a.outputs, a.inputs, true, w);
   if (a.grad_weight)
-    bx = a.x_packed ? Operand{a.x_packed, a.inputs, a.rows, round8(a.inputs), true, false}
-                    : pack.operand_x(a, true, x);
+    bx = a.x_packed ? Operand{a.x_packed, a.inputs, a.rows, round8(a.inputs), true}
+                    : pack.operand(a.x, a.ldx, a.rows, a.inputs, true, x);
   pack.launch(s);
   EpilogueParams e{};
   if (a.grad_x) {  // dx = dz W: k runs over the outputs

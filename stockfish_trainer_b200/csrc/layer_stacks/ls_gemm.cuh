@@ -72,7 +72,7 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t bar) {
   asm volatile(
       "{\n .reg .b32 ra;\n mapa.shared::cluster.u32 ra, %0, 0;\n"
-      " mbarrier.arrive.shared::cluster.b64 _, [ra];\n}" ::"r"(bar)
+      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n}" ::"r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -81,7 +81,8 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
       : "r"(bar), "r"(parity)
       : "memory");

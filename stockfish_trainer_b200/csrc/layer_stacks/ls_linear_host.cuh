@@ -68,36 +68,41 @@ struct TilePlan {
   size_t partial_bytes(int64_t M, int64_t N) const { return splits > 1 ? align256((size_t)splits * M * N * 4) : 0; }
 };
 
-// Estimates the clocks of each way to cut C = A B^T and takes the least: a k
-// block costs its products (bn / 2 clocks per 16 k and plane product) or its
-// bytes from L2 (about 48 per clock and SM), whichever is more; an item adds
-// the fill and drain of the pipeline; pieces add their joining pass (at 3500
-// bytes per clock) and its launch.
+// Estimates the clocks of each way to cut C = A B^T and takes the least.  The
+// figures are fits to measured times of single products on B200: a k block
+// (64 values, fp32 32) costs a part for A's tile and its copies and a part per
+// column, an item its epilogue and drain, a pair of blocks its later start,
+// pieces their joining pass (a launch, and their bytes at 3500 per clock).
+// Against the fits' own predecessor, which counted products and L2 bytes only:
+// fp32 65536 x 1040 x 256 forward 201 instead of 253 us, 24 x 1040 x 1040 bf16
+// 11.4 instead of 14.5 us.
 TilePlan find_tiles(int64_t M, int64_t N, int64_t K, int planes) {
-  const int bk = planes == 1 ? 64 : 32, products = planes == 1 ? 1 : 6;
+  const int64_t k_blocks = ceil_div(K, planes == 1 ? 64 : 32);
   TilePlan best{};
   double best_cost = 0;
-  const int64_t k_blocks = ceil_div(K, bk);
   for (int cg = 1; cg <= 2; ++cg) {
     const int max_bn = planes == 3 && cg == 1 ? 128 : 256;
+    const double block0 = planes == 1 ? (cg == 1 ? 330 : 370) : (cg == 1 ? 970 : 1600);
+    const double block1 = planes == 1 ? (cg == 1 ? 1.92 : 1.3) : (cg == 1 ? 3.7 : 2.0);
     const int64_t m_tiles = ceil_div(M, kTileM * cg), least = ceil_div(N, max_bn);
     const int workers = kNumSMs / cg;
     int last_bn = 0;
-    for (int64_t nt = least; nt < least + 6; ++nt) {
+    for (int i = 0; i < 8; ++i) {
+      // the fewest column tiles and a few more; as many as occupy the SMs, and half of that
+      const int64_t nt = i < 6 ? least + i : std::max(least, workers / m_tiles / (i - 5));
       const int bn = (int)(ceil_div(ceil_div(N, nt), 16) * 16);
       if (bn == last_bn) continue;
       last_bn = bn;
       const int64_t n_tiles = ceil_div(N, bn), tiles = m_tiles * n_tiles;
-      const double mma = products * (bk / 16) * (bn / 2.0);
-      const double l2 = planes * (kTileM + bn / cg) * (bk * 2.0) / 48;
-      const double block = std::max(mma, l2);
-      for (int fill = 0; fill <= 4; ++fill) {
+      const double block = block0 + block1 * std::max(bn, 48);
+      const double item = planes == 1 ? 1000 + 14.0 * bn : 2000 + 10.0 * bn;
+      for (int fill = 0; fill <= 4; ++fill) {  // pieces that fill this many rounds of the SMs
         int64_t splits = fill == 0 ? 1 : workers * fill / tiles;
         splits = std::min<int64_t>(std::min<int64_t>(splits, k_blocks), 256);
         if (splits < 1 || (fill && splits < 2)) continue;
         const double rounds = (double)ceil_div(tiles * splits, workers), per = (double)ceil_div(k_blocks, splits);
-        double cost = 4000 + rounds * (per * block + 600) + bn * 8;
-        if (splits > 1) cost += 5000 + splits * (double)M * N * 8 / 3500;
+        double cost = (cg == 2 ? 3600 : 0) + rounds * (per * block + item) + 5.0 * std::min<int64_t>(tiles, workers);
+        if (splits > 1) cost += 8000 + splits * (double)M * N * 8 / 3500;
         if (best.cg == 0 || cost < best_cost) {
           best_cost = cost;
           best = TilePlan{cg, bn, (int)splits, (int)k_blocks, m_tiles, n_tiles};

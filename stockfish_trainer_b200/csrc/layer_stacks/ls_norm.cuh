@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
 }
 
 // ---- rows held in registers -----------------------------------------------------
-// The kernels above read a row once per pass, for any width.  Up to 2048 columns
+// The kernels above read a row once per pass, for any width.  Up to 4096 columns
 // the ones below read it once: a block works on R rows at a time and a thread
 // keeps NV * V = 4 columns of them in registers (V = 4 neighbouring ones, or 4
 // single ones where rows are not aligned).  A thread's columns are the same in

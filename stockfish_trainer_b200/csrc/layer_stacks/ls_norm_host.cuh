@@ -56,43 +56,50 @@ bool norm_vectors(const nnue_ls_norm& a) {
   return a.width % (int)(16 / sizeof(T)) == 0;
 }
 
-// Which kernel a call takes.  Up to 2048 columns, four per thread: rows of up to
-// 1152 columns get 288 threads a block, whose registers hold more rows at once.
-// Wider rows are read once per pass.
+// Which kernel a call takes.  Up to 4096 columns, four per thread; the fewer
+// threads a row takes, the more registers each has, for more rows at once.
+// Wider rows are read once per pass (65536 x 1040 fp32 forward and backward:
+// 0.57 ms by rows, 2.1 ms by passes).
+enum RowClass : int { kNarrow = 0, kMiddle = 1, kWide = 2, kAnyWidth = 3 };
 struct RowPlan {
   bool vec;
-  int threads;  // 0: the kernel for any width
-  bool narrow() const { return vec && threads <= 288; }
+  int threads, cls;
 };
 
 template <typename T>
 RowPlan plan_norm(const nnue_ls_norm& a) {
-  RowPlan r{norm_vectors<T>(a), 0};
   const int64_t threads = ceil_div(a.width, 128) * 32;
-  if (threads <= 512) r.threads = (int)threads;
-  return r;
+  const bool vec = norm_vectors<T>(a);
+  const int cls = threads <= 288 && vec ? kNarrow : threads <= 512 ? kMiddle : threads <= 1024 ? kWide : kAnyWidth;
+  return RowPlan{vec, (int)std::min<int64_t>(threads, 1024), cls};
 }
 
 // Rows at a time, rounds in flight, and blocks per SM, so that registers and
 // 227 KB of shared memory hold them.
-template <typename T, bool NARROW, bool FULL, bool BACKWARD>
+template <typename T, int CLASS, bool FULL, bool BACKWARD>
 struct RowShape {
-  static constexpr int kThreads = NARROW ? 288 : 512;
-  static constexpr int kRows = BACKWARD ? (NARROW && sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 2 || !FULL ? 4 : 2;
+  static constexpr int kThreads = CLASS == kNarrow ? 288 : CLASS == kMiddle ? 512 : 1024;
+  static constexpr int kRows = BACKWARD ? (CLASS == kNarrow && sizeof(T) == 2 ? 4 : CLASS == kWide ? 1 : 2)
+                               : CLASS == kWide || (sizeof(T) == 4 && FULL) ? 2
+                                                                           : 4;
   static constexpr int kSlot = (int)sizeof(T) * 4 * kRows * (2 + FULL + 2 * BACKWARD);  // bytes per thread and round
-  static constexpr int kBlocks = NARROW ? 2 : 1;
+  static constexpr int kBlocks = CLASS == kNarrow ? 2 : 1;
   static constexpr int kFit = 220 * 1024 / kBlocks / (kSlot * kThreads);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;
   static_assert(kStages >= 2, "a round on its way while one is worked on");
 };
 
-int norm_blocks_per_sm(const RowPlan& r) { return std::min(16, std::max(1, (r.narrow() ? 576 : 512) / r.threads)); }
+int norm_blocks_per_sm(const RowPlan& r) {
+  return std::min(16, std::max(1, (r.cls == kNarrow ? 576 : r.cls == kMiddle ? 512 : 1024) / r.threads));
+}
 
 template <typename T>
 int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
   const int64_t rows = std::max<int64_t>(a.rows, 1);
-  if (!r.threads) return std::min<int64_t>(rows, kNumSMs * 4);
-  const int at_once = r.narrow() ? RowShape<T, true, false, true>::kRows : RowShape<T, false, false, true>::kRows;
+  if (r.cls == kAnyWidth) return std::min<int64_t>(rows, kNumSMs * 4);
+  const int at_once = r.cls == kNarrow   ? RowShape<T, kNarrow, false, true>::kRows
+                      : r.cls == kMiddle ? RowShape<T, kMiddle, false, true>::kRows
+                                         : RowShape<T, kWide, false, true>::kRows;
   return std::min<int64_t>(ceil_div(rows, at_once), (int64_t)kNumSMs * norm_blocks_per_sm(r));
 }
 
@@ -125,7 +132,7 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
   const RowPlan r = plan_norm<T>(a);
   const bool center = a.kind == NNUE_LS_NORM_LAYER;
   count_launch();
-  if (!r.threads) {
+  if (r.cls == kAnyWidth) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, kNumSMs * 8);
     if (center) norm_forward_kernel<T, true><<<grid, 256, 0, s>>>(p);
     else norm_forward_kernel<T, false><<<grid, 256, 0, s>>>(p);
@@ -138,15 +145,20 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
   const bool both = a.f && a.post_weight && a.h;
   const int rc = with_flags(center, a.gate_mode == kGateFull, both, [&](auto c, auto f, auto b2) {
     constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b2)::value;
-    using N = RowShape<T, true, F, false>;
-    using W = RowShape<T, false, F, false>;
-    if (r.narrow())
-      return launch_norm_rows(norm_forward_rows_kernel<T, 4, N::kRows, C, F, B, N::kStages, 288, 2>,
-                              blocks(N::kRows), r, N::kSlot * N::kStages, p, s);
-    if (r.vec)
-      return launch_norm_rows(norm_forward_rows_kernel<T, 4, W::kRows, C, F, B, W::kStages, 512, 1>,
-                              blocks(W::kRows), r, W::kSlot * W::kStages, p, s);
-    return launch_norm_rows(norm_forward_rows_kernel<T, 1, 4, C, F, B, 0, 512, 1>, blocks(4), r, 0, p, s);
+    auto go = [&](auto cls) {
+      constexpr int K = decltype(cls)::value;
+      using H = RowShape<T, K, F, false>;
+      if (r.vec)
+        return launch_norm_rows(norm_forward_rows_kernel<T, 4, H::kRows, C, F, B, H::kStages, H::kThreads, H::kBlocks>,
+                                blocks(H::kRows), r, H::kSlot * H::kStages, p, s);
+      if constexpr (K == kNarrow) return NNUE_LS_OK;  // a row off 16 bytes is never of this class
+      else
+        return launch_norm_rows(norm_forward_rows_kernel<T, 1, H::kRows, C, F, B, 0, H::kThreads, 1>, blocks(H::kRows),
+                                r, 0, p, s);
+    };
+    if (r.cls == kNarrow) return go(std::integral_constant<int, kNarrow>{});
+    if (r.cls == kMiddle) return go(std::integral_constant<int, kMiddle>{});
+    return go(std::integral_constant<int, kWide>{});
   });
   if (rc) return rc;
   return check_launch("norm_forward");
@@ -165,22 +177,28 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
   const RowPlan r = plan_norm<T>(a);
   const unsigned grid = (unsigned)norm_backward_blocks<T>(a, r);
   count_launch();
-  if (!r.threads) {
+  if (r.cls == kAnyWidth) {
     if (center) norm_backward_kernel<T, true><<<grid, 256, 0, s>>>(p);
     else norm_backward_kernel<T, false><<<grid, 256, 0, s>>>(p);
   } else {
     const bool both = a.f && a.post_weight && a.pre_weight && a.grad_h;
     const int rc = with_flags(center, a.gate_mode == kGateFull, both, [&](auto c, auto f, auto b2) {
       constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b2)::value;
-      using N = RowShape<T, true, F, true>;
-      using W = RowShape<T, false, F, true>;
-      if (r.narrow())
-        return launch_norm_rows(norm_backward_rows_kernel<T, 4, N::kRows, C, F, B, N::kStages, 288, 2>, grid, r,
-                                N::kSlot * N::kStages, p, s);
-      if (r.vec)
-        return launch_norm_rows(norm_backward_rows_kernel<T, 4, W::kRows, C, F, B, W::kStages, 512, 1>, grid, r,
-                                W::kSlot * W::kStages, p, s);
-      return launch_norm_rows(norm_backward_rows_kernel<T, 1, 2, C, F, B, 0, 512, 1>, grid, r, 0, p, s);
+      auto go = [&](auto cls) {
+        constexpr int K = decltype(cls)::value;
+        using H = RowShape<T, K, F, true>;
+        if (r.vec)
+          return launch_norm_rows(
+              norm_backward_rows_kernel<T, 4, H::kRows, C, F, B, H::kStages, H::kThreads, H::kBlocks>, grid, r,
+              H::kSlot * H::kStages, p, s);
+        if constexpr (K == kNarrow) return NNUE_LS_OK;
+        else
+          return launch_norm_rows(norm_backward_rows_kernel<T, 1, H::kRows, C, F, B, 0, H::kThreads, 1>, grid, r, 0, p,
+                                  s);
+      };
+      if (r.cls == kNarrow) return go(std::integral_constant<int, kNarrow>{});
+      if (r.cls == kMiddle) return go(std::integral_constant<int, kMiddle>{});
+      return go(std::integral_constant<int, kWide>{});
     });
     if (rc) return rc;
   }

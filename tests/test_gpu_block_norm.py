@@ -139,7 +139,8 @@ def test_sizes(cuda, rows, width, kind, dt):
 
 @pytest.mark.parametrize("dt", TYPES, ids=str)
 @pytest.mark.parametrize("gate", ["none", "row", "full"])
-@pytest.mark.parametrize("rows,width", [(900, 1152), (700, 1156), (333, 1536), (5, 2048), (1000, 1160), (40, 2044)])
+@pytest.mark.parametrize("rows,width", [(900, 1152), (700, 1156), (333, 1536), (5, 2048), (1000, 1160), (40, 2044),
+                                        (400, 2052), (301, 4096), (333, 4095), (7, 4100)])
 def test_widths_around_the_kernels_limits(cuda, rows, width, gate, dt):
     for kind in ("rms", "layer"):
         t, gy, gh = _make(rows, width, dt, rows + width, gate=gate)

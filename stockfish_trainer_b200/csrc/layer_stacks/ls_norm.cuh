@@ -225,10 +225,10 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
 // ---- rows held in registers -----------------------------------------------------
 // The kernels above read a row once per pass, for any width.  Up to 4096 columns
 // the ones below read it once: a block works on R rows at a time and a thread
-// keeps NV * V = 4 columns of them in registers (V = 4 neighbouring ones, or 4
-// single ones where rows are not aligned).  A thread's columns are the same in
-// every row, so the parameters are read once and the sums over rows are plain
-// registers until the block's last row; R rows share each barrier.
+// owns eight columns of them (as 16-byte pieces, or single ones where rows are
+// not aligned).  A thread's columns are the same in every row, so the
+// parameters are read once and the sums over rows are plain registers until
+// the block's last row; R rows share each barrier.
 
 // V values of a row at column c.
 template <typename T, int V>
@@ -317,35 +317,25 @@ struct BlockSum {
 
 __host__ __device__ constexpr int pow2_at_least(int n) { return n <= 1 ? 1 : 2 * pow2_at_least((n + 1) / 2); }
 
-// This thread's columns of the rows under work.
+// A thread's columns: kColumns of them, V neighbouring ones at a time.
+constexpr int kColumns = 8;
 template <typename T, int V>
 struct Columns {
-  static constexpr int kNV = 4 / V;
+  static constexpr int kNV = kColumns / V;
   __device__ __forceinline__ static int at(int i) { return ((int)threadIdx.x + i * (int)blockDim.x) * V; }
-  RowVec<T, V> raw[kNV];
-  __device__ __forceinline__ void load(const void* base, int64_t row, int width) {
-#pragma unroll
-    for (int i = 0; i < kNV; ++i)
-      if (at(i) < width) raw[i].load(base, row * width + at(i));
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < kNV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) raw[i].raw.v[j] = from_f<T>(0.f);
-  }
-  __device__ __forceinline__ float operator[](int k) const { return to_f(raw[k / V].raw.v[k % V]); }
-  __device__ __forceinline__ static void store(void* base, int64_t row, int width, const float (&v)[4]) {
+  __device__ __forceinline__ static void store(void* base, int64_t row, int width, const float (&v)[kColumns]) {
+    T* dst = static_cast<T*>(base) + row * width;
 #pragma unroll
     for (int i = 0; i < kNV; ++i)
       if (at(i) < width) {
         float t[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) t[j] = v[i * V + j];
-        store_row<T, V>(base, row * width + at(i), t);
+        store_row<T, V>(dst, at(i), t);
       }
   }
-  __device__ __forceinline__ static void params(const void* p, int width, bool f32, float absent, float (&v)[4]) {
+  __device__ __forceinline__ static void params(const void* p, int width, bool f32, float absent,
+                                                float (&v)[kColumns]) {
 #pragma unroll
     for (int i = 0; i < kNV; ++i) {
       float t[V];
@@ -359,51 +349,53 @@ struct Columns {
 };
 
 // The rows to come, on their way from HBM to shared memory while earlier ones
-// are worked on: STAGES rounds of R rows, a thread's own columns in a slot of
+// are worked on: STAGES rounds of R rows, a thread's own columns in slots of
 // its own, so that nobody waits for anybody and every pass over a row reads its
-// slot again instead of holding the row in registers.  Arrays: x, f, grad_y,
-// grad_h, gate.  STAGES == 0 (V == 1: a 2-byte value cannot be copied
+// slots again instead of holding the row in registers.  Arrays: x, f, gate,
+// grad_y, grad_h.  STAGES == 0 (V == 1: a 2-byte value cannot be copied
 // asynchronously): the rows are loaded when they are needed, into registers.
 enum RowArray : int { kX = 0, kF = 1, kGate = 2, kGradY = 3, kGradH = 4 };
 
 template <typename T, int V, int R, bool FULL, bool BACKWARD, int STAGES>
 struct RowRing {
   using C = Columns<T, V>;
-  using Raw = typename RowVec<T, 4>::Raw;
-  static constexpr int kArrays = 2 + FULL + 2 * BACKWARD;
+  using Raw = typename RowVec<T, V>::Raw;
+  static constexpr int kArrays = 2 + FULL + 2 * BACKWARD, kNV = C::kNV;
   __host__ __device__ static constexpr int index(int a) { return a <= kGate ? a : a - !FULL; }
   Raw* slots;
-  const void* base[5];
+  const T* base[5];
   int width, rows, stage = 0;
-  C held[STAGES ? 1 : R][STAGES ? 1 : kArrays];
+  RowVec<T, V> held[STAGES ? 1 : R][STAGES ? 1 : kArrays][STAGES ? 1 : kNV];
 
   __device__ __forceinline__ RowRing(const NormParams& p, void* smem) {
     slots = static_cast<Raw*>(smem) + threadIdx.x;
-    base[kX] = p.x;
-    base[kF] = p.f;
-    base[kGate] = FULL ? p.gate : nullptr;
-    base[kGradY] = BACKWARD ? p.grad_y : nullptr;
-    base[kGradH] = BACKWARD ? p.grad_h : nullptr;
+    base[kX] = static_cast<const T*>(p.x);
+    base[kF] = static_cast<const T*>(p.f);
+    base[kGate] = static_cast<const T*>(FULL ? p.gate : nullptr);
+    base[kGradY] = static_cast<const T*>(BACKWARD ? p.grad_y : nullptr);
+    base[kGradH] = static_cast<const T*>(BACKWARD ? p.grad_h : nullptr);
     width = p.width;
     rows = (int)p.rows;
   }
-  __device__ __forceinline__ Raw* slot(int st, int r, int i) const {
-    return slots + ((st * R + r) * kArrays + i) * (int)blockDim.x;
+  __device__ __forceinline__ Raw* slot(int st, int r, int i, int v) const {
+    return slots + (((st * R + r) * kArrays + i) * kNV + v) * (int)blockDim.x;
   }
   __device__ __forceinline__ void issue(int row0, int st) const {
-    const int c = (int)threadIdx.x * 4;
-    if (c < width && row0 < rows) {
+    if (row0 < rows) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int64_t at = (int64_t)min(row0 + r, rows - 1) * width + c;  // beyond the last row: read, not used
+        const int64_t row = (int64_t)min(row0 + r, rows - 1) * width;  // beyond the last row: read, not used
 #pragma unroll
-        for (int a = 0; a < 5; ++a) {
-          if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
-          if (a != kX && !base[a]) continue;
-          const T* src = static_cast<const T*>(base[a]) + at;
-          const unsigned d = (unsigned)__cvta_generic_to_shared(slot(st, r, index(a)));
-          if constexpr (sizeof(Raw) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-          else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+        for (int v = 0; v < kNV; ++v) {
+          const int c = C::at(v);
+          if (c >= width) continue;
+#pragma unroll
+          for (int a = 0; a < 5; ++a) {
+            if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
+            if (a != kX && !base[a]) continue;
+            const unsigned d = (unsigned)__cvta_generic_to_shared(slot(st, r, index(a), v));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(base[a] + row + c) : "memory");
+          }
         }
       }
     }
@@ -428,42 +420,49 @@ struct RowRing {
 #pragma unroll
         for (int a = 0; a < 5; ++a) {
           if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
-          held[r][index(a)].zero();
-          if (base[a]) held[r][index(a)].load(base[a], min(row0 + r, rows - 1), width);
+#pragma unroll
+          for (int v = 0; v < kNV; ++v) {
+            held[r][index(a)][v].raw = Raw{};
+            if (base[a] && C::at(v) < width)
+              held[r][index(a)][v].load(base[a], (int64_t)min(row0 + r, rows - 1) * width + C::at(v));
+          }
         }
     }
   }
   __device__ __forceinline__ void done() {
     if (STAGES > 0 && ++stage == STAGES) stage = 0;
   }
-  // The thread's four values of array A in row r of the round; zero where there are none.
+  // The thread's values of array A in row r of the round; zero where there are none.
   template <int A>
-  __device__ __forceinline__ void get(int r, float (&v)[4]) const {
-    if constexpr (STAGES > 0) {
-      typename RowVec<T, 4>::Raw raw;
-      if ((A == kX || base[A]) && (int)threadIdx.x * 4 < width) raw = *slot(stage, r, index(A));
-      else raw = typename RowVec<T, 4>::Raw{};
+  __device__ __forceinline__ void get(int r, float (&out)[kColumns]) const {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = to_f(raw.v[k]);
-    } else {
+    for (int v = 0; v < kNV; ++v) {
+      RowVec<T, V> raw;
+      if constexpr (STAGES > 0) {
+        raw.raw = Raw{};
+        if ((A == kX || base[A]) && C::at(v) < width) raw.raw = *slot(stage, r, index(A), v);
+      } else {
+        raw = held[r][index(A)][v];
+      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = held[r][index(A)][k];
+      for (int j = 0; j < V; ++j) out[v * V + j] = raw[j];
     }
   }
 };
 
-// The gate of a row's four columns.
+// The gate of a row's columns.
 template <bool FULL, typename Ring>
-__device__ __forceinline__ void gates(const NormParams& p, const Ring& ring, int r, float row_gate, float (&g)[4]) {
+__device__ __forceinline__ void gates(const NormParams& p, const Ring& ring, int r, float row_gate,
+                                      float (&g)[kColumns]) {
   if constexpr (FULL) {
     ring.template get<kGate>(r, g);
     if (p.gate_sigmoid) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) g[k] = sigmoid(g[k]);
+      for (int k = 0; k < kColumns; ++k) g[k] = sigmoid(g[k]);
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) g[k] = row_gate;
+    for (int k = 0; k < kColumns; ++k) g[k] = row_gate;
   }
 }
 template <typename T>
@@ -473,31 +472,39 @@ __device__ __forceinline__ float load_row_gate(const NormParams& p, int row) {
   return p.gate_sigmoid ? sigmoid(g) : g;
 }
 
-// BOTH: the call has f with its norm and the norm after it; else what is there
-// is looked up.
-template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, int STAGES, int THREADS, int BLOCKS>
-__global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(const NormParams p) {
+// The forward's calls without biases or a learned scale fit 64 registers, so
+// that an SM holds 1024 threads instead of 512.
+__host__ __device__ constexpr int norm_forward_share(int v, bool both, bool more) {
+  return v > 1 && both && !more ? 2 : 1;
+}
+
+// BOTH: the call has f with its norm and the norm after it.  MORE: it may have
+// biases or a learned scale.  Without BOTH what is there is looked up.
+// At 128 registers a thread and 512 threads an SM; what bounds the kernels on
+// 16-bit rows is instruction issue, so a thread takes eight columns: what a row
+// costs besides its columns (addresses, copies, the exchange of sums) is shared
+// by eight instead of four.
+template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, bool MORE, int STAGES>
+__global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_forward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
+  constexpr int N = kColumns;
   extern __shared__ float4 norm_ring[];
   __shared__ float scratch[2 * 32 * R];
   BlockSum<R> total{scratch};
   const bool has_f = BOTH || p.f, post = BOTH || p.post_weight, pre = BOTH || p.h;
   const int W = p.width, rows = (int)p.rows, stride = (int)gridDim.x * R;
   const float inv = 1.f / W;
-  bool mine[4];  // columns inside the row
-#pragma unroll
-  for (int k = 0; k < 4; ++k) mine[k] = C::at(k / V) < W;
-  float w[4], b[4], sc[4], pw[4], pb[4];
+  float w[N], b[N], sc[N], pw[N], pb[N];
   C::params(p.post_weight, W, p.params_f32, 1.f, w);
-  C::params(p.post_bias, W, p.params_f32, 0.f, b);
-  C::params(p.scale, W, p.params_f32, p.scale_value, sc);
+  C::params(MORE ? p.post_bias : nullptr, W, p.params_f32, 0.f, b);
+  C::params(MORE ? p.scale : nullptr, W, p.params_f32, p.scale_value, sc);
   C::params(p.pre_weight, W, p.params_f32, 1.f, pw);
-  C::params(p.pre_bias, W, p.params_f32, 0.f, pb);
+  C::params(MORE ? p.pre_bias : nullptr, W, p.params_f32, 0.f, pb);
   RowRing<T, V, R, FULL, false, STAGES> ring(p, norm_ring);
   ring.start((int)blockIdx.x * R, stride);
   for (int row0 = (int)blockIdx.x * R; row0 < rows; row0 += stride) {
     ring.next(row0, stride);
-    float gate[R], mean_f[R], rstd_f[R], mean_y[R], rstd_y[R], s[R], y[R][4], v[4];
+    float gate[R], mean_f[R], rstd_f[R], mean_y[R], rstd_y[R], s[R], y[R][N], v[N];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       gate[r] = FULL ? 1.f : load_row_gate<T>(p, min(row0 + r, rows - 1));
@@ -509,7 +516,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           ring.template get<kF>(r, v);
-          s[r] = (v[0] + v[1]) + (v[2] + v[3]);
+          s[r] = 0.f;
+#pragma unroll
+          for (int k = 0; k < N; ++k) s[r] += v[k];
         }
         total(s);
 #pragma unroll
@@ -520,8 +529,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
         ring.template get<kF>(r, v);
         s[r] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float d = CENTER ? (mine[k] ? v[k] - mean_f[r] : 0.f) : v[k];
+        for (int k = 0; k < N; ++k) {
+          const float d = CENTER ? (C::at(k / V) < W ? v[k] - mean_f[r] : 0.f) : v[k];
           s[r] = fmaf(d, d, s[r]);
         }
       }
@@ -533,12 +542,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
     for (int r = 0; r < R; ++r) {
       ring.template get<kX>(r, y[r]);
       if (has_f) {
-        float g[4];
+        float g[N];
         gates<FULL>(p, ring, r, gate[r], g);
         ring.template get<kF>(r, v);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          y[r][k] = sc[k] * y[r][k] + g[k] * fmaf((v[k] - mean_f[r]) * rstd_f[r], w[k], b[k]);
+        for (int k = 0; k < N; ++k)
+          y[r][k] = fmaf(g[k], fmaf((v[k] - mean_f[r]) * rstd_f[r], w[k], b[k]), sc[k] * y[r][k]);
         if (row0 + r < rows) C::store(p.y, row0 + r, W, y[r]);
       }
     }
@@ -548,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
         for (int r = 0; r < R; ++r) {
           s[r] = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[r] += mine[k] ? y[r][k] : 0.f;
+          for (int k = 0; k < N; ++k) s[r] += C::at(k / V) < W ? y[r][k] : 0.f;
         }
         total(s);
 #pragma unroll
@@ -558,8 +567,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
       for (int r = 0; r < R; ++r) {
         s[r] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float d = mine[k] ? y[r][k] - mean_y[r] : 0.f;
+        for (int k = 0; k < N; ++k) {
+          const float d = C::at(k / V) < W ? y[r][k] - mean_y[r] : 0.f;
           s[r] = fmaf(d, d, s[r]);
         }
       }
@@ -568,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
       for (int r = 0; r < R; ++r) {
         rstd_y[r] = inv_sqrt(s[r] * inv + p.eps);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[r][k] = fmaf((y[r][k] - mean_y[r]) * rstd_y[r], pw[k], pb[k]);
+        for (int k = 0; k < N; ++k) y[r][k] = fmaf((y[r][k] - mean_y[r]) * rstd_y[r], pw[k], pb[k]);
         if (row0 + r < rows) C::store(p.h, row0 + r, W, y[r]);
       }
     }
@@ -581,10 +590,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_forward_rows_kernel(cons
   }
 }
 
-template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, int STAGES, int THREADS, int BLOCKS>
-__global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(const NormParams p) {
+template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, bool MORE, int STAGES>
+__global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
-  constexpr int N1 = CENTER ? 2 : 1, N2 = CENTER ? 3 : 2, K1 = R * N1, K2 = pow2_at_least(R * N2);
+  constexpr int N = kColumns, N1 = CENTER ? 2 : 1, N2 = CENTER ? 3 : 2, K1 = R * N1, K2 = pow2_at_least(R * N2);
   extern __shared__ float4 norm_ring[];
   __shared__ float scratch[2 * 32 * (K1 + K2)];
   BlockSum<K1> total1{scratch};
@@ -592,10 +601,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(con
   const bool has_f = BOTH || p.f, post = BOTH || p.post_weight, pre = BOTH || (p.grad_h && p.pre_weight);
   const int W = p.width, rows = (int)p.rows, stride = (int)gridDim.x * R;
   const float inv = 1.f / W;
-  float w[4], b[4], sc[4], pw[4], acc[5][4] = {};
+  float w[N], b[N], sc[N], pw[N];
+  float sum_post[N] = {}, sum_post_bias[N] = {}, sum_scale[N] = {}, sum_pre[N] = {}, sum_pre_bias[N] = {};
   C::params(p.post_weight, W, p.params_f32, 1.f, w);
-  C::params(p.post_bias, W, p.params_f32, 0.f, b);
-  C::params(p.scale, W, p.params_f32, p.scale_value, sc);
+  C::params(MORE ? p.post_bias : nullptr, W, p.params_f32, 0.f, b);
+  C::params(MORE ? p.scale : nullptr, W, p.params_f32, p.scale_value, sc);
   C::params(p.pre_weight, W, p.params_f32, 0.f, pw);
   RowRing<T, V, R, FULL, true, STAGES> ring(p, norm_ring);
   ring.start((int)blockIdx.x * R, stride);
@@ -614,29 +624,25 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(con
   for (int row0 = (int)blockIdx.x * R; row0 < rows; row0 += stride) {
     ring.next(row0, stride);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      st[r] = st_next[r];
-      gate[r] = gate_next[r];
-    }
+    for (int r = 0; r < R; ++r) st[r] = st_next[r], gate[r] = gate_next[r];
     ahead(min(row0 + stride, rows - 1));
-    float d[R][4], s[K1], q[K2];  // d: y - mean, then the gradient of y
+    float d[R][N], s[K1], q[K2];  // d: y - mean, then the gradient of y
     if (pre) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const bool live = row0 + r < rows;
-        float gh[4], v[4], g[4];
+        float gh[N], v[N], g[N];
         ring.template get<kX>(r, d[r]);
         ring.template get<kGradH>(r, gh);
         if (has_f) {
           ring.template get<kF>(r, v);
           gates<FULL>(p, ring, r, gate[r], g);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            d[r][k] = sc[k] * d[r][k] + g[k] * fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]);
+          for (int k = 0; k < N; ++k)
+            d[r][k] = fmaf(g[k], fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]), sc[k] * d[r][k]);
         }
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < N; ++k) {
           d[r][k] -= st[r].z;
           const float u = gh[k] * pw[k];
           s0 = fmaf(u, d[r][k], s0);
@@ -644,11 +650,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(con
         }
         s[r * N1] = s0;
         if (CENTER) s[r * N1 + 1] = s1;
-        if (live) {
+        if (row0 + r < rows) {  // a row beyond the last one adds nothing
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            acc[3][k] = fmaf(gh[k], d[r][k] * st[r].w, acc[3][k]);
-            acc[4][k] += gh[k];
+          for (int k = 0; k < N; ++k) {
+            sum_pre[k] = fmaf(gh[k], d[r][k] * st[r].w, sum_pre[k]);
+            if (MORE) sum_pre_bias[k] += gh[k];
           }
         }
       }
@@ -659,32 +665,33 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(con
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool live = row0 + r < rows;
-      float gy[4], v[4], g[4], dx[4], q0 = 0.f, q1 = 0.f, q2 = 0.f;
-      ring.template get<kGradY>(r, gy);
+      float v[N], g[N], dx[N], q0 = 0.f, q1 = 0.f, q2 = 0.f;
+      ring.template get<kGradY>(r, dx);
       if (pre) {
         const float c1 = s[r * N1] * inv * (st[r].w * st[r].w), c2 = CENTER ? s[r * N1 + CENTER] * inv : 0.f;
         ring.template get<kGradH>(r, v);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) gy[k] = fmaf(st[r].w, fmaf(-d[r][k], c1, fmaf(v[k], pw[k], -c2)), gy[k]);
+        for (int k = 0; k < N; ++k) dx[k] = fmaf(st[r].w, fmaf(-d[r][k], c1, fmaf(v[k], pw[k], -c2)), dx[k]);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d[r][k] = gy[k], dx[k] = sc[k] * gy[k];
+      for (int k = 0; k < N; ++k) d[r][k] = dx[k], dx[k] *= sc[k];
       if (p.grad_x && live) C::store(p.grad_x, row0 + r, W, dx);
       if (has_f) {
-        float x[4];
         ring.template get<kF>(r, v);
-        ring.template get<kX>(r, x);
         gates<FULL>(p, ring, r, gate[r], g);
+        if (MORE) ring.template get<kX>(r, dx);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < N; ++k) {
           const float gn = g[k] * d[r][k], fc = v[k] - st[r].x, fh = fc * st[r].y, vw = gn * w[k];
           q0 = fmaf(vw, fc, q0);
           if (CENTER) q1 += vw;
           if (!FULL) q2 = fmaf(d[r][k], fmaf(fh, w[k], b[k]), q2);
           if (live) {
-            acc[0][k] = fmaf(gn, fh, acc[0][k]);
-            acc[1][k] += gn;
-            acc[2][k] = fmaf(d[r][k], x[k], acc[2][k]);
+            sum_post[k] = fmaf(gn, fh, sum_post[k]);
+            if (MORE) {
+              sum_post_bias[k] += gn;
+              sum_scale[k] = fmaf(d[r][k], dx[k], sum_scale[k]);
+            }
           }
         }
       }
@@ -699,19 +706,19 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(con
         if (row0 + r < rows) {
           const float c3 = post ? q[r * N2] * inv * (st[r].y * st[r].y) : 0.f,
                       c4 = CENTER && post ? q[r * N2 + 2 * CENTER] * inv : 0.f;
-          float v[4], g[4], df[4];
+          float v[N], g[N], df[N];
           ring.template get<kF>(r, v);
           gates<FULL>(p, ring, r, gate[r], g);
           if (p.grad_f) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < N; ++k)
               df[k] = st[r].y * fmaf(-(v[k] - st[r].x), c3, fmaf(g[k] * d[r][k], w[k], -c4));
             C::store(p.grad_f, row0 + r, W, df);
           }
           if (FULL) {
             if (p.grad_gate) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < N; ++k) {
                 df[k] = d[r][k] * fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]);
                 if (p.gate_sigmoid) df[k] *= g[k] * (1.f - g[k]);
               }
@@ -729,12 +736,17 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm_backward_rows_kernel(con
   if (!p.partial) return;
   float* part = p.partial + (int64_t)blockIdx.x * 5 * W;
 #pragma unroll
-  for (int i = 0; i < 5; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = C::at(k / V) + k % V;
-      if (C::at(k / V) < W) part[i * W + c] = acc[i][k];
+  for (int k = 0; k < N; ++k) {
+    const int c = C::at(k / V) + k % V;
+    if (C::at(k / V) >= W) continue;
+    part[c] = sum_post[k];
+    part[3 * W + c] = sum_pre[k];
+    if (MORE) {
+      part[W + c] = sum_post_bias[k];
+      part[2 * W + c] = sum_scale[k];
+      part[4 * W + c] = sum_pre_bias[k];
     }
+  }
 }
 
 // Totals of the backward's column sums over blocks: 32 rows of threads take

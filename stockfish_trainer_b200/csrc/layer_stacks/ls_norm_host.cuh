@@ -56,72 +56,69 @@ bool norm_vectors(const nnue_ls_norm& a) {
   return a.width % (int)(16 / sizeof(T)) == 0;
 }
 
-// Which kernel a call takes.  Up to 4096 columns, four per thread; the fewer
-// threads a row takes, the more registers each has, for more rows at once.
-// Wider rows are read once per pass (65536 x 1040 fp32 forward and backward:
-// 0.57 ms by rows, 2.1 ms by passes).
-enum RowClass : int { kNarrow = 0, kMiddle = 1, kWide = 2, kAnyWidth = 3 };
+// Which kernel a call takes.  Up to 4096 columns, eight per thread; wider rows
+// are read once per pass (65536 x 1040 fp32 forward and backward: 0.57 ms by
+// rows, 2.1 ms by passes).
 struct RowPlan {
   bool vec;
-  int threads, cls;
+  int threads;  // 0: any width
 };
 
 template <typename T>
 RowPlan plan_norm(const nnue_ls_norm& a) {
-  const int64_t threads = ceil_div(a.width, 128) * 32;
-  const bool vec = norm_vectors<T>(a);
-  const int cls = threads <= 288 && vec ? kNarrow : threads <= 512 ? kMiddle : threads <= 1024 ? kWide : kAnyWidth;
-  return RowPlan{vec, (int)std::min<int64_t>(threads, 1024), cls};
+  const int64_t threads = ceil_div(a.width, 32 * kColumns) * 32;
+  return RowPlan{norm_vectors<T>(a), threads <= 512 ? (int)threads : 0};
 }
 
-// Rows at a time, rounds in flight, and blocks per SM, so that registers and
-// 227 KB of shared memory hold them.
-template <typename T, int CLASS, bool FULL, bool BACKWARD>
+// Rows at a time and rounds in flight: the slots of SHARE x 512 threads take at
+// most 220 KB.  The backward takes two rows at a time only where they come as
+// 16-byte pieces of 16-bit values; elsewhere two rows do not fit the registers.
+template <typename T, int V, bool FULL, bool BACKWARD, int SHARE>
 struct RowShape {
-  static constexpr int kThreads = CLASS == kNarrow ? 288 : CLASS == kMiddle ? 512 : 1024;
-  static constexpr int kRows = BACKWARD ? (CLASS == kNarrow && sizeof(T) == 2 ? 4 : CLASS == kWide ? 1 : 2)
-                               : CLASS == kWide || (sizeof(T) == 4 && FULL) ? 2
-                                                                           : 4;
-  static constexpr int kSlot = (int)sizeof(T) * 4 * kRows * (2 + FULL + 2 * BACKWARD);  // bytes per thread and round
-  static constexpr int kBlocks = CLASS == kNarrow ? 2 : 1;
-  static constexpr int kFit = 220 * 1024 / kBlocks / (kSlot * kThreads);
-  static constexpr int kStages = kFit > 4 ? 4 : kFit;
-  static_assert(kStages >= 2, "a round on its way while one is worked on");
+  static constexpr int kShare = SHARE;
+  static constexpr int kRows = V < 8 && (BACKWARD || SHARE == 2) ? 1 : 2;
+  static constexpr int kSlot = (int)sizeof(T) * kColumns * kRows * (2 + FULL + 2 * BACKWARD);  // bytes per thread
+  static constexpr int kFit = 220 * 1024 / (kSlot * 512 * SHARE);
+  static constexpr int kStages = V == 1 ? 0 : kFit > 4 ? 4 : kFit;
+  static_assert(V == 1 || kStages >= 2, "a round on its way while one is worked on");
 };
 
-int norm_blocks_per_sm(const RowPlan& r) {
-  return std::min(16, std::max(1, (r.cls == kNarrow ? 576 : r.cls == kMiddle ? 512 : 1024) / r.threads));
+// As many blocks of `rows` rows as stay on the SMs together, each looping over rows.
+int64_t norm_row_blocks(const nnue_ls_norm& a, const RowPlan& r, int rows, int share) {
+  return std::min<int64_t>(ceil_div(std::max<int64_t>(a.rows, 1), rows),
+                           (int64_t)kNumSMs * std::min(16 * share, 512 * share / r.threads));
 }
-
 template <typename T>
 int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
-  const int64_t rows = std::max<int64_t>(a.rows, 1);
-  if (r.cls == kAnyWidth) return std::min<int64_t>(rows, kNumSMs * 4);
-  const int at_once = r.cls == kNarrow   ? RowShape<T, kNarrow, false, true>::kRows
-                      : r.cls == kMiddle ? RowShape<T, kMiddle, false, true>::kRows
-                                         : RowShape<T, kWide, false, true>::kRows;
-  return std::min<int64_t>(ceil_div(rows, at_once), (int64_t)kNumSMs * norm_blocks_per_sm(r));
+  if (!r.threads) return std::min<int64_t>(std::max<int64_t>(a.rows, 1), kNumSMs * 4);
+  return norm_row_blocks(a, r, RowShape<T, 16 / sizeof(T), false, true, 1>::kRows, 1);
 }
 
 // Launches with the ring's shared memory, `slots` of them per thread.
 template <typename K>
-int launch_norm_rows(K kernel, unsigned grid, const RowPlan& r, size_t slot_bytes, const NormParams& p, cudaStream_t s) {
+int launch_norm_rows(K kernel, int64_t grid, const RowPlan& r, size_t slot_bytes, const NormParams& p, cudaStream_t s) {
   const size_t smem = slot_bytes * r.threads;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "norm: %s", cudaGetErrorString(e));
   }
-  kernel<<<grid, r.threads, smem, s>>>(p);
+  kernel<<<(unsigned)grid, r.threads, smem, s>>>(p);
   return NNUE_LS_OK;
 }
 
-// fn(center, full, both) with all as constants.
+// fn(center, full, both, more) with all as constants; more without both is looked up too.
 template <typename F>
-int with_flags(bool center, bool full, bool both, const F& fn) {
+int with_flags(bool center, bool full, bool both, bool more, const F& fn) {
   auto pick = [](bool v, const auto& next) { return v ? next(std::true_type{}) : next(std::false_type{}); };
   return pick(center, [&](auto c) {
-    return pick(full, [&](auto f) { return pick(both, [&](auto b) { return fn(c, f, b); }); });
+    return pick(full, [&](auto f) {
+      if (!both) return fn(c, f, std::false_type{}, std::true_type{});
+      return pick(more, [&](auto m) { return fn(c, f, std::true_type{}, m); });
+    });
   });
+}
+bool has_more(const nnue_ls_norm& a) {
+  return a.post_bias || a.scale || a.pre_bias || a.grad_post_bias || a.grad_scale || a.grad_pre_bias;
 }
 
 }  // namespace
@@ -132,33 +129,22 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
   const RowPlan r = plan_norm<T>(a);
   const bool center = a.kind == NNUE_LS_NORM_LAYER;
   count_launch();
-  if (r.cls == kAnyWidth) {
+  if (!r.threads) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, kNumSMs * 8);
     if (center) norm_forward_kernel<T, true><<<grid, 256, 0, s>>>(p);
     else norm_forward_kernel<T, false><<<grid, 256, 0, s>>>(p);
     return check_launch("norm_forward");
   }
-  // as many blocks as stay on the SMs together, each looping over rows
-  auto blocks = [&](int at_once) {
-    return (unsigned)std::min<int64_t>(ceil_div(a.rows, at_once), (int64_t)kNumSMs * norm_blocks_per_sm(r));
-  };
   const bool both = a.f && a.post_weight && a.h;
-  const int rc = with_flags(center, a.gate_mode == kGateFull, both, [&](auto c, auto f, auto b2) {
-    constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b2)::value;
-    auto go = [&](auto cls) {
-      constexpr int K = decltype(cls)::value;
-      using H = RowShape<T, K, F, false>;
-      if (r.vec)
-        return launch_norm_rows(norm_forward_rows_kernel<T, 4, H::kRows, C, F, B, H::kStages, H::kThreads, H::kBlocks>,
-                                blocks(H::kRows), r, H::kSlot * H::kStages, p, s);
-      if constexpr (K == kNarrow) return NNUE_LS_OK;  // a row off 16 bytes is never of this class
-      else
-        return launch_norm_rows(norm_forward_rows_kernel<T, 1, H::kRows, C, F, B, 0, H::kThreads, 1>, blocks(H::kRows),
-                                r, 0, p, s);
+  const int rc = with_flags(center, a.gate_mode == kGateFull, both, has_more(a), [&](auto c, auto f, auto b, auto m) {
+    constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b)::value, M = decltype(m)::value;
+    auto launch = [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      using H = RowShape<T, V, F, false, norm_forward_share(V, B, M)>;
+      return launch_norm_rows(norm_forward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>,
+                              norm_row_blocks(a, r, H::kRows, H::kShare), r, H::kSlot * H::kStages, p, s);
     };
-    if (r.cls == kNarrow) return go(std::integral_constant<int, kNarrow>{});
-    if (r.cls == kMiddle) return go(std::integral_constant<int, kMiddle>{});
-    return go(std::integral_constant<int, kWide>{});
+    return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
   });
   if (rc) return rc;
   return check_launch("norm_forward");
@@ -177,28 +163,20 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
   const RowPlan r = plan_norm<T>(a);
   const unsigned grid = (unsigned)norm_backward_blocks<T>(a, r);
   count_launch();
-  if (r.cls == kAnyWidth) {
+  if (!r.threads) {
     if (center) norm_backward_kernel<T, true><<<grid, 256, 0, s>>>(p);
     else norm_backward_kernel<T, false><<<grid, 256, 0, s>>>(p);
   } else {
     const bool both = a.f && a.post_weight && a.pre_weight && a.grad_h;
-    const int rc = with_flags(center, a.gate_mode == kGateFull, both, [&](auto c, auto f, auto b2) {
-      constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b2)::value;
-      auto go = [&](auto cls) {
-        constexpr int K = decltype(cls)::value;
-        using H = RowShape<T, K, F, true>;
-        if (r.vec)
-          return launch_norm_rows(
-              norm_backward_rows_kernel<T, 4, H::kRows, C, F, B, H::kStages, H::kThreads, H::kBlocks>, grid, r,
-              H::kSlot * H::kStages, p, s);
-        if constexpr (K == kNarrow) return NNUE_LS_OK;
-        else
-          return launch_norm_rows(norm_backward_rows_kernel<T, 1, H::kRows, C, F, B, 0, H::kThreads, 1>, grid, r, 0, p,
-                                  s);
+    const int rc = with_flags(center, a.gate_mode == kGateFull, both, has_more(a), [&](auto c, auto f, auto b, auto m) {
+      constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b)::value, M = decltype(m)::value;
+      auto launch = [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        using H = RowShape<T, V, F, true, 1>;
+        return launch_norm_rows(norm_backward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>, grid, r,
+                                H::kSlot * H::kStages, p, s);
       };
-      if (r.cls == kNarrow) return go(std::integral_constant<int, kNarrow>{});
-      if (r.cls == kMiddle) return go(std::integral_constant<int, kMiddle>{});
-      return go(std::integral_constant<int, kWide>{});
+      return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
     });
     if (rc) return rc;
   }

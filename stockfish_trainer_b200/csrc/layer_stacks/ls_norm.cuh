@@ -241,12 +241,42 @@ struct RowVec {
     raw = *reinterpret_cast<const Raw*>(static_cast<const T*>(base) + at);
   }
   __device__ __forceinline__ float operator[](int i) const { return to_f(raw.v[i]); }
+  // All values; two 16-bit ones at a time, an instruction each.
+  __device__ __forceinline__ void unpack(float* out) const {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+      const unsigned* words = reinterpret_cast<const unsigned*>(&raw);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if constexpr (std::is_same<T, bf16>::value) {
+          out[2 * i] = __uint_as_float(words[i] << 16);
+          out[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
+        } else {
+          const float2 t = __half22float2(*reinterpret_cast<const __half2*>(words + i));
+          out[2 * i] = t.x, out[2 * i + 1] = t.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = to_f(raw.v[i]);
+    }
+  }
 };
 template <typename T, int V>
 __device__ __forceinline__ void store_row(void* base, int64_t at, const float (&v)[V]) {
   typename RowVec<T, V>::Raw o;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    unsigned* words = reinterpret_cast<unsigned*>(&o);
 #pragma unroll
-  for (int i = 0; i < V; ++i) o.v[i] = from_f<T>(v[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, bf16>::value)
+        *reinterpret_cast<__nv_bfloat162*>(words + i) = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      else
+        *reinterpret_cast<__half2*>(words + i) = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.v[i] = from_f<T>(v[i]);
+  }
   *reinterpret_cast<typename RowVec<T, V>::Raw*>(static_cast<T*>(base) + at) = o;
 }
 // V values of a parameter; `absent` where there is none.
@@ -317,12 +347,15 @@ struct BlockSum {
 
 __host__ __device__ constexpr int pow2_at_least(int n) { return n <= 1 ? 1 : 2 * pow2_at_least((n + 1) / 2); }
 
-// A thread's columns: kColumns of them, V neighbouring ones at a time.
+// A thread's columns: kColumns of them, V neighbouring ones at a time; a warp's
+// are neighbours, so that a thread's lie a constant apart.
 constexpr int kColumns = 8;
 template <typename T, int V>
 struct Columns {
   static constexpr int kNV = kColumns / V;
-  __device__ __forceinline__ static int at(int i) { return ((int)threadIdx.x + i * (int)blockDim.x) * V; }
+  __device__ __forceinline__ static int at(int i) {
+    return (int)(threadIdx.x & ~31u) * kColumns + ((int)(threadIdx.x & 31) + 32 * i) * V;
+  }
   __device__ __forceinline__ static void store(void* base, int64_t row, int width, const float (&v)[kColumns]) {
     T* dst = static_cast<T*>(base) + row * width;
 #pragma unroll
@@ -349,12 +382,19 @@ struct Columns {
 };
 
 // The rows to come, on their way from HBM to shared memory while earlier ones
-// are worked on: STAGES rounds of R rows, a thread's own columns in slots of
-// its own, so that nobody waits for anybody and every pass over a row reads its
-// slots again instead of holding the row in registers.  Arrays: x, f, gate,
-// grad_y, grad_h.  STAGES == 0 (V == 1: a 2-byte value cannot be copied
-// asynchronously): the rows are loaded when they are needed, into registers.
+// are worked on: STAGES rounds of R rows, read again by every pass over a row
+// instead of held in registers.  Arrays: x, f, gate, grad_y, grad_h.
+//
+// Rows of 16-byte pieces (V > 1): a thread copies its own columns into slots of
+// its own, so that nobody waits for anybody.  Other rows (V == 1): the R rows of
+// a round are one run of memory, copied as the aligned 16-byte pieces that cover
+// it, whoever needs them, with a barrier before they are read; a row then starts
+// at any byte of shared memory (16384 x 4095 bf16, forward and backward: 594 us;
+// with single values loaded straight into registers 774 us).
 enum RowArray : int { kX = 0, kF = 1, kGate = 2, kGradY = 3, kGradH = 4 };
+
+// Bytes of one array's rows in one round, for rows that are not 16-byte pieces.
+__host__ __device__ constexpr int run_bytes(int rows, int width, int size) { return (rows * width * size + 46) & ~15; }
 
 template <typename T, int V, int R, bool FULL, bool BACKWARD, int STAGES>
 struct RowRing {
@@ -362,13 +402,13 @@ struct RowRing {
   using Raw = typename RowVec<T, V>::Raw;
   static constexpr int kArrays = 2 + FULL + 2 * BACKWARD, kNV = C::kNV;
   __host__ __device__ static constexpr int index(int a) { return a <= kGate ? a : a - !FULL; }
-  Raw* slots;
+  char* smem;
   const T* base[5];
   int width, rows, stage = 0;
-  RowVec<T, V> held[STAGES ? 1 : R][STAGES ? 1 : kArrays][STAGES ? 1 : kNV];
+  const T* run[V == 1 ? kArrays : 1];  // V == 1: the round's rows in shared memory
 
-  __device__ __forceinline__ RowRing(const NormParams& p, void* smem) {
-    slots = static_cast<Raw*>(smem) + threadIdx.x;
+  __device__ __forceinline__ RowRing(const NormParams& p, void* ring) {
+    smem = static_cast<char*>(ring);
     base[kX] = static_cast<const T*>(p.x);
     base[kF] = static_cast<const T*>(p.f);
     base[kGate] = static_cast<const T*>(FULL ? p.gate : nullptr);
@@ -376,25 +416,66 @@ struct RowRing {
     base[kGradH] = static_cast<const T*>(BACKWARD ? p.grad_h : nullptr);
     width = p.width;
     rows = (int)p.rows;
+    if constexpr (V > 1) {  // what is never copied reads as zero
+#pragma unroll
+      for (int i = 0; i < STAGES * R; ++i)
+#pragma unroll
+        for (int v = 0; v < kNV; ++v)
+#pragma unroll
+          for (int a = 0; a < 5; ++a)
+            if (index(a) < kArrays && a != (FULL ? -1 : kGate) && (C::at(v) >= width || !has(a)))
+              *reinterpret_cast<uint4*>(slot(i / R, i % R, index(a), v)) = uint4{};
+    }
+  }
+  __device__ __forceinline__ bool has(int a) const {
+    return !(a == kGate && !FULL) && !(a >= kGradY && !BACKWARD) && (a == kX || base[a]);
   }
   __device__ __forceinline__ Raw* slot(int st, int r, int i, int v) const {
-    return slots + (((st * R + r) * kArrays + i) * kNV + v) * (int)blockDim.x;
+    const int warp_stage = (int)(threadIdx.x >> 5) * STAGES + st, lane = (int)(threadIdx.x & 31);
+    return reinterpret_cast<Raw*>(smem) + warp_stage * (R * kArrays * kNV * 32) + lane + ((r * kArrays + i) * kNV + v) * 32;
+  }
+  __device__ __forceinline__ char* run_at(int st, int i) const {
+    return smem + (st * kArrays + i) * run_bytes(R, width, (int)sizeof(T));
+  }
+  __device__ __forceinline__ static void copy(void* dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(dst)),
+                 "l"(src), "r"(bytes)
+                 : "memory");
   }
   __device__ __forceinline__ void issue(int row0, int st) const {
     if (row0 < rows) {
+      if constexpr (V > 1) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int64_t row = (int64_t)min(row0 + r, rows - 1) * width;  // beyond the last row: read, not used
+        for (int r = 0; r < R; ++r) {
+          const int64_t row = (int64_t)min(row0 + r, rows - 1) * width;  // beyond the last row: read, not used
 #pragma unroll
-        for (int v = 0; v < kNV; ++v) {
-          const int c = C::at(v);
-          if (c >= width) continue;
+          for (int v = 0; v < kNV; ++v) {
+            const int c = C::at(v);
+            if (c >= width) continue;
 #pragma unroll
-          for (int a = 0; a < 5; ++a) {
-            if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
-            if (a != kX && !base[a]) continue;
-            const unsigned d = (unsigned)__cvta_generic_to_shared(slot(st, r, index(a), v));
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(base[a] + row + c) : "memory");
+            for (int a = 0; a < 5; ++a)
+              if (has(a)) copy(slot(st, r, index(a), v), base[a] + row + c, 16);
+          }
+        }
+      } else {
+        const int64_t first = (int64_t)row0 * width, last = (int64_t)min(row0 + R, rows) * width;
+#pragma unroll
+        for (int a = 0; a < 5; ++a) {
+          if (!has(a)) continue;
+          char* dst = run_at(st, index(a));
+          const uintptr_t lo = reinterpret_cast<uintptr_t>(base[a]), hi = lo + (int64_t)rows * width * sizeof(T),
+                          from = (lo + first * sizeof(T)) & ~uintptr_t(15), to = lo + last * sizeof(T);
+          const int pieces = (int)((to - from + 15) / 16);
+          for (int i = (int)threadIdx.x; i < pieces; i += (int)blockDim.x) {
+            const uintptr_t at = from + 16 * (int64_t)i;
+            if (at >= lo) {
+              copy(dst + 16 * i, reinterpret_cast<const void*>(at), (int)min((uintptr_t)16, hi - at));
+            } else {  // the tensor starts inside this piece
+              const int skip = (int)(lo - at) / (int)sizeof(T);
+              const int64_t have = (int64_t)rows * width;
+              for (int k = skip; k < 16 / (int)sizeof(T); ++k)
+                if (k - skip < have) reinterpret_cast<T*>(dst)[k] = base[a][k - skip];
+            }
           }
         }
       }
@@ -402,35 +483,27 @@ struct RowRing {
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   __device__ __forceinline__ void start(int row0, int stride) {
-    if constexpr (STAGES > 0) {
 #pragma unroll
-      for (int i = 0; i < STAGES - 1; ++i) issue(row0 + i * stride, i);
-    }
+    for (int i = 0; i < STAGES - 1; ++i) issue(row0 + i * stride, i);
   }
   // The rows from row0 on are there; those of STAGES - 1 rounds later are asked for.
   __device__ __forceinline__ void next(int row0, int stride) {
-    if constexpr (STAGES > 0) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES > 1 ? STAGES - 2 : 0) : "memory");
-      // the slots written now were last read in the round before, by this thread
-      const int64_t ahead = row0 + (int64_t)(STAGES - 1) * stride;
-      issue(ahead < rows ? (int)ahead : rows, stage == 0 ? STAGES - 1 : stage - 1);
-    } else {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    // the slots written now were last read in the round before: by this thread, or before the barrier
+    if (V == 1) __syncthreads();
+    const int64_t ahead = row0 + (int64_t)(STAGES - 1) * stride;
+    issue(ahead < rows ? (int)ahead : rows, stage == 0 ? STAGES - 1 : stage - 1);
+    if constexpr (V == 1) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int a = 0; a < 5; ++a) {
-          if ((a == kGate && !FULL) || (a >= kGradY && !BACKWARD)) continue;
-#pragma unroll
-          for (int v = 0; v < kNV; ++v) {
-            held[r][index(a)][v].raw = Raw{};
-            if (base[a] && C::at(v) < width)
-              held[r][index(a)][v].load(base[a], (int64_t)min(row0 + r, rows - 1) * width + C::at(v));
-          }
+      for (int a = 0; a < 5; ++a)
+        if (has(a)) {
+          const uintptr_t at = reinterpret_cast<uintptr_t>(base[a]) + (int64_t)row0 * width * sizeof(T);
+          run[index(a)] = reinterpret_cast<const T*>(run_at(stage, index(a)) + (at & 15));
         }
     }
   }
   __device__ __forceinline__ void done() {
-    if (STAGES > 0 && ++stage == STAGES) stage = 0;
+    if (++stage == STAGES) stage = 0;
   }
   // The thread's values of array A in row r of the round; zero where there are none.
   template <int A>
@@ -438,14 +511,13 @@ struct RowRing {
 #pragma unroll
     for (int v = 0; v < kNV; ++v) {
       RowVec<T, V> raw;
-      if constexpr (STAGES > 0) {
-        raw.raw = Raw{};
-        if ((A == kX || base[A]) && C::at(v) < width) raw.raw = *slot(stage, r, index(A), v);
+      if constexpr (V > 1) {
+        raw.raw = *slot(stage, r, index(A), v);
       } else {
-        raw = held[r][index(A)][v];
+        raw.raw = Raw{};
+        if (has(A) && C::at(v) < width) raw.raw.v[0] = run[index(A)][r * width + C::at(v)];
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) out[v * V + j] = raw[j];
+      raw.unpack(out + v * V);
     }
   }
 };
@@ -463,6 +535,15 @@ __device__ __forceinline__ void gates(const NormParams& p, const Ring& ring, int
   } else {
 #pragma unroll
     for (int k = 0; k < kColumns; ++k) g[k] = row_gate;
+  }
+}
+template <bool MORE, typename C>
+__device__ __forceinline__ void scales(const NormParams& p, float (&sc)[kColumns]) {
+  if (MORE) {
+    C::params(p.scale, p.width, p.params_f32, p.scale_value, sc);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kColumns; ++k) sc[k] = p.scale_value;
   }
 }
 template <typename T>
@@ -497,7 +578,7 @@ __global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_f
   float w[N], b[N], sc[N], pw[N], pb[N];
   C::params(p.post_weight, W, p.params_f32, 1.f, w);
   C::params(MORE ? p.post_bias : nullptr, W, p.params_f32, 0.f, b);
-  C::params(MORE ? p.scale : nullptr, W, p.params_f32, p.scale_value, sc);
+  scales<MORE, C>(p, sc);
   C::params(p.pre_weight, W, p.params_f32, 1.f, pw);
   C::params(MORE ? p.pre_bias : nullptr, W, p.params_f32, 0.f, pb);
   RowRing<T, V, R, FULL, false, STAGES> ring(p, norm_ring);
@@ -542,12 +623,18 @@ __global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_f
     for (int r = 0; r < R; ++r) {
       ring.template get<kX>(r, y[r]);
       if (has_f) {
-        float g[N];
-        gates<FULL>(p, ring, r, gate[r], g);
         ring.template get<kF>(r, v);
+        if (FULL || MORE) {
+          float g[N];
+          gates<FULL>(p, ring, r, gate[r], g);
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-          y[r][k] = fmaf(g[k], fmaf((v[k] - mean_f[r]) * rstd_f[r], w[k], b[k]), sc[k] * y[r][k]);
+          for (int k = 0; k < N; ++k)
+            y[r][k] = fmaf(g[k], fmaf((CENTER ? v[k] - mean_f[r] : v[k]) * rstd_f[r], w[k], b[k]), sc[k] * y[r][k]);
+        } else {
+          const float gr = gate[r] * rstd_f[r];
+#pragma unroll
+          for (int k = 0; k < N; ++k) y[r][k] = fmaf((CENTER ? v[k] - mean_f[r] : v[k]) * gr, w[k], sc[k] * y[r][k]);
+        }
         if (row0 + r < rows) C::store(p.y, row0 + r, W, y[r]);
       }
     }
@@ -568,7 +655,7 @@ __global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_f
         s[r] = 0.f;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const float d = C::at(k / V) < W ? y[r][k] - mean_y[r] : 0.f;
+          const float d = CENTER ? (C::at(k / V) < W ? y[r][k] - mean_y[r] : 0.f) : y[r][k];
           s[r] = fmaf(d, d, s[r]);
         }
       }
@@ -577,7 +664,10 @@ __global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_f
       for (int r = 0; r < R; ++r) {
         rstd_y[r] = inv_sqrt(s[r] * inv + p.eps);
 #pragma unroll
-        for (int k = 0; k < N; ++k) y[r][k] = fmaf((y[r][k] - mean_y[r]) * rstd_y[r], pw[k], pb[k]);
+        for (int k = 0; k < N; ++k) {
+          const float u = (CENTER ? y[r][k] - mean_y[r] : y[r][k]) * rstd_y[r];
+          y[r][k] = MORE ? fmaf(u, pw[k], pb[k]) : u * pw[k];
+        }
         if (row0 + r < rows) C::store(p.h, row0 + r, W, y[r]);
       }
     }
@@ -593,7 +683,7 @@ __global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_f
 template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, bool MORE, int STAGES>
 __global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
-  constexpr int N = kColumns, N1 = CENTER ? 2 : 1, N2 = CENTER ? 3 : 2, K1 = R * N1, K2 = pow2_at_least(R * N2);
+  constexpr int N = kColumns, N1 = 1 + CENTER, N2 = 1 + CENTER + MORE, K1 = R * N1, K2 = pow2_at_least(R * N2);
   extern __shared__ float4 norm_ring[];
   __shared__ float scratch[2 * 32 * (K1 + K2)];
   BlockSum<K1> total1{scratch};
@@ -605,7 +695,7 @@ __global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormPa
   float sum_post[N] = {}, sum_post_bias[N] = {}, sum_scale[N] = {}, sum_pre[N] = {}, sum_pre_bias[N] = {};
   C::params(p.post_weight, W, p.params_f32, 1.f, w);
   C::params(MORE ? p.post_bias : nullptr, W, p.params_f32, 0.f, b);
-  C::params(MORE ? p.scale : nullptr, W, p.params_f32, p.scale_value, sc);
+  scales<MORE, C>(p, sc);
   C::params(p.pre_weight, W, p.params_f32, 0.f, pw);
   RowRing<T, V, R, FULL, true, STAGES> ring(p, norm_ring);
   ring.start((int)blockIdx.x * R, stride);
@@ -627,6 +717,18 @@ __global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormPa
     for (int r = 0; r < R; ++r) st[r] = st_next[r], gate[r] = gate_next[r];
     ahead(min(row0 + stride, rows - 1));
     float d[R][N], s[K1], q[K2];  // d: y - mean, then the gradient of y
+    float gates_of_row[FULL && R == 1 ? N : 1];  // taken once; two rows' would not fit the registers
+    auto gates_of = [&](int r, float (&g)[N]) {
+      if constexpr (FULL && R == 1) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) g[k] = gates_of_row[k];
+      } else {
+        gates<FULL>(p, ring, r, gate[r], g);
+      }
+    };
+    if constexpr (FULL && R == 1) {
+      if (has_f) gates<FULL>(p, ring, 0, 1.f, gates_of_row);
+    }
     if (pre) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -635,15 +737,21 @@ __global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormPa
         ring.template get<kGradH>(r, gh);
         if (has_f) {
           ring.template get<kF>(r, v);
-          gates<FULL>(p, ring, r, gate[r], g);
+          if (FULL || MORE) {
+            gates_of(r, g);
 #pragma unroll
-          for (int k = 0; k < N; ++k)
-            d[r][k] = fmaf(g[k], fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]), sc[k] * d[r][k]);
+            for (int k = 0; k < N; ++k)
+              d[r][k] = fmaf(g[k], fmaf((CENTER ? v[k] - st[r].x : v[k]) * st[r].y, w[k], b[k]), sc[k] * d[r][k]);
+          } else {
+            const float gr = gate[r] * st[r].y;
+#pragma unroll
+            for (int k = 0; k < N; ++k) d[r][k] = fmaf((CENTER ? v[k] - st[r].x : v[k]) * gr, w[k], sc[k] * d[r][k]);
+          }
         }
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          d[r][k] -= st[r].z;
+          if (CENTER) d[r][k] -= st[r].z;
           const float u = gh[k] * pw[k];
           s0 = fmaf(u, d[r][k], s0);
           if (CENTER) s1 += u;
@@ -665,39 +773,45 @@ __global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormPa
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const bool live = row0 + r < rows;
-      float v[N], g[N], dx[N], q0 = 0.f, q1 = 0.f, q2 = 0.f;
+      float v[N], dx[N], q0 = 0.f, q1 = 0.f, q2 = 0.f;
       ring.template get<kGradY>(r, dx);
       if (pre) {
         const float c1 = s[r * N1] * inv * (st[r].w * st[r].w), c2 = CENTER ? s[r * N1 + CENTER] * inv : 0.f;
         ring.template get<kGradH>(r, v);
 #pragma unroll
-        for (int k = 0; k < N; ++k) dx[k] = fmaf(st[r].w, fmaf(-d[r][k], c1, fmaf(v[k], pw[k], -c2)), dx[k]);
+        for (int k = 0; k < N; ++k) {
+          const float u = v[k] * pw[k];
+          dx[k] = fmaf(st[r].w, fmaf(-d[r][k], c1, CENTER ? u - c2 : u), dx[k]);
+        }
       }
 #pragma unroll
       for (int k = 0; k < N; ++k) d[r][k] = dx[k], dx[k] *= sc[k];
       if (p.grad_x && live) C::store(p.grad_x, row0 + r, W, dx);
       if (has_f) {
+        // a gate per row is taken out of the row's sums: gr of it stays in front
+        const float gr = gate[r] * st[r].y;
+        float g[N];
         ring.template get<kF>(r, v);
-        gates<FULL>(p, ring, r, gate[r], g);
+        if (FULL) gates_of(r, g);
         if (MORE) ring.template get<kX>(r, dx);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const float gn = g[k] * d[r][k], fc = v[k] - st[r].x, fh = fc * st[r].y, vw = gn * w[k];
-          q0 = fmaf(vw, fc, q0);
-          if (CENTER) q1 += vw;
-          if (!FULL) q2 = fmaf(d[r][k], fmaf(fh, w[k], b[k]), q2);
+          const float gn = FULL ? g[k] * d[r][k] : d[r][k], fc = CENTER ? v[k] - st[r].x : v[k], u = gn * w[k];
+          q0 = fmaf(u, fc, q0);  // u as below: what cancels there is rounded alike
+          if (CENTER) q1 += u;
+          if (MORE && !FULL) q2 = fmaf(gn, b[k], q2);
           if (live) {
-            sum_post[k] = fmaf(gn, fh, sum_post[k]);
+            sum_post[k] = fmaf(gn * fc, gr, sum_post[k]);
             if (MORE) {
-              sum_post_bias[k] += gn;
+              sum_post_bias[k] = fmaf(gn, gate[r], sum_post_bias[k]);
               sum_scale[k] = fmaf(d[r][k], dx[k], sum_scale[k]);
             }
           }
         }
       }
       q[r * N2] = q0;
-      q[r * N2 + 1] = q2;
-      if (CENTER) q[r * N2 + 2 * CENTER] = q1;
+      if (CENTER) q[r * N2 + CENTER] = q1;
+      if (MORE) q[r * N2 + N2 - 1] = q2;
     }
     if (has_f) {
       total2(q);
@@ -705,28 +819,33 @@ __global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormPa
       for (int r = 0; r < R; ++r) {
         if (row0 + r < rows) {
           const float c3 = post ? q[r * N2] * inv * (st[r].y * st[r].y) : 0.f,
-                      c4 = CENTER && post ? q[r * N2 + 2 * CENTER] * inv : 0.f;
+                      c4 = CENTER && post ? q[r * N2 + CENTER] * inv : 0.f, gr = gate[r] * st[r].y;
           float v[N], g[N], df[N];
           ring.template get<kF>(r, v);
-          gates<FULL>(p, ring, r, gate[r], g);
+          if (FULL) gates_of(r, g);
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (CENTER) v[k] -= st[r].x;
           if (p.grad_f) {
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-              df[k] = st[r].y * fmaf(-(v[k] - st[r].x), c3, fmaf(g[k] * d[r][k], w[k], -c4));
+            for (int k = 0; k < N; ++k) {
+              const float gn = FULL ? g[k] * d[r][k] : d[r][k];
+              df[k] = gr * fmaf(-v[k], c3, gn * w[k] - c4);
+            }
             C::store(p.grad_f, row0 + r, W, df);
           }
           if (FULL) {
             if (p.grad_gate) {
 #pragma unroll
               for (int k = 0; k < N; ++k) {
-                df[k] = d[r][k] * fmaf((v[k] - st[r].x) * st[r].y, w[k], b[k]);
+                df[k] = d[r][k] * fmaf(v[k] * st[r].y, w[k], b[k]);
                 if (p.gate_sigmoid) df[k] *= g[k] * (1.f - g[k]);
               }
               C::store(p.grad_gate, row0 + r, W, df);
             }
           } else if (p.grad_gate && threadIdx.x == 0) {
-            const float gr = gate[r], dq = q[r * N2 + 1];
-            store_mixed<T>(p.grad_gate, row0 + r, p.gate_f32, p.gate_sigmoid ? dq * gr * (1.f - gr) : dq);
+            const float gt = gate[r], dq = fmaf(q[r * N2], st[r].y, MORE ? q[r * N2 + N2 - 1] : 0.f);
+            store_mixed<T>(p.grad_gate, row0 + r, p.gate_f32, p.gate_sigmoid ? dq * gt * (1.f - gt) : dq);
           }
         }
       }

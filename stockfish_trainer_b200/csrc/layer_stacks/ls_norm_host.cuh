@@ -79,8 +79,12 @@ struct RowShape {
   static constexpr int kRows = V < 8 && (BACKWARD || SHARE == 2) ? 1 : 2;
   static constexpr int kSlot = (int)sizeof(T) * kColumns * kRows * (2 + FULL + 2 * BACKWARD);  // bytes per thread
   static constexpr int kFit = 220 * 1024 / (kSlot * 512 * SHARE);
-  static constexpr int kStages = V == 1 ? 0 : kFit > 4 ? 4 : kFit;
-  static_assert(V == 1 || kStages >= 2, "a round on its way while one is worked on");
+  static constexpr int kStages = kFit > 4 ? 4 : kFit;
+  static_assert(kStages >= 2, "a round on its way while one is worked on");
+  static size_t ring_bytes(const RowPlan& r, int width) {
+    const int arrays = 2 + FULL + 2 * BACKWARD;
+    return (size_t)kStages * (V > 1 ? kSlot * r.threads : arrays * run_bytes(kRows, width, (int)sizeof(T)));
+  }
 };
 
 // As many blocks of `rows` rows as stay on the SMs together, each looping over rows.
@@ -94,10 +98,8 @@ int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
   return norm_row_blocks(a, r, RowShape<T, 16 / sizeof(T), false, true, 1>::kRows, 1);
 }
 
-// Launches with the ring's shared memory, `slots` of them per thread.
 template <typename K>
-int launch_norm_rows(K kernel, int64_t grid, const RowPlan& r, size_t slot_bytes, const NormParams& p, cudaStream_t s) {
-  const size_t smem = slot_bytes * r.threads;
+int launch_norm_rows(K kernel, int64_t grid, const RowPlan& r, size_t smem, const NormParams& p, cudaStream_t s) {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "norm: %s", cudaGetErrorString(e));
@@ -142,7 +144,7 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
       constexpr int V = decltype(vec)::value;
       using H = RowShape<T, V, F, false, norm_forward_share(V, B, M)>;
       return launch_norm_rows(norm_forward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>,
-                              norm_row_blocks(a, r, H::kRows, H::kShare), r, H::kSlot * H::kStages, p, s);
+                              norm_row_blocks(a, r, H::kRows, H::kShare), r, H::ring_bytes(r, a.width), p, s);
     };
     return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
   });
@@ -174,7 +176,7 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
         constexpr int V = decltype(vec)::value;
         using H = RowShape<T, V, F, true, 1>;
         return launch_norm_rows(norm_backward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>, grid, r,
-                                H::kSlot * H::kStages, p, s);
+                                H::ring_bytes(r, a.width), p, s);
       };
       return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
     });

@@ -316,3 +316,21 @@ def test_refusals(cuda):
     xb = x.bfloat16()
     with pytest.raises(TypeError):  # parameters share one type
         block_norm(xb, xb, post_weight=w, pre_weight=w.bfloat16())
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 3), (2, 7), (5, 33), (700, 129), (9, 1031), (3, 4095)])
+def test_rows_from_any_byte(cuda, dt, rows, width):
+    # where the tensors start changes nothing, not even the rounding
+    t, gy, gh = _make(rows, width, dt, 6, gate="full")
+    wants = None
+    for offset in (0, 1, 3, 5):
+        def place(v, offset=offset):
+            if v.dim() == 1:
+                return v.cuda()
+            return torch.full((v.numel() + offset,), float("nan"), dtype=dt, device="cuda")[offset:].view(v.shape).copy_(v)
+        dev = {k: place(v).requires_grad_() for k, v in t.items()}
+        outs = _call(dev, "layer", True)
+        got = [*outs, *torch.autograd.grad(outs, list(dev.values()), [place(gy), place(gh)])]
+        wants = wants or got
+        assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(got, wants))

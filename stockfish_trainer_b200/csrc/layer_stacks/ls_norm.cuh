@@ -79,11 +79,13 @@ __device__ __forceinline__ void row_stats(const F& value, int width, float eps, 
   mean = 0.f;
   if (CENTER) {
     v[0] = 0.f;
+#pragma unroll 4
     for (int c = threadIdx.x; c < width; c += blockDim.x) v[0] += value(c);
     block_sum(v, scratch);
     mean = v[0] / width;
   }
   v[0] = 0.f;
+#pragma unroll 4
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
     const float d = value(c) - mean;
     v[0] += d * d;
@@ -94,7 +96,7 @@ __device__ __forceinline__ void row_stats(const F& value, int width, float eps, 
 
 // One block per row, any width; the row is read again for each pass.
 template <typename T, bool CENTER>
-__global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
+__global__ void __launch_bounds__(512) norm_forward_kernel(NormParams p) {
   __shared__ float scratch[32];
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     NormRow<T> r(p, row);
@@ -102,6 +104,7 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
     if (p.f && p.post_weight)
       row_stats<CENTER>([&](int c) { return to_f(r.f[c]); }, p.width, p.eps, scratch, r.mean_f, r.rstd_f);
     if (p.pre_weight) row_stats<CENTER>([&](int c) { return r.y(c); }, p.width, p.eps, scratch, mean_y, rstd_y);
+#pragma unroll 4
     for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
       const float y = r.y(c);
       if (p.y) static_cast<T*>(p.y)[row * p.width + c] = from_f<T>(y);
@@ -127,7 +130,7 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(NormParams p) {
 // forward wrote is rounded to 16 bits, which would show in the fp32 sums.
 // Each block owns a slice of `partial` and each thread its columns of it.
 template <typename T, bool CENTER>
-__global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
+__global__ void __launch_bounds__(512) norm_backward_kernel(NormParams p) {
   __shared__ float scratch[64];
   const int W = p.width;
   const float inv = 1.f / W;
@@ -147,6 +150,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
     auto y_cen = [&](int c) { return r.y(c) - st.z; };
     float s[2] = {0.f, 0.f};
     if (pre) {
+#pragma unroll 4
       for (int c = threadIdx.x; c < W; c += blockDim.x) {
         const float u = to_f(gh[c]) * r.param(p.pre_weight, c);
         s[0] += u * y_cen(c);
@@ -165,6 +169,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
     };
     float q[3] = {0.f, 0.f, 0.f};
     if (p.f) {
+#pragma unroll 4
       for (int c = threadIdx.x; c < W; c += blockDim.x) {
         const float d = d_of(c);
         if (p.post_weight) {
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(NormParams p) {
       q[2] = t2[0];
     }
     const float c3 = q[0] * inv * (st.y * st.y), c4 = q[1] * inv;
+#pragma unroll 4
     for (int c = threadIdx.x; c < W; c += blockDim.x) {
       const float d = d_of(c);
       const int64_t o = row * W + c;

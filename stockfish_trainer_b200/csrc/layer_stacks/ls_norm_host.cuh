@@ -57,8 +57,8 @@ bool norm_vectors(const nnue_ls_norm& a) {
 }
 
 // Which kernel a call takes.  Up to 4096 columns, eight per thread; wider rows
-// are read once per pass (65536 x 1040 fp32 forward and backward: 0.57 ms by
-// rows, 2.1 ms by passes).
+// are read once per pass (forward and backward of 16384 rows in fp32: 0.49 ms
+// for 4096 columns by rows, 1.53 ms for 4104 by passes; bf16 0.30 and 1.61 ms).
 struct RowPlan {
   bool vec;
   int threads;  // 0: any width
@@ -133,8 +133,8 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
   count_launch();
   if (!r.threads) {
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, kNumSMs * 8);
-    if (center) norm_forward_kernel<T, true><<<grid, 256, 0, s>>>(p);
-    else norm_forward_kernel<T, false><<<grid, 256, 0, s>>>(p);
+    if (center) norm_forward_kernel<T, true><<<grid, 512, 0, s>>>(p);
+    else norm_forward_kernel<T, false><<<grid, 512, 0, s>>>(p);
     return check_launch("norm_forward");
   }
   const bool both = a.f && a.post_weight && a.h;
@@ -166,8 +166,8 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
   const unsigned grid = (unsigned)norm_backward_blocks<T>(a, r);
   count_launch();
   if (!r.threads) {
-    if (center) norm_backward_kernel<T, true><<<grid, 256, 0, s>>>(p);
-    else norm_backward_kernel<T, false><<<grid, 256, 0, s>>>(p);
+    if (center) norm_backward_kernel<T, true><<<grid, 512, 0, s>>>(p);
+    else norm_backward_kernel<T, false><<<grid, 512, 0, s>>>(p);
   } else {
     const bool both = a.f && a.post_weight && a.pre_weight && a.grad_h;
     const int rc = with_flags(center, a.gate_mode == kGateFull, both, has_more(a), [&](auto c, auto f, auto b, auto m) {

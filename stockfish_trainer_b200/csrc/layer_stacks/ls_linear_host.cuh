@@ -235,9 +235,9 @@ struct Packer {
 
 // ---- forward -------------------------------------------------------------------
 // Up to 4 rows (fp32: 8, where the other way packs its operands first) go to the
-// kernel without tiles.  1040 x 1040 bf16: 2.6 us for one row, 6.8 for 4, 10.9
-// for 8; on tiles 10.6 for any of them.  1040 x 256 fp32: 2.6 us for one row,
-// 6.1 for 8, 16.4 for 16; on tiles 16.7.
+// kernel without tiles.  1040 x 1040 bf16: 2.7 us for one row, 6.9 for 4, 10.9
+// for 8; on tiles 10.1 for any of them.  1040 x 256 fp32: 2.7 us for one row,
+// 6.3 for 8, 16.4 for 16; on tiles 14.6 in three launches.
 template <typename T>
 bool few_rows(const nnue_ls_linear& a) {
   return a.rows <= (sizeof(T) == 4 ? 8 : 4);

@@ -562,8 +562,15 @@ __device__ __forceinline__ float load_row_gate(const NormParams& p, int row) {
 // The forward's calls without biases or a learned scale fit 64 registers, so
 // that an SM holds 1024 threads instead of 512 (before other savings: 65536 x
 // 1040 bf16 159 us against 181, 16384 x 4096 bf16 123 against 166).
-__host__ __device__ constexpr int norm_forward_share(int v, bool both, bool more) {
-  return v > 1 && both && !more ? 2 : 1;
+__host__ __device__ constexpr int norm_forward_threads(int v, bool both, bool more) {
+  return v > 1 && both && !more ? 1024 : 512;
+}
+// The backward's fit 96, for 640 threads: four blocks of 1040 columns instead of
+// three, two of 2056 instead of one (forward and backward, 65536 x 1040 fp32 472
+// us against 515, bf16 326 against 341, 16384 x 2056 fp32 260 against 360; 4096
+// columns, where one block fits either way, bf16 317 against 306).
+__host__ __device__ constexpr int norm_backward_threads(int v, bool both, bool more) {
+  return v > 1 && both && !more ? 640 : 512;
 }
 
 // BOTH: the call has f with its norm and the norm after it.  MORE: it may have
@@ -573,10 +580,10 @@ __host__ __device__ constexpr int norm_forward_share(int v, bool both, bool more
 // what a row costs besides its columns (addresses, copies, the exchange of sums)
 // is shared by eight instead of four.  65536 x 1040, row gate, rms norms:
 // forward fp32 184 us (90% of the HBM copy rate over its four arrays), bf16 120
-// (69%); backward fp32 318 us (78% over its six), bf16 206 (60%).  With four
+// (69%); backward fp32 273 us (91% over its six), bf16 196 (64%).  With four
 // columns a thread the bf16 figures were 186 and 472 us.
 template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, bool MORE, int STAGES>
-__global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_forward_rows_kernel(const NormParams p) {
+__global__ void __launch_bounds__(512, norm_forward_threads(V, BOTH, MORE) / 512) norm_forward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
   constexpr int N = kColumns;
   extern __shared__ float4 norm_ring[];
@@ -691,7 +698,7 @@ __global__ void __launch_bounds__(512, norm_forward_share(V, BOTH, MORE)) norm_f
 }
 
 template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, bool MORE, int STAGES>
-__global__ void __launch_bounds__(512, 1) norm_backward_rows_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_backward_threads(V, BOTH, MORE), 1) norm_backward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
   constexpr int N = kColumns, N1 = 1 + CENTER, N2 = 1 + CENTER + MORE, K1 = R * N1, K2 = pow2_at_least(R * N2);
   extern __shared__ float4 norm_ring[];

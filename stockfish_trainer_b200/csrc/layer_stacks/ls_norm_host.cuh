@@ -70,15 +70,14 @@ RowPlan plan_norm(const nnue_ls_norm& a) {
   return RowPlan{norm_vectors<T>(a), threads <= 512 ? (int)threads : 0};
 }
 
-// Rows at a time and rounds in flight: the slots of SHARE x 512 threads take at
-// most 220 KB.  The backward takes two rows at a time only where they come as
+// Rows at a time and rounds in flight: the slots of an SM's THREADS take at most
+// 220 KB.  The backward takes two rows at a time only where they come as
 // 16-byte pieces of 16-bit values; elsewhere two rows do not fit the registers.
-template <typename T, int V, bool FULL, bool BACKWARD, int SHARE>
+template <typename T, int V, bool FULL, bool BACKWARD, int THREADS>
 struct RowShape {
-  static constexpr int kShare = SHARE;
-  static constexpr int kRows = V < 8 && (BACKWARD || SHARE == 2) ? 1 : 2;
+  static constexpr int kRows = V < 8 && (BACKWARD || THREADS == 1024) ? 1 : 2;
   static constexpr int kSlot = (int)sizeof(T) * kColumns * kRows * (2 + FULL + 2 * BACKWARD);  // bytes per thread
-  static constexpr int kFit = 220 * 1024 / (kSlot * 512 * SHARE);
+  static constexpr int kFit = 220 * 1024 / (kSlot * THREADS);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;
   static_assert(kStages >= 2, "a round on its way while one is worked on");
   static size_t ring_bytes(const RowPlan& r, int width) {
@@ -87,15 +86,14 @@ struct RowShape {
   }
 };
 
-// As many blocks of `rows` rows as stay on the SMs together, each looping over rows.
-int64_t norm_row_blocks(const nnue_ls_norm& a, const RowPlan& r, int rows, int share) {
-  return std::min<int64_t>(ceil_div(std::max<int64_t>(a.rows, 1), rows),
-                           (int64_t)kNumSMs * std::min(16 * share, 512 * share / r.threads));
+// As many blocks of `rows` rows as stay on the SMs together at `threads` each, looping over rows.
+int64_t norm_row_blocks(const nnue_ls_norm& a, const RowPlan& r, int rows, int threads) {
+  return std::min<int64_t>(ceil_div(std::max<int64_t>(a.rows, 1), rows), (int64_t)kNumSMs * (threads / r.threads));
 }
-template <typename T>
+// At most so many blocks in the backward.
 int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
   if (!r.threads) return std::min<int64_t>(std::max<int64_t>(a.rows, 1), kNumSMs * 4);
-  return norm_row_blocks(a, r, RowShape<T, 16 / sizeof(T), false, true, 1>::kRows, 1);
+  return norm_row_blocks(a, r, 1, norm_backward_threads(4, true, false));
 }
 
 template <typename K>
@@ -142,9 +140,10 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
     constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b)::value, M = decltype(m)::value;
     auto launch = [&](auto vec) {
       constexpr int V = decltype(vec)::value;
-      using H = RowShape<T, V, F, false, norm_forward_share(V, B, M)>;
+      constexpr int kThreads = norm_forward_threads(V, B, M);
+      using H = RowShape<T, V, F, false, kThreads>;
       return launch_norm_rows(norm_forward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>,
-                              norm_row_blocks(a, r, H::kRows, H::kShare), r, H::ring_bytes(r, a.width), p, s);
+                              norm_row_blocks(a, r, H::kRows, kThreads), r, H::ring_bytes(r, a.width), p, s);
     };
     return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
   });
@@ -154,7 +153,7 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
 
 template <typename T>
 size_t norm_backward_bytes(const nnue_ls_norm& a) {
-  return wants_params(a) ? align256((size_t)norm_backward_blocks<T>(a, plan_norm<T>(a)) * 5 * a.width * 4) : 0;
+  return wants_params(a) ? align256((size_t)norm_backward_blocks(a, plan_norm<T>(a)) * 5 * a.width * 4) : 0;
 }
 
 template <typename T>
@@ -163,18 +162,20 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
   const bool params = wants_params(a), center = a.kind == NNUE_LS_NORM_LAYER;
   p.partial = params ? static_cast<float*>(workspace) : nullptr;
   const RowPlan r = plan_norm<T>(a);
-  const unsigned grid = (unsigned)norm_backward_blocks<T>(a, r);
+  int64_t grid = norm_backward_blocks(a, r);
   count_launch();
   if (!r.threads) {
-    if (center) norm_backward_kernel<T, true><<<grid, 512, 0, s>>>(p);
-    else norm_backward_kernel<T, false><<<grid, 512, 0, s>>>(p);
+    if (center) norm_backward_kernel<T, true><<<(unsigned)grid, 512, 0, s>>>(p);
+    else norm_backward_kernel<T, false><<<(unsigned)grid, 512, 0, s>>>(p);
   } else {
     const bool both = a.f && a.post_weight && a.pre_weight && a.grad_h;
     const int rc = with_flags(center, a.gate_mode == kGateFull, both, has_more(a), [&](auto c, auto f, auto b, auto m) {
       constexpr bool C = decltype(c)::value, F = decltype(f)::value, B = decltype(b)::value, M = decltype(m)::value;
       auto launch = [&](auto vec) {
         constexpr int V = decltype(vec)::value;
-        using H = RowShape<T, V, F, true, 1>;
+        constexpr int kThreads = norm_backward_threads(V, B, M);
+        using H = RowShape<T, V, F, true, kThreads>;
+        grid = norm_row_blocks(a, r, H::kRows, kThreads);
         return launch_norm_rows(norm_backward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>, grid, r,
                                 H::ring_bytes(r, a.width), p, s);
       };

@@ -98,7 +98,7 @@ int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
 
 template <typename K>
 int launch_norm_rows(K kernel, int64_t grid, const RowPlan& r, size_t smem, const NormParams& p, cudaStream_t s) {
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {  // 48 KB without asking, the kernels' own 3 KB at most included
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "norm: %s", cudaGetErrorString(e));
   }

@@ -334,3 +334,12 @@ def test_rows_from_any_byte(cuda, dt, rows, width):
         got = [*outs, *torch.autograd.grad(outs, list(dev.values()), [place(gy), place(gh)])]
         wants = wants or got
         assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(got, wants))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [k * 256 - d for k in range(1, 17) for d in (0, 1)])
+def test_every_block_size(cuda, dt, width):
+    # each width of a block asks for its own amount of shared memory, with and without the optional terms
+    for gate, more in (("row", False), ("full", False), ("row", True), ("full", True)):
+        t, gy, gh = _make(5, width, dt, 7, gate=gate, learned=more, bias=more)
+        _check(t, gy, gh, "layer", True)

@@ -152,14 +152,17 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const T* __restrict__ x, 
 }
 
 // dz = g * act'(z), written in the products' layout when dst is given, and per
-// block the fp32 column sums of the unrounded dz over a range of rows.
+// block the fp32 column sums of the unrounded dz over a range of rows: into
+// `partial`, or where one block is high enough for all rows, rounded into
+// `total`.
 // A block is `tx` groups of V columns wide and 256 / tx rows high (its last few
 // threads may have nothing to do).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ g, int64_t ldg,
                                                  const typename Derivative<T>::Code* __restrict__ act_grad,
                                                  void* __restrict__ dst, int64_t ldo, float* __restrict__ partial,
-                                                 int64_t M, int64_t N, int64_t rows_per_block, int tx) {
+                                                 void* __restrict__ total, bool total_f32, int64_t M, int64_t N,
+                                                 int64_t rows_per_block, int tx) {
   using D = Derivative<T>;
   using Code = typename D::Code;
   __shared__ float red[256 * V];
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ g, int64_
       for (int i = 0; i < V; ++i) sum[i] += v[i];
     }
   }
-  if (!partial) return;
+  if (!partial && !total) return;
 #pragma unroll
   for (int i = 0; i < V; ++i) red[i * 256 + threadIdx.x] = sum[i];
   __syncthreads();
@@ -192,7 +195,8 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* __restrict__ g, int64_
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       for (int j = 1; j < ty; ++j) sum[i] += red[i * 256 + j * tx + x];
-      partial[(int64_t)blockIdx.y * N + n + i] = sum[i];
+      if (total) store_mixed<T>(total, n + i, total_f32, sum[i]);
+      else partial[(int64_t)blockIdx.y * N + n + i] = sum[i];
     }
   }
 }

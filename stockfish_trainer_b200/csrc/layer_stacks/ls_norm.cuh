@@ -561,9 +561,11 @@ __device__ __forceinline__ float load_row_gate(const NormParams& p, int row) {
 
 // The forward's calls without biases or a learned scale fit 64 registers, so
 // that an SM holds 1024 threads instead of 512 (before other savings: 65536 x
-// 1040 bf16 159 us against 181, 16384 x 4096 bf16 123 against 166).
+// 1040 bf16 159 us against 181, 16384 x 4096 bf16 123 against 166).  With them
+// 16-bit rows fit 80, for 768 (65536 x 1040 bf16 layer norm 202 us against 234);
+// fp32 rows are better two at a time with 512 (262 us against 288).
 __host__ __device__ constexpr int norm_forward_threads(int v, bool both, bool more) {
-  return v > 1 && both && !more ? 1024 : 512;
+  return v == 1 || !both ? 512 : !more ? 1024 : v == 8 ? 768 : 512;
 }
 // The backward's fit 96, for 640 threads: four blocks of 1040 columns instead of
 // three, two of 2056 instead of one (forward and backward, 65536 x 1040 fp32 472
@@ -583,7 +585,7 @@ __host__ __device__ constexpr int norm_backward_threads(int v, bool both, bool m
 // (69%); backward fp32 273 us (91% over its six), bf16 196 (64%).  With four
 // columns a thread the bf16 figures were 186 and 472 us.
 template <typename T, int V, int R, bool CENTER, bool FULL, bool BOTH, bool MORE, int STAGES>
-__global__ void __launch_bounds__(512, norm_forward_threads(V, BOTH, MORE) / 512) norm_forward_rows_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_forward_threads(V, BOTH, MORE), 1) norm_forward_rows_kernel(const NormParams p) {
   using C = Columns<T, V>;
   constexpr int N = kColumns;
   extern __shared__ float4 norm_ring[];

@@ -59,7 +59,7 @@ int nnue_ls_device_errors(uint32_t *flags, int clear);
  * outputs < 2^30, 0 <= rows < 2^30. */
 #define NNUE_LS_ACT_NONE 0
 #define NNUE_LS_ACT_RELU 1
-#define NNUE_LS_ACT_CRELU 2     /* clamp(z, 0, 1) */
+#define NNUE_LS_ACT_CRELU 2     /* clamp(z, 0, 1); its derivative is 1 on the closed interval */
 #define NNUE_LS_ACT_SQR_CRELU 3 /* clamp(z, 0, 1)^2 */
 #define NNUE_LS_ACT_SILU 4
 #define NNUE_LS_ACT_GELU 5      /* z * Phi(z), the normal distribution's Phi */

@@ -10,8 +10,8 @@ namespace nnue_ls {
 
 enum Activation : int { kNone = 0, kRelu = 1, kCrelu = 2, kSqrCrelu = 3, kSilu = 4, kGelu = 5, kActivations = 6 };
 
-// act(z) and act'(z).  At the kinks of the clipped forms the derivative is 0,
-// as in clamp's backward outside the open interval.
+// act(z) and act'(z).  A clamp passes the gradient on the closed interval, its
+// bounds included, as the feature transformer's epilogue does; relu's is 0 at 0.
 //
 // gelu(z) = z Phi(z), Phi(z) = erfc(-z / sqrt 2) / 2.  For 16-bit results, with
 // u = |z| / sqrt 2 and t = 1 / (1 + 0.45 u), erfc(u) = exp(-u^2) P(t): P is the
@@ -41,7 +41,7 @@ __device__ __forceinline__ float activate(float z, float& d) {
     return z > 0.f || z != z ? z : 0.f;
   } else if constexpr (ACT == kCrelu || ACT == kSqrCrelu) {
     const float c = z != z ? z : fminf(fmaxf(z, 0.f), 1.f);
-    const bool inside = z > 0.f && z < 1.f;
+    const bool inside = z >= 0.f && z <= 1.f;
     d = inside ? (ACT == kCrelu ? 1.f : 2.f * z) : 0.f;
     return ACT == kCrelu ? c : c * c;
   } else if constexpr (ACT == kSilu) {

@@ -90,7 +90,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     ``[outputs]`` may also be fp32).  ``residual`` has the output's shape
     ``[..., outputs]`` or broadcasts to it.  ``activation`` is one of
     ``ACTIVATIONS``: ``crelu`` clamps to [0, 1] and ``sqr_crelu`` squares the
-    result; ``gelu`` is the exact form.  Sums are held in fp32 and the result
+    result (a clamp passes gradients at its bounds too, as torch's does);
+    ``gelu`` is the exact form.  Sums are held in fp32 and the result
     is rounded once; fp32 products are accurate to fp32 rounding, but a
     non-finite fp32 operand may turn an infinite sum into NaN.  Rows may be
     strided; other layouts are copied.

@@ -15,6 +15,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200); run with -m gpu")
 
 
+# Their expectation is wrong (crelu and sqr_crelu pass gradients at 0 and 1, as torch.clamp does; see
+# test_clipped_derivatives_at_the_bounds).  They fail, after all others, so that -x reaches those first.
+WRONG_EXPECTATION = ("test_derivatives_at_the_kinks_are_zero",)
+
+
+def pytest_collection_modifyitems(items):
+    items.sort(key=lambda item: getattr(item, "originalname", None) in WRONG_EXPECTATION)
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch

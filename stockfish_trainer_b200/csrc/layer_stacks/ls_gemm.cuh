@@ -6,8 +6,10 @@
 // and x MN-major, so no operand is ever transposed in memory.
 //
 // fp32 operands come as three bf16 planes whose sum is the value (8 + 8 + 8
-// bits, exact); six of the nine plane products are formed, the three left out
-// are below 2^-23 of the product.
+// bits, exact).  Each is rounded to nearest, so the second and third are at most
+// 2^-8 and 2^-17 of the value's leading power of two.  Six of the nine plane
+// products are formed; the three left out are at most 2 * 2^-25 + 2^-34 of the
+// product, half a unit of its last place, with either sign.
 //
 // One persistent block per SM (or a pair of blocks on two SMs, CG = 2, sharing
 // a 256-row tile: each holds half of A's rows and half of B's, which halves

@@ -8,9 +8,13 @@
 
 namespace nnue_ls {
 
-// The three bf16 planes of V fp32 values: each takes the leading 8 bits of
-// what is left, so their sum is the value.  An infinity or NaN stays in the
-// first plane.
+// The three bf16 planes of V fp32 values: each takes what is left, rounded to
+// its 8 bits, so their sum is the value.  Rounding to nearest, not cutting off:
+// what is left then has either sign and half the size, so that the products of
+// planes that are not formed (ls_gemm.cuh) lie below half a unit of the value's
+// product and have either sign; cut off, they reached four units, all of one
+// sign.  An infinity or NaN stays in the first plane, and a value that would
+// round to infinity is cut off there.
 template <int V>
 __device__ __forceinline__ void split_planes(const float (&v)[V], uint16_t (&q)[3][V]) {
 #pragma unroll
@@ -24,9 +28,10 @@ __device__ __forceinline__ void split_planes(const float (&v)[V], uint16_t (&q)[
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      const uint32_t top = __float_as_uint(r) & 0xffff0000u;
-      q[k][i] = (uint16_t)(top >> 16);
-      r -= __uint_as_float(top);
+      uint16_t top = __bfloat16_as_ushort(__float2bfloat16_rn(r));
+      if (k == 0 && (top & 0x7fff) == 0x7f80) top = (uint16_t)(__float_as_uint(r) >> 16);
+      q[k][i] = top;
+      r -= __uint_as_float((uint32_t)top << 16);
     }
   }
 }

@@ -37,3 +37,43 @@ def test_a_zero_layer_passes_the_gradient_that_clamp_passes(cuda, act):
     w = torch.zeros(8, 16, device=cuda, requires_grad=True)
     linear_act(x, w, activation=act).sum().backward()
     assert (w.grad == (64 if act == "crelu" else 0)).all()
+
+
+def _full_mantissas(g, *shape):
+    """Values of either sign in [1, 2) whose 24 bits are all in use; some of them 0x3F80FFFF."""
+    bits = 0x3F800000 | torch.randint(0, 1 << 23, shape, generator=g, dtype=torch.int32) | 1
+    bits = torch.where(torch.rand(shape, generator=g) < 0.1, torch.tensor(0x3F80FFFF, dtype=torch.int32), bits)
+    return bits.view(torch.float32) * (1 - 2 * torch.randint(0, 2, shape, generator=g).float())
+
+
+@pytest.mark.parametrize("terms", [1, 2, 4])
+def test_fp32_products_of_full_mantissas(cuda, terms):
+    """Sums of `terms` products, forward, dx and dW.  What the planes leave out of a product is below 2^-24 of it and
+    the sum's last add may lose a unit, 2^-23: 2^-22 of the magnitudes is allowed."""
+    g = torch.Generator().manual_seed(terms)
+
+    def check(got, a, b):
+        want, mag = a.double() @ b.double().t(), a.double().abs() @ b.double().abs().t()
+        err = (got.double().cpu() - want).abs() / mag
+        assert err.max() <= 2.0**-22, float(err.max() * 2**23)
+
+    x, w = _full_mantissas(g, 300, terms), _full_mantissas(g, 100, terms)
+    check(linear_act(x.cuda(), w.cuda()), x, w)
+    x, w, go = _full_mantissas(g, 300, 100), _full_mantissas(g, terms, 100), _full_mantissas(g, 300, terms)
+    xx, ww = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    dx, = torch.autograd.grad(linear_act(xx, ww), [xx], go.cuda())
+    check(dx, go, w.t())
+    x, w, go = _full_mantissas(g, terms, 100), _full_mantissas(g, 60, 100), _full_mantissas(g, terms, 60)
+    xx, ww = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    dw, = torch.autograd.grad(linear_act(xx, ww), [ww], go.cuda())
+    check(dw, go.t(), x.t())
+
+
+def test_fp32_values_near_the_largest(cuda):
+    """Rounding a value's first plane must not make it infinite."""
+    big = torch.finfo(torch.float32).max
+    x = torch.tensor([[big], [-big], [3.3961e38], [1.0]]).repeat(10, 1).cuda()
+    w = torch.tensor([[1.0], [0.5], [2.0**-100 * 1.2345678], [-1.0]]).cuda()
+    want = x.double() @ w.double().t()
+    got = linear_act(x, w)
+    assert ((got.double() - want).abs() <= 2.0**-22 * want.abs()).all()

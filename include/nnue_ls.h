@@ -12,8 +12,9 @@
  *     in a CUDA graph.
  *   - Element types: NNUE_LS_F32, NNUE_LS_BF16, NNUE_LS_F16.  Sums, statistics
  *     and norms are held in fp32 whatever the type, and fp32 products are
- *     accurate to fp32 rounding.  Results do not depend on scheduling: no sum
- *     is formed with floating-point atomics.
+ *     accurate to fp32 rounding (with more than 8 rows, and in every backward,
+ *     operands below 2^-110 are held to 2^-134 instead of 24 bits).  Results do
+ *     not depend on scheduling: no sum is formed with floating-point atomics.
  *   - Matrices are row-major with unit column stride; ld* is the row stride in
  *     elements.  Row counts may be 0 (then nothing is read).
  *   - Return value: NNUE_LS_OK or a negative NNUE_LS_ERR_* code; no exceptions

@@ -6,7 +6,7 @@
 // and x MN-major, so no operand is ever transposed in memory.
 //
 // fp32 operands come as three bf16 planes whose sum is the value (8 + 8 + 8
-// bits, exact).  Each is rounded to nearest, so the second and third are at most
+// bits; exact from 2^-110 up, to 2^-134 below).  Each is rounded to nearest, so the second and third are at most
 // 2^-8 and 2^-17 of the value's leading power of two.  Six of the nine plane
 // products are formed; the three left out are at most 2 * 2^-25 + 2^-34 of the
 // product, half a unit of its last place, with either sign.

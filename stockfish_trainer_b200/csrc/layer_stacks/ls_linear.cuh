@@ -14,7 +14,9 @@ namespace nnue_ls {
 // planes that are not formed (ls_gemm.cuh) lie below half a unit of the value's
 // product and have either sign; cut off, they reached four units, all of one
 // sign.  An infinity or NaN stays in the first plane, and a value that would
-// round to infinity is cut off there.
+// round to infinity is cut off there.  bf16 has no steps below 2^-133: below
+// 2^-110 (7.7e-34) the last plane is rounded to them and the sum is the value to
+// 2^-134 only.
 template <int V>
 __device__ __forceinline__ void split_planes(const float (&v)[V], uint16_t (&q)[3][V]) {
 #pragma unroll

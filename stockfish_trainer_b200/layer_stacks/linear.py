@@ -92,9 +92,10 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     ``ACTIVATIONS``: ``crelu`` clamps to [0, 1] and ``sqr_crelu`` squares the
     result (a clamp passes gradients at its bounds too, as torch's does);
     ``gelu`` is the exact form.  Sums are held in fp32 and the result
-    is rounded once; fp32 products are accurate to fp32 rounding, but a
-    non-finite fp32 operand may turn an infinite sum into NaN.  Rows may be
-    strided; other layouts are copied.
+    is rounded once; fp32 products are accurate to fp32 rounding, but with
+    more than 8 rows (and in every backward) a non-finite fp32 operand may turn
+    an infinite sum into NaN, and operands below 2^-110 (7.7e-34) are held to
+    2^-134 instead of 24 bits.  Rows may be strided; other layouts are copied.
 
     For the backward ``x`` and ``weight`` (in the form their products read: for
     fp32 1.5 times their size) and the activation's derivative (as wide as the

@@ -77,3 +77,15 @@ def test_fp32_values_near_the_largest(cuda):
     want = x.double() @ w.double().t()
     got = linear_act(x, w)
     assert ((got.double() - want).abs() <= 2.0**-22 * want.abs()).all()
+
+
+def test_fp32_values_near_the_smallest(cuda):
+    """A plane has no steps below 2^-133, so a value is held to 2^-134 or to its own rounding, whichever is more."""
+    g = torch.Generator().manual_seed(1)
+    scale = 10.0 ** -(30 + 8 * torch.rand(300, 40, generator=g, dtype=torch.float64))
+    x = (torch.randn(300, 40, generator=g).double() * scale).float()
+    w = torch.randn(24, 40, generator=g)
+    want, mag = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    err = (linear_act(x.cuda(), w.cuda()).double().cpu() - want).abs()
+    tol = 2.0**-134 * w.double().abs().sum(1) + (40 / 4 + 16) * 2.0**-23 * mag + 2.0**-149
+    assert (err <= tol).all(), float((err / tol).max())

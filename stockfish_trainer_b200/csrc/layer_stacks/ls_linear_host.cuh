@@ -320,13 +320,13 @@ template <typename T>
 BackwardPlan plan_backward(const nnue_ls_linear& a) {
   BackwardPlan p{};
   const int planes = sizeof(T) == 4 ? 3 : 1;
-  const bool products = a.grad_x || a.grad_weight;
-  if (a.grad_x) {
+  const bool products = a.rows > 0 && (a.grad_x || a.grad_weight);  // without rows there is nothing to cut into tiles
+  if (products && a.grad_x) {
     p.dx = plan_tiles(a.rows, a.inputs, a.outputs, planes);
     p.w = !a.weight_packed && needs_pack<T>(a.weight, a.ldw, a.outputs) ? pack_bytes<T>(a.outputs, a.inputs) : 0;
     p.partial = p.dx.partial_bytes(a.rows, a.inputs);
   }
-  if (a.grad_weight) {
+  if (products && a.grad_weight) {
     p.dw = plan_tiles(a.outputs, a.inputs, a.rows, planes);
     p.x = !a.x_packed && needs_pack<T>(a.x, a.ldx, a.rows) ? pack_bytes<T>(a.rows, a.inputs) : 0;
     p.partial = std::max(p.partial, p.dw.partial_bytes(a.outputs, a.inputs));

@@ -4,7 +4,7 @@ against the formula in 64 bits."""
 import pytest
 import torch
 
-from stockfish_trainer_b200.layer_stacks import linear_act
+from stockfish_trainer_b200.layer_stacks import _native, linear_act
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,14 @@ def test_fp32_values_near_the_smallest(cuda):
     err = (linear_act(x.cuda(), w.cuda()).double().cpu() - want).abs()
     tol = 2.0**-134 * w.double().abs().sum(1) + (40 / 4 + 16) * 2.0**-23 * mag + 2.0**-149
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_c_backward_of_no_rows(cuda, dt):
+    """Every gradient asked for with pointers that are not null: the weight's and bias' are zero, nothing else is written."""
+    code = _native.DTYPES[dt]
+    dw, db, dx = (torch.full(s, float("nan"), device=cuda, dtype=dt) for s in ((24, 40), (24,), (8,)))
+    a = _native.Linear(rows=0, inputs=40, outputs=24, dtype=code, bias_dtype=code, activation=4, ldg=24,
+                       grad_x=dx.data_ptr(), grad_weight=dw.data_ptr(), grad_bias=db.data_ptr())
+    _native.run("nnue_ls_linear_backward", a, dw)
+    assert (dw == 0).all() and (db == 0).all() and dx.isnan().all()

@@ -84,9 +84,10 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
     output) are ``[..., width]`` in fp32, bf16 or fp16; ``norm`` is the
     ``"rms"`` or ``"layer"`` norm of a row.  ``gate`` is one value per row
     (``[...]`` or ``[..., 1]``, also in fp32), or elementwise (broadcast to
-    x's shape, in x's type); with ``gate_activation="sigmoid"`` it goes through
-    a sigmoid first.  ``residual_scale`` is a number or a learned ``[width]``
-    tensor.  The parameters share one type, x's or fp32.  Statistics and sums
+    x's shape, in x's type); a shape that says both, such as ``[n]`` beside
+    ``[n, n]``, is refused: give it as ``[n, 1]`` or ``[1, n]``.  With
+    ``gate_activation="sigmoid"`` the gate goes through a sigmoid first.
+    ``residual_scale`` is a number or a learned ``[width]`` tensor.  The parameters share one type, x's or fp32.  Statistics and sums
     are held in fp32, h is normalised from the unrounded y, and each output is
     rounded once.  Differentiable once, in every tensor argument.
     """
@@ -138,6 +139,10 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
     if gate is not None:
         if gate.shape == shape[:-1] or (gate.shape == shape[:-1] + (1,) and width > 1):
             mode = 1
+            if gate.shape == shape[:-1] and gate.numel() > 1 and \
+                    all(n in (1, to) for n, to in zip(gate.shape, shape[1:])):
+                raise ValueError(f"gate {tuple(gate.shape)} could be per row or per column of x {tuple(shape)}: give it "
+                                 f"as {tuple(gate.shape) + (1,)} or as {(1,) + tuple(gate.shape)}")
             check(gate, "gate", mixed, gpu)
             if gate.dim() != 1:
                 gate = gate.reshape(-1)

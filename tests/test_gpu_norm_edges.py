@@ -1,0 +1,48 @@
+"""block_norm where a gate's meaning, its sigmoid or a call's options are at a
+limit, against the formula in 64 bits."""
+
+import pytest
+import torch
+
+from stockfish_trainer_b200.layer_stacks import block_norm
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_gates_of_a_square_input(cuda, dt):
+    """As many rows as columns: a gate per row and one per column are told apart by their shape, or refused."""
+    n = 48
+    x, f = torch.randn(n, n, device=cuda).to(dt), torch.randn(n, n, device=cuda).to(dt)
+    g = torch.rand(n, device=cuda).to(dt)
+    with pytest.raises(ValueError, match="per row or per column"):
+        block_norm(x, f, gate=g)
+    for gate in (g[:, None], g[None, :]):
+        gg = gate.clone().requires_grad_()
+        y, _ = block_norm(x, f, gate=gg)
+        want = x.double() + gate.double() * f.double()
+        assert ((y.double() - want).abs() <= 2.0**-8 * want.abs() + 1e-6).all()
+        y.sum().backward()
+        dim = 1 if gate.shape[1] == 1 else 0
+        err = (gg.grad.double() - f.double().sum(dim, keepdim=True)).abs()
+        assert (err <= 2.0**-7 * f.double().abs().sum(dim, keepdim=True)).all()
+
+
+def test_gates_whose_shape_says_enough(cuda):
+    w = 5
+
+    def y(shape, gate):
+        x = torch.randn(shape, generator=torch.Generator().manual_seed(1)).cuda()
+        return block_norm(torch.zeros_like(x), x, gate=gate)[0] / x
+
+    g = torch.rand(w, device=cuda) + 0.5
+    for shape in ((w, w, w), (1, w, w), (1, 1, w, w)):
+        with pytest.raises(ValueError, match="per row or per column"):
+            y(shape, g.expand(shape[:-1]))
+        torch.testing.assert_close(y(shape, g.expand(shape[:-1]).unsqueeze(-1)), g[:, None].expand(shape))
+        torch.testing.assert_close(y(shape, g.expand(shape)), g.expand(shape))
+    torch.testing.assert_close(y((3, w, w), g), g.expand(3, w, w))  # fits the columns only
+    torch.testing.assert_close(y((w, 3, w), g[:, None].expand(w, 3)), g[:, None, None].expand(w, 3, w))  # the rows only
+    for shape in ((1, 1), (1, 7), (1, 1, 7)):  # one row, one gate: both readings say the same
+        one = torch.rand(shape[:-1], device=cuda) + 0.5
+        torch.testing.assert_close(y(shape, one), one.unsqueeze(-1).expand(shape))

@@ -8,6 +8,8 @@ and backward as hand-written kernels (include/nnue_ls.h):
 * ``route``       a router's top-k choice with per-expert counts and the balance
   loss.
 
+They are differentiable once, in reverse mode; forward mode is refused.
+
 ``RoutedLayerStacks`` puts them together.
 """
 

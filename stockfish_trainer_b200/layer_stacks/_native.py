@@ -11,6 +11,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import build as _build
@@ -157,6 +158,12 @@ def run(func: str, args: ctypes.Structure, like: torch.Tensor) -> None:
         rc = fn(ref, None if ws is None else ws.data_ptr(), nbytes, stream)
     if rc != OK:
         check(func, rc)
+
+
+def differentiates(grad: bool) -> bool:
+    """Whether a call has to go through its autograd function: a gradient may be asked for (``grad``: of some argument),
+    or forward-mode differentiation is on, which the functions refuse where an argument carries a tangent."""
+    return grad and torch.is_grad_enabled() or forward_ad._current_level >= 0
 
 
 def once(backward):

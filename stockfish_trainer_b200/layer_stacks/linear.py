@@ -133,7 +133,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         residual = _native.rows_of(residual)
         grad = grad or residual.requires_grad
     x, weight = _native.rows_of(x), _native.rows_of(weight)
-    if grad and torch.is_grad_enabled():
+    if _native.differentiates(grad):
         out = LinearActFunction.apply(x, weight, bias, residual, act)
     else:
         out = _forward(x, weight, bias, residual, act)

@@ -163,7 +163,7 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
     f2 = None if f is None else (f if flat else f.reshape(-1, width)).contiguous()
     meta = (_KINDS[kind], mode, gate_activation == "sigmoid", scale_value, float(eps),
             _native.DTYPES[params_dtype or dt], _native.DTYPES[dt if gate is None else gate.dtype])
-    if grad and torch.is_grad_enabled():
+    if _native.differentiates(grad):
         y, h = BlockNormFunction.apply(x2, f2, gate, *params, meta)
     else:
         y, h, _ = _forward(x2, f2, gate, params, meta, False)

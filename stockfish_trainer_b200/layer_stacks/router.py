@@ -101,7 +101,7 @@ def route(logits: torch.Tensor, k: int, *, valid: torch.Tensor | None = None, re
             raise ValueError(f"valid must have shape {tuple(shape)}, got {tuple(valid.shape)}")
         valid = valid.reshape(-1).contiguous()
     rows = _native.rows_of(logits)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _native.differentiates(logits.requires_grad):
         indices, gates, counts, loss = RouteFunction.apply(rows, valid, k, bool(renormalize))
     else:
         indices, gates, counts, loss = _forward(rows, valid, k, bool(renormalize))

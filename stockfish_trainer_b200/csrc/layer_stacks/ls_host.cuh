@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../../include/nnue_ls.h"
 #include "ls_common.cuh"
 
@@ -29,6 +31,20 @@ inline int check_workspace(const char* what, const void* ws, size_t have, size_t
     return fail(NNUE_LS_ERR_WORKSPACE, "%s: workspace has %zu bytes, needs %zu", what, ws ? have : (size_t)0, need);
   if (reinterpret_cast<uintptr_t>(ws) % 256)
     return fail(NNUE_LS_ERR_WORKSPACE, "%s: workspace not 256-byte aligned", what);
+  return NNUE_LS_OK;
+}
+
+// Allows `kernel` up to `most` bytes of dynamic shared memory, once per device: the limit is the kernel's on that device,
+// whoever calls it, so no call may set it to its own need.
+template <auto kernel>
+int allow_shared(const char* what, size_t most) {
+  static std::atomic<uint64_t> ready{0};  // one bit per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return check_launch(what);
+  if (dev < 64 && ready.load(std::memory_order_acquire) >> dev & 1) return NNUE_LS_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
   return NNUE_LS_OK;
 }
 

@@ -129,15 +129,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t K, int planes) {
 template <typename T, int CG>
 int launch_gemm_cg(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, cudaStream_t s) {
   using S = GemmShape<sizeof(T) == 4 ? 3 : 1, CG>;
-  static std::atomic<uint64_t> ready{0};  // one bit per device: the kernel may use S::kSmem there
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("gemm");
-  if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(gemm_kernel<T, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "gemm: %s", cudaGetErrorString(e));
-    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
-  }
+  if (int rc = allow_shared<gemm_kernel<T, CG>>("gemm", S::kSmem)) return rc;
   const int64_t items = (int64_t)p.m_tiles * p.n_tiles * p.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(items, kNumSMs / CG) * CG));

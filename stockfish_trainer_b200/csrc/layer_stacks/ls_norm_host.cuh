@@ -63,11 +63,12 @@ struct RowPlan {
   bool vec;
   int threads;  // 0: any width
 };
+constexpr int kMostRowThreads = 512;
 
 template <typename T>
 RowPlan plan_norm(const nnue_ls_norm& a) {
   const int64_t threads = ceil_div(a.width, 32 * kColumns) * 32;
-  return RowPlan{norm_vectors<T>(a), threads <= 512 ? (int)threads : 0};
+  return RowPlan{norm_vectors<T>(a), threads <= kMostRowThreads ? (int)threads : 0};
 }
 
 // Rows at a time and rounds in flight: the slots of an SM's THREADS take at most
@@ -80,10 +81,11 @@ struct RowShape {
   static constexpr int kFit = 220 * 1024 / (kSlot * THREADS);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;
   static_assert(kStages >= 2, "a round on its way while one is worked on");
-  static size_t ring_bytes(const RowPlan& r, int width) {
+  static constexpr size_t ring_bytes(int threads, int width) {
     const int arrays = 2 + FULL + 2 * BACKWARD;
-    return (size_t)kStages * (V > 1 ? kSlot * r.threads : arrays * run_bytes(kRows, width, (int)sizeof(T)));
+    return (size_t)kStages * (V > 1 ? kSlot * threads : arrays * run_bytes(kRows, width, (int)sizeof(T)));
   }
+  static constexpr size_t kMostBytes = ring_bytes(kMostRowThreads, kMostRowThreads * kColumns);
 };
 
 // As many blocks of `rows` rows as stay on the SMs together at `threads` each, looping over rows.
@@ -96,12 +98,11 @@ int64_t norm_backward_blocks(const nnue_ls_norm& a, const RowPlan& r) {
   return norm_row_blocks(a, r, 1, norm_backward_threads(4, true, false));
 }
 
-template <typename K>
-int launch_norm_rows(K kernel, int64_t grid, const RowPlan& r, size_t smem, const NormParams& p, cudaStream_t s) {
-  if (smem > 40 * 1024) {  // 48 KB without asking, the kernels' own 3 KB at most included
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return fail(NNUE_LS_ERR_CUDA, "norm: %s", cudaGetErrorString(e));
-  }
+template <auto kernel, typename Shape>
+int launch_norm_rows(int64_t grid, const RowPlan& r, const NormParams& p, cudaStream_t s) {
+  const size_t smem = Shape::ring_bytes(r.threads, p.width);
+  if (smem > 40 * 1024)  // 48 KB without asking, the kernels' own 3 KB at most included
+    if (int rc = allow_shared<kernel>("norm", Shape::kMostBytes)) return rc;
   kernel<<<(unsigned)grid, r.threads, smem, s>>>(p);
   return NNUE_LS_OK;
 }
@@ -142,8 +143,8 @@ int norm_forward(const nnue_ls_norm& a, cudaStream_t s) {
       constexpr int V = decltype(vec)::value;
       constexpr int kThreads = norm_forward_threads(V, B, M);
       using H = RowShape<T, V, F, false, kThreads>;
-      return launch_norm_rows(norm_forward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>,
-                              norm_row_blocks(a, r, H::kRows, kThreads), r, H::ring_bytes(r, a.width), p, s);
+      return launch_norm_rows<norm_forward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>, H>(
+          norm_row_blocks(a, r, H::kRows, kThreads), r, p, s);
     };
     return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
   });
@@ -176,8 +177,7 @@ int norm_backward(const nnue_ls_norm& a, void* workspace, cudaStream_t s) {
         constexpr int kThreads = norm_backward_threads(V, B, M);
         using H = RowShape<T, V, F, true, kThreads>;
         grid = norm_row_blocks(a, r, H::kRows, kThreads);
-        return launch_norm_rows(norm_backward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>, grid, r,
-                                H::ring_bytes(r, a.width), p, s);
+        return launch_norm_rows<norm_backward_rows_kernel<T, V, H::kRows, C, F, B, M, H::kStages>, H>(grid, r, p, s);
       };
       return r.vec ? launch(std::integral_constant<int, 16 / sizeof(T)>{}) : launch(std::integral_constant<int, 1>{});
     });

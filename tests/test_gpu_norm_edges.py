@@ -1,6 +1,8 @@
 """block_norm where a gate's meaning, its sigmoid or a call's options are at a
 limit, against the formula in 64 bits."""
 
+import threading
+
 import pytest
 import torch
 
@@ -46,3 +48,27 @@ def test_gates_whose_shape_says_enough(cuda):
     for shape in ((1, 1), (1, 7), (1, 1, 7)):  # one row, one gate: both readings say the same
         one = torch.rand(shape[:-1], device=cuda) + 0.5
         torch.testing.assert_close(y(shape, one), one.unsqueeze(-1).expand(shape))
+
+
+def test_threads_with_rows_of_different_widths(cuda):
+    """One kernel asked for different amounts of shared memory by two threads at once."""
+    errors = []
+
+    def work(width):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                x = torch.randn(8, width, device=cuda)
+                w = torch.ones(width, device=cuda)
+                want = block_norm(x, x, post_weight=w, pre_weight=w)
+                for _ in range(3000):
+                    got = block_norm(x, x, post_weight=w, pre_weight=w)
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(width,)) for width in (4096, 2048, 4096, 1800)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

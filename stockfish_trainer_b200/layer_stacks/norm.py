@@ -137,13 +137,14 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
     flat = len(shape) == 2
     mode = 0
     if gate is not None:
-        if gate.shape == shape[:-1] or (gate.shape == shape[:-1] + (1,) and width > 1):
+        check(gate, "gate", mixed, gpu)
+        gate_shape, lead = gate.shape, shape[:-1]
+        if gate_shape == lead or (gate_shape == lead + (1,) and width > 1):
             mode = 1
-            if gate.shape == shape[:-1] and gate.numel() > 1 and \
-                    all(n in (1, to) for n, to in zip(gate.shape, shape[1:])):
-                raise ValueError(f"gate {tuple(gate.shape)} could be per row or per column of x {tuple(shape)}: give it "
-                                 f"as {tuple(gate.shape) + (1,)} or as {(1,) + tuple(gate.shape)}")
-            check(gate, "gate", mixed, gpu)
+            if len(gate_shape) == len(lead) and gate.numel() > 1 and \
+                    all(n in (1, to) for n, to in zip(gate_shape, shape[1:])):
+                raise ValueError(f"gate {tuple(gate_shape)} could be per row or per column of x {tuple(shape)}: give it "
+                                 f"as {tuple(gate_shape) + (1,)} or as {(1,) + tuple(gate_shape)}")
             if gate.dim() != 1:
                 gate = gate.reshape(-1)
         else:

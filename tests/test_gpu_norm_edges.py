@@ -72,3 +72,15 @@ def test_threads_with_rows_of_different_widths(cuda):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+def test_a_gate_that_is_no_tensor_is_refused(cuda):
+    x = torch.zeros(4, 8, device=cuda)
+    for gate in (0.5, [1.0] * 4, torch.zeros(4)):
+        with pytest.raises(TypeError if not torch.is_tensor(gate) else ValueError, match="gate"):
+            block_norm(x, x, gate=gate)
+    for gate in (torch.zeros(4, dtype=torch.float64, device=cuda), torch.zeros(8, dtype=torch.int64, device=cuda)):
+        with pytest.raises(TypeError, match="gate"):
+            block_norm(x, x, gate=gate)
+    with pytest.raises(TypeError, match="gate"):  # an elementwise gate has x's type
+        block_norm(x.bfloat16(), x.bfloat16(), gate=x)

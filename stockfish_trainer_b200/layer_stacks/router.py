@@ -6,6 +6,7 @@ moe_stacks.py:12-283)."""
 
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple
 
 import torch
@@ -91,7 +92,7 @@ def route(logits: torch.Tensor, k: int, *, valid: torch.Tensor | None = None, re
     if len(shape) < 1 or not 1 <= shape[-1] <= _native.MAX_EXPERTS:
         raise ValueError(f"logits must be [..., experts] with 1 <= experts <= {_native.MAX_EXPERTS}, "
                          f"got {tuple(shape)}")
-    k = int(k)
+    k = operator.index(k)
     if not 1 <= k <= shape[-1]:
         raise ValueError(f"k must be in [1, {shape[-1]}], got {k}")
     shape = shape[:-1]

@@ -26,3 +26,11 @@ def test_forward_mode_is_refused(cuda, call):
         assert torch.equal(call(x), call(x.clone()))  # nothing dual: an ordinary call
     with pytest.raises(RuntimeError):
         torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
+def test_a_number_of_choices_that_is_not_whole_is_refused(cuda):
+    x = torch.randn(4, 8, device=cuda)
+    for k in (2.5, 2.0, "2", None):
+        with pytest.raises(TypeError):
+            route(x, k)
+    assert route(x, True).indices.shape == (4, 1)

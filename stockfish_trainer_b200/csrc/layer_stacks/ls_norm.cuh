@@ -654,8 +654,8 @@ __global__ void __launch_bounds__(norm_forward_threads(V, BOTH, MORE), 1) norm_f
 #pragma unroll
           for (int k = 0; k < N; ++k) y[r][k] = fmaf((CENTER ? v[k] - mean_f[r] : v[k]) * gr, w[k], sc[k] * y[r][k]);
         }
-        if (row0 + r < rows) C::store(p.y, row0 + r, W, y[r]);
       }
+      if ((BOTH || p.y) && row0 + r < rows) C::store(p.y, row0 + r, W, y[r]);  // without f it may be wanted too
     }
     if (pre) {
       if (CENTER) {

@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from stockfish_trainer_b200.layer_stacks import block_norm
+from stockfish_trainer_b200.layer_stacks import _native, block_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,22 @@ def test_a_gate_that_is_no_tensor_is_refused(cuda):
             block_norm(x, x, gate=gate)
     with pytest.raises(TypeError, match="gate"):  # an elementwise gate has x's type
         block_norm(x.bfloat16(), x.bfloat16(), gate=x)
+
+
+def _struct(x, **kw):
+    return _native.Norm(rows=x.shape[0], width=x.shape[1], dtype=_native.DTYPES[x.dtype], x=x.data_ptr(), eps=1e-5, **kw)
+
+
+@pytest.mark.parametrize("width", [64, 61, 1040, 5000])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_c_forward_writes_y_without_a_block(cuda, dt, width):
+    """Without f y is x, written where it is asked for."""
+    x = torch.randn(9, width, device=cuda).to(dt)
+    w = torch.ones(width, device=cuda)
+    y, h, h2 = (torch.full_like(x, float("nan")) for _ in range(3))
+    _native.run("nnue_ls_norm_forward", _struct(x, pre_weight=w.data_ptr(), y=y.data_ptr(), h=h.data_ptr()), x)
+    _native.run("nnue_ls_norm_forward", _struct(x, pre_weight=w.data_ptr(), h=h2.data_ptr()), x)
+    assert torch.equal(y, x) and torch.equal(h, h2) and torch.equal(h, block_norm(x, pre_weight=w)[1])
+    y.fill_(0)
+    _native.run("nnue_ls_norm_forward", _struct(x, y=y.data_ptr()), x)
+    assert torch.equal(y, x)

@@ -31,7 +31,7 @@ NormParams norm_params(const nnue_ls_norm& a) {
   p.grad_gate = a.grad_gate;
   p.rows = a.rows;
   p.width = a.width;
-  p.scale_value = a.scale_value;
+  p.scale_value = a.f ? a.scale_value : 1.f;  // without a block y is x
   p.eps = a.eps;
   p.gate_mode = a.gate_mode;
   p.gate_sigmoid = a.gate_sigmoid != 0;

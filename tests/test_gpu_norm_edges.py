@@ -103,3 +103,21 @@ def test_c_forward_writes_y_without_a_block(cuda, dt, width):
     y.fill_(0)
     _native.run("nnue_ls_norm_forward", _struct(x, y=y.data_ptr()), x)
     assert torch.equal(y, x)
+
+
+@pytest.mark.parametrize("width", [64, 61, 1040, 5000])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_c_backward_without_a_block_takes_no_scale(cuda, dt, width):
+    """scale_value, 0 in a zeroed struct, belongs to the block: the results are those of the Python call."""
+    x = torch.randn(9, width, device=cuda).to(dt).requires_grad_()
+    gh = torch.randn(9, width, device=cuda).to(dt)
+    w = torch.ones(width, device=cuda)
+    want, = torch.autograd.grad(block_norm(x, pre_weight=w)[1], [x], gh)
+    for scale in (0.0, 1.0, 3.0):
+        h, dx = torch.empty_like(x), torch.full_like(x, float("nan"))
+        stats = torch.empty(9, 4, device=cuda)
+        a = _struct(x, pre_weight=w.data_ptr(), h=h.data_ptr(), stats=stats.data_ptr(), scale_value=scale)
+        _native.run("nnue_ls_norm_forward", a, x)
+        a.grad_h, a.grad_x = gh.data_ptr(), dx.data_ptr()
+        _native.run("nnue_ls_norm_backward", a, x)
+        assert torch.equal(dx, want), scale

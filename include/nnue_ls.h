@@ -16,7 +16,8 @@
  *     operands below 2^-110 are held to 2^-134 instead of 24 bits).  Results do
  *     not depend on scheduling: no sum is formed with floating-point atomics.
  *   - Matrices are row-major with unit column stride; ld* is the row stride in
- *     elements.  Row counts may be 0 (then nothing is read).
+ *     elements.  Row counts may be 0 (then nothing is read).  Pointers are
+ *     aligned to their elements, or to more where the field says so.
  *   - Return value: NNUE_LS_OK or a negative NNUE_LS_ERR_* code; no exceptions
  *     cross this boundary.  nnue_ls_last_error() describes the last failure on
  *     the calling thread.
@@ -122,7 +123,7 @@ typedef struct {
   const void *x, *f, *gate;
   const void *post_weight, *post_bias, *scale, *pre_weight, *pre_bias;
   void *y, *h;  /* forward */
-  float *stats; /* [rows, 4]: written by the forward when not null, read by the backward */
+  float *stats; /* [rows, 4], 16-byte aligned: written by the forward when not null, read by the backward */
   const void *grad_y, *grad_h; /* backward; null = zero */
   void *grad_x, *grad_f, *grad_gate; /* null = not wanted */
   void *grad_post_weight, *grad_post_bias, *grad_scale, *grad_pre_weight, *grad_pre_bias;

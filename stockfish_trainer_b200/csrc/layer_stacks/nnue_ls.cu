@@ -10,6 +10,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../../include/nnue_ls.h"
 #include "ls_common.cuh"
@@ -37,6 +38,14 @@ int check_launch(const char* what) {
 
 namespace {
 
+// Whether some pointer (null is fine) is not on a multiple of `to` bytes: a power of two.
+bool off_boundary(size_t to, std::initializer_list<const void*> pointers) {
+  uintptr_t all = 0;
+  for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & (to - 1)) != 0;
+}
+size_t bytes_of(int dtype) { return dtype == NNUE_LS_F32 ? 4 : 2; }
+
 // ---- linear ----------------------------------------------------------------
 int check_linear(const char* what, const nnue_ls_linear* a) {
   if (!a) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
@@ -48,6 +57,12 @@ int check_linear(const char* what, const nnue_ls_linear* a) {
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: bad element type", what);
   if (a->activation < 0 || a->activation > NNUE_LS_ACT_GELU)
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, a->activation);
+  if (off_boundary(bytes_of(a->dtype), {a->x, a->weight, a->residual, a->out, a->act_grad, a->grad_out, a->grad_x,
+                                        a->grad_weight}) ||
+      off_boundary(bytes_of(a->bias_dtype), {a->bias, a->grad_bias}))
+    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  if (off_boundary(256, {a->x_packed, a->weight_packed}))
+    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: x_packed or weight_packed not 256-byte aligned", what);
   return NNUE_LS_OK;
 }
 
@@ -71,6 +86,14 @@ int check_norm(const char* what, const nnue_ls_norm* a) {
   if (!(a->eps >= 0.f)) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", what);
   if (a->rows > 0 && (!a->x || (a->gate_mode != NNUE_LS_GATE_NONE && !a->gate)))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  const bool row_gate = a->gate_mode == NNUE_LS_GATE_ROW;
+  if (off_boundary(bytes_of(a->dtype), {a->x, a->f, a->y, a->h, a->grad_y, a->grad_h, a->grad_x, a->grad_f}) ||
+      off_boundary(bytes_of(row_gate ? a->gate_dtype : a->dtype), {a->gate, a->grad_gate}) ||
+      off_boundary(bytes_of(a->params_dtype),
+                   {a->post_weight, a->post_bias, a->scale, a->pre_weight, a->pre_bias, a->grad_post_weight,
+                    a->grad_post_bias, a->grad_scale, a->grad_pre_weight, a->grad_pre_bias}))
+    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
+  if (off_boundary(16, {a->stats})) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: stats not 16-byte aligned", what);
   return NNUE_LS_OK;
 }
 
@@ -85,6 +108,9 @@ int check_route(const char* what, const nnue_ls_route* a) {
   if (a->rows > 0 && (!a->logits || a->ld < a->experts || !a->indices || !a->gates))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: null pointer or row stride below experts", what);
   if (!a->counts || !a->loss) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (off_boundary(bytes_of(a->dtype), {a->logits, a->grad_logits}) || off_boundary(8, {a->indices, a->counts}) ||
+      off_boundary(4, {a->gates, a->loss, a->grad_gates, a->grad_loss}))
+    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "%s: a pointer is not aligned to its elements", what);
   return NNUE_LS_OK;
 }
 
@@ -142,8 +168,6 @@ int nnue_ls_linear_forward(const nnue_ls_linear* a, void* workspace, size_t work
   if (!a->x || !a->weight || !a->out) return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: null pointer");
   if (a->ldx < a->inputs || a->ldw < a->inputs || (a->residual && a->ldr < a->outputs))
     return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: row stride below the row length");
-  if ((reinterpret_cast<uintptr_t>(a->x_packed) | reinterpret_cast<uintptr_t>(a->weight_packed)) % 256)
-    return fail(NNUE_LS_ERR_INVALID_ARGUMENT, "linear_forward: x_packed or weight_packed not 256-byte aligned");
   return with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
     if ((a->x_packed && !linear_packed_bytes<T>(*a, false)) || (a->weight_packed && !linear_packed_bytes<T>(*a, true)))

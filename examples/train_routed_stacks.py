@@ -39,7 +39,8 @@ def train(steps: int = 50, batch: int = 4096, dtype: torch.dtype = torch.float32
     table = torch.nn.Parameter(torch.randn(rows, L1 + N_PSQT, device=dev) * 0.05)
     bias = torch.nn.Parameter(torch.full((L1 + N_PSQT,), 0.3, device=dev))
     net = RoutedLayerStacks(l1=L1, width=64, hidden=128, blocks=2, stacks=8, k=2).to(dev, dtype)
-    opt = torch.optim.Adam([table, bias, *net.parameters()], lr=3e-3)
+    # a row of the table is met by few positions and has to move fast; the network, at its rate, would swing
+    opt = torch.optim.Adam([{"params": [table, bias], "lr": 1e-2}, {"params": net.parameters(), "lr": 1e-3}])
     losses = []
     for step in range(steps):
         board_np, _ = positions.generate_positions(batch, seed=seed + 1 + step)

@@ -63,6 +63,16 @@ __device__ __forceinline__ void store_mixed(void* p, int64_t i, bool is_f32, flo
   else static_cast<T*>(p)[i] = from_f<T>(v);
 }
 
+// 1 / (1 + exp(-v)) to about three units at any v: with e = exp(-|v|) the sum lies in [1, 2], where the short reciprocal
+// (one unit) needs neither a division's slow path nor care for subnormal results.  fp32 65536 x 1040, elementwise gate,
+// layer norm forward: 260 us; with a division 305, with the short exponential, whose error grows with |v|, 246.
+__device__ __forceinline__ float logistic(float v) {
+  float r;
+  const float e = expf(-fabsf(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return v < 0.f ? e * r : r;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);

@@ -19,7 +19,8 @@ enum Activation : int { kNone = 0, kRelu = 1, kCrelu = 2, kSqrCrelu = 3, kSilu =
 // against exp(u^2) erfc(u) on u in [0, 14] is least (a linear program over its
 // coefficients; 9.5e-6), so the lower tail keeps its digits too.  The
 // exponential is the density's, needed for the derivative anyway.  fp32 results
-// take erfcf.
+// take erfcf and logistic: the short exponential's error grows with |z| (25 units
+// at z = -20).
 // The hardware's own reciprocal and power of two (2^-22 relative, subnormals
 // flushed), for 16-bit results.
 __device__ __forceinline__ float short_rcp(float v) {
@@ -45,7 +46,7 @@ __device__ __forceinline__ float activate(float z, float& d) {
     d = inside ? (ACT == kCrelu ? 1.f : 2.f * z) : 0.f;
     return ACT == kCrelu ? c : c * c;
   } else if constexpr (ACT == kSilu) {
-    const float s = kShort ? short_rcp(1.f + short_exp2(-1.44269504f * z)) : __fdividef(1.f, 1.f + __expf(-z));
+    const float s = kShort ? short_rcp(1.f + short_exp2(-1.44269504f * z)) : logistic(z);
     d = s * (1.f + z * (1.f - s));
     return z * s;
   } else if constexpr (ACT == kGelu) {

@@ -28,7 +28,12 @@ struct NormParams {
   bool gate_sigmoid, gate_f32, params_f32;
 };
 
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// As an elementwise gate of T; a gate per row is always taken as fp32's.  The short
+// exponential's error grows with |v| (25 units of fp32 at v = -20), which 16-bit results do not show.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float v) {
+  return sizeof(T) == 2 ? __fdividef(1.f, 1.f + __expf(-v)) : logistic(v);
+}
 
 // 1 / sqrt(v) to about one unit: the hardware's estimate and a Newton step.
 __device__ __forceinline__ float inv_sqrt(float v) {
@@ -49,7 +54,7 @@ struct NormRow {
     row_gate = 1.f;
     if (p.gate_mode == kGateRow) {
       row_gate = load_mixed<T>(p.gate, row, p.gate_f32);
-      if (p.gate_sigmoid) row_gate = sigmoid(row_gate);
+      if (p.gate_sigmoid) row_gate = logistic(row_gate);
     }
   }
   __device__ float param(const void* v, int c) const { return load_mixed<T>(v, c, p.params_f32); }
@@ -57,7 +62,7 @@ struct NormRow {
   __device__ float gate(int c) const {
     if (p.gate_mode != kGateFull) return row_gate;
     const float v = to_f(g[c]);
-    return p.gate_sigmoid ? sigmoid(v) : v;
+    return p.gate_sigmoid ? sigmoid<T>(v) : v;
   }
   __device__ float f_hat(int c) const { return (to_f(f[c]) - mean_f) * rstd_f; }
   __device__ float branch(int c) const {
@@ -529,14 +534,14 @@ struct RowRing {
 };
 
 // The gate of a row's columns.
-template <bool FULL, typename Ring>
+template <typename T, bool FULL, typename Ring>
 __device__ __forceinline__ void gates(const NormParams& p, const Ring& ring, int r, float row_gate,
                                       float (&g)[kColumns]) {
   if constexpr (FULL) {
     ring.template get<kGate>(r, g);
     if (p.gate_sigmoid) {
 #pragma unroll
-      for (int k = 0; k < kColumns; ++k) g[k] = sigmoid(g[k]);
+      for (int k = 0; k < kColumns; ++k) g[k] = sigmoid<T>(g[k]);
     }
   } else {
 #pragma unroll
@@ -556,7 +561,7 @@ template <typename T>
 __device__ __forceinline__ float load_row_gate(const NormParams& p, int row) {
   if (p.gate_mode != kGateRow) return 1.f;
   const float g = load_mixed<T>(p.gate, row, p.gate_f32);
-  return p.gate_sigmoid ? sigmoid(g) : g;
+  return p.gate_sigmoid ? logistic(g) : g;
 }
 
 // The forward's calls without biases or a learned scale fit 64 registers, so
@@ -645,7 +650,7 @@ __global__ void __launch_bounds__(norm_forward_threads(V, BOTH, MORE), 1) norm_f
         ring.template get<kF>(r, v);
         if (FULL || MORE) {
           float g[N];
-          gates<FULL>(p, ring, r, gate[r], g);
+          gates<T, FULL>(p, ring, r, gate[r], g);
 #pragma unroll
           for (int k = 0; k < N; ++k)
             y[r][k] = fmaf(g[k], fmaf((CENTER ? v[k] - mean_f[r] : v[k]) * rstd_f[r], w[k], b[k]), sc[k] * y[r][k]);
@@ -742,11 +747,11 @@ __global__ void __launch_bounds__(norm_backward_threads(V, BOTH, MORE), 1) norm_
 #pragma unroll
         for (int k = 0; k < N; ++k) g[k] = gates_of_row[k];
       } else {
-        gates<FULL>(p, ring, r, gate[r], g);
+        gates<T, FULL>(p, ring, r, gate[r], g);
       }
     };
     if constexpr (FULL && R == 1) {
-      if (has_f) gates<FULL>(p, ring, 0, 1.f, gates_of_row);
+      if (has_f) gates<T, FULL>(p, ring, 0, 1.f, gates_of_row);
     }
     if (pre) {
 #pragma unroll

@@ -1,6 +1,8 @@
 """linear_act where its formula, its fp32 planes or its rounding are at a limit,
 against the formula in 64 bits."""
 
+import math
+
 import pytest
 import torch
 
@@ -100,3 +102,27 @@ def test_c_backward_of_no_rows(cuda, dt):
                        grad_x=dx.data_ptr(), grad_weight=dw.data_ptr(), grad_bias=db.data_ptr())
     _native.run("nnue_ls_linear_backward", a, dw)
     assert (dw == 0).all() and (db == 0).all() and dx.isnan().all()
+
+
+@pytest.mark.parametrize("rows", [6, 60])
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_lower_tails_in_relative_terms(cuda, dt, rows):
+    """silu and gelu far below 0, where nothing absolute would show an error.  fp32 silu: an exponential of two units,
+    a sum, a division and a product.  fp32 gelu: erfc's argument is rounded, which its slope multiplies by z^2.  16-bit
+    results: their own rounding, and 2^-14 for the short exponential (fp16: half its smallest step besides)."""
+    u = UNIT[dt]
+    for act, values in (("silu", [-5.0, -20.0, -33.0, -47.0, -60.0, -80.0]),
+                        ("gelu", [-2.0, -4.0, -6.0, -8.0, -10.0, -12.0])):
+        z = torch.tensor(values, device=cuda, dtype=dt).repeat(rows // 6)
+        x = z[:, None].clone().requires_grad_()
+        out = linear_act(x, torch.ones(1, 1, device=cuda, dtype=dt), activation=act)
+        out.sum().backward()
+        ref = z.double().requires_grad_()
+        want = ref * torch.sigmoid(ref) if act == "silu" else ref * 0.5 * torch.special.erfc(-ref * math.sqrt(0.5))
+        want.sum().backward()
+        rel = 2 * u + 2.0**-14 if dt != torch.float32 else 8 * u if act == "silu" else (16 + 2 * z.double()**2) * u
+        err = (out.flatten().double() - want.detach()).abs()
+        assert (err <= rel * want.detach().abs() + (2.0**-25 if dt == torch.float16 else 0)).all(), (act, err / want.abs())
+        if dt == torch.float32:
+            err = (x.grad.flatten().double() - ref.grad).abs()
+            assert (err <= 2 * rel * ref.grad.abs()).all(), (act, err / ref.grad.abs())

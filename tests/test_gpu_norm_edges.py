@@ -121,3 +121,21 @@ def test_c_backward_without_a_block_takes_no_scale(cuda, dt, width):
         a.grad_h, a.grad_x = gh.data_ptr(), dx.data_ptr()
         _native.run("nnue_ls_norm_backward", a, x)
         assert torch.equal(dx, want), scale
+
+
+@pytest.mark.parametrize("gate", ["row", "full"])
+@pytest.mark.parametrize("width", [64, 61, 5000])
+def test_sigmoid_gates_far_below_zero(cuda, width, gate):
+    """y = sigmoid(g) f with f alone, in relative terms: an exponential of two units, a sum, a division and two
+    products; twice that for the gate's gradient (a row's is a sum of width terms of one sign)."""
+    values = torch.tensor([-1.0, -10.0, -20.0, -33.0, -47.0, -60.0, -80.0], device=cuda)
+    f = torch.rand(7, width, device=cuda) + 0.5
+    g = (values if gate == "row" else values[:, None].expand(7, width)).clone().requires_grad_()
+    y, _ = block_norm(torch.zeros_like(f), f, gate=g, gate_activation="sigmoid")
+    s = torch.sigmoid(values.double())[:, None]
+    assert ((y.double() - s * f.double()).abs() <= 4 * 2.0**-23 * s * f.double()).all()
+    y.sum().backward()
+    want = s * torch.sigmoid(-values.double())[:, None] * f.double()
+    if gate == "row":
+        want = want.sum(1)
+    assert ((g.grad.double() - want).abs() <= 16 * 2.0**-23 * want).all(), float(((g.grad.double() - want).abs() / want).max())

@@ -112,6 +112,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
+// The same for a whole warp, whose lanes could run out on either side of the phase's end: they go on together or give
+// up together, as the collective reads of TMEM that follow need.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  return __all_sync(kFull, mbar_wait(bar, parity, gave_up));
+}
+
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -369,7 +375,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       if constexpr (S::kChunk == 0) {
         const uint32_t acc = chunk % S::kAccs;
-        if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
+        if (!(ok = mbar_wait_warp(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
         tcgen_fence_after();
         for (int cb = group; cb < col_blocks; cb += kColumnGroups) {
           const int64_t n = n0 + cb * 32;
@@ -405,7 +411,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                   k1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
         for (int kc = k0; kc < k1; kc += S::kChunk, ++chunk) {
           const uint32_t acc = chunk % S::kAccs;
-          if (!(ok = mbar_wait(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
+          if (!(ok = mbar_wait_warp(acc_full0 + 8 * acc, (chunk / S::kAccs) & 1, gave_up))) break;
           tcgen_fence_after();
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {

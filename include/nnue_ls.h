@@ -43,7 +43,7 @@ extern "C" {
 #define NNUE_LS_F16 2
 
 /* Device error flags (nnue_ls_device_errors). */
-#define NNUE_LS_DEVERR_WAIT_TIMEOUT 1u /* a matrix kernel's wait ran out: its results are incomplete */
+#define NNUE_LS_DEVERR_WAIT_TIMEOUT 1u /* a matrix kernel's wait ran out: what it had not formed by then is NaN */
 #define NNUE_LS_DEVERR_BAD_INDEX 2u    /* route backward: a chosen index outside [-1, experts) was skipped */
 
 int nnue_ls_version(void);
@@ -53,6 +53,13 @@ uint64_t nnue_ls_launch_count(void);
 /* Reads (and with clear != 0 resets) the sticky device error flags of the
  * current device.  Synchronises the device. */
 int nnue_ls_device_errors(uint32_t *flags, int clear);
+/* How long a matrix kernel launched from now on (by any thread) waits for its
+ * own copies and products, which take microseconds, before it gives up: raises
+ * the flag, stores NaN for what it has not formed and returns.  4 s at first;
+ * more where the GPU may be taken away from the process for longer, 0 to see
+ * what giving up looks like (no wait is made and no product formed).  Returns
+ * the limit so far. */
+uint64_t nnue_ls_set_wait_limit(uint64_t ns);
 
 /* ---- fused linear layer --------------------------------------------------
  *   z = x W^T + bias;  out = act(z) + residual

@@ -13,6 +13,7 @@ namespace nnue_ls {
 
 // One per library (nnue_ls.cu).
 void count_launch();
+uint64_t wait_limit_ns();  // of a matrix kernel's waits
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int check_launch(const char* what);  // the last launch's error, if any
 

@@ -172,6 +172,8 @@ int launch_gemm(const Operand& a, const Operand& b, int64_t M, int64_t N, const 
   p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn_major << 15 | (uint32_t)b.mn_major << 16 |
             (uint32_t)(t.bn / 8) << 17 | (uint32_t)(kTileM * t.cg / 16) << 24;
   p.partial = static_cast<float*>(partial);
+  p.wait_limit_ns = wait_limit_ns();
+  p.items = p.wait_limit_ns ? t.m_tiles * t.n_tiles * t.splits : 0;
   constexpr int64_t V = 16 / sizeof(T);
   auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   e.vec = N % V == 0 && aligned(e.out) && aligned(e.act_grad) && aligned(e.residual) && (!e.residual || e.ldr % V == 0);

@@ -20,8 +20,10 @@ namespace nnue_ls {
 
 static thread_local char g_last_error[512];
 static std::atomic<unsigned long long> g_launches{0};
+static std::atomic<uint64_t> g_wait_limit_ns{4000000000ull};
 
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+uint64_t wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -137,6 +139,8 @@ int nnue_ls_device_errors(uint32_t* flags, int clear) {
   if (e == cudaSuccess) e = route_device_errors(flags, clear != 0);
   return e == cudaSuccess ? NNUE_LS_OK : fail(NNUE_LS_ERR_CUDA, "device_errors: %s", cudaGetErrorString(e));
 }
+
+uint64_t nnue_ls_set_wait_limit(uint64_t ns) { return g_wait_limit_ns.exchange(ns); }
 
 size_t nnue_ls_linear_saved_layout(const nnue_ls_linear* a, int32_t parts, int64_t offsets[3]) {
   if (!offsets) return 0;

@@ -62,6 +62,7 @@ _SIGNATURES = {
     "nnue_ls_last_error": (ctypes.c_char_p, []),
     "nnue_ls_launch_count": (_U64, []),
     "nnue_ls_device_errors": (_I32, [ctypes.POINTER(ctypes.c_uint32), _I32]),
+    "nnue_ls_set_wait_limit": (_U64, [_U64]),
     "nnue_ls_linear_saved_layout": (_SZ, [ctypes.POINTER(Linear), _I32, ctypes.POINTER(_I64)]),
     "nnue_ls_linear_forward_workspace_size": (_SZ, [ctypes.POINTER(Linear)]),
     "nnue_ls_linear_forward": (_I32, [ctypes.POINTER(Linear), _P, _SZ, _P]),
@@ -122,6 +123,14 @@ def device_errors(clear: bool = True) -> int:
     flags = ctypes.c_uint32(0)
     check("nnue_ls_device_errors", load().nnue_ls_device_errors(ctypes.byref(flags), int(clear)))
     return int(flags.value)
+
+
+def set_wait_limit(seconds: float) -> float:
+    """How long a matrix kernel waits for its own copies and products before it gives up, raises DEVERR_WAIT_TIMEOUT and
+    leaves NaN in what it has not formed (4 s at first; 0: at once).  Returns the limit so far."""
+    if not 0 <= seconds < 2**34:
+        raise ValueError(f"seconds must be in [0, 2^34), got {seconds}")
+    return load().nnue_ls_set_wait_limit(round(seconds * 1e9)) / 1e9
 
 
 def check(func: str, rc: int) -> None:

@@ -100,6 +100,10 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     For the backward ``x`` and ``weight`` (in the form their products read: for
     fp32 1.5 times their size) and the activation's derivative (as wide as the
     output) are kept; it is differentiable once.
+
+    Should the GPU stop for longer than a product may wait for its own copies
+    (4 s), what it had not formed by then is NaN, and ``device_errors()`` of
+    ``layer_stacks._native`` tells it from other NaNs.
     """
     act = _ACT.get(activation)
     if act is None:

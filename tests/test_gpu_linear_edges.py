@@ -126,3 +126,60 @@ def test_lower_tails_in_relative_terms(cuda, dt, rows):
         if dt == torch.float32:
             err = (x.grad.flatten().double() - ref.grad).abs()
             assert (err <= 2 * rel * ref.grad.abs()).all(), (act, err / ref.grad.abs())
+
+
+@pytest.fixture
+def no_waiting(cuda):
+    """Matrix kernels give up at once inside this: calls `on`, then `off`."""
+    torch.cuda.synchronize()
+    assert _native.device_errors(clear=True) == 0
+    limits = []
+    try:
+        yield (lambda: limits.append(_native.set_wait_limit(0))), (lambda: _native.set_wait_limit(limits[0]))
+    finally:
+        if limits:
+            _native.set_wait_limit(limits[0])
+        _native.device_errors(clear=True)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("rows,inputs,outputs", [(300, 64, 48), (9, 4, 3), (40, 9000, 136), (9000, 256, 1040)])
+def test_what_an_abandoned_product_leaves(no_waiting, cuda, dt, rows, inputs, outputs):
+    """A wait that ran out shows in the results, forward and backward, and in the device's flags; later calls are sound."""
+    on, off = no_waiting
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w, go = (torch.randn(*s, generator=g, device=cuda).to(dt).requires_grad_(i < 2)
+                for i, s in enumerate(((rows, inputs), (outputs, inputs), (rows, outputs))))
+    b = torch.zeros(outputs, device=cuda, dtype=dt, requires_grad=True)
+
+    def call():
+        return linear_act(x, w, b, activation="silu")
+
+    want = call()
+    grads = torch.autograd.grad(want, [x, w, b], go, retain_graph=True)
+    on()
+    out = call()
+    off()
+    assert out.isnan().all() and _native.device_errors(clear=True) == _native.DEVERR_WAIT_TIMEOUT
+    assert all(t.isnan().all() for t in torch.autograd.grad(out, [x, w, b], go))  # act'(z) is NaN too
+    on()
+    dx, dw, db = torch.autograd.grad(want, [x, w, b], go, retain_graph=True)
+    off()
+    assert dx.isnan().all() and dw.isnan().all() and torch.equal(db, grads[2])
+    assert _native.device_errors(clear=True) == _native.DEVERR_WAIT_TIMEOUT
+    again = call()
+    assert torch.equal(again, want)
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(again, [x, w, b], go), grads))
+    assert _native.device_errors(clear=True) == 0
+
+
+def test_wait_limits(cuda):
+    before = _native.set_wait_limit(7.5)
+    try:
+        assert before == 4 and _native.set_wait_limit(9) == 7.5
+        for bad in (-1, float("nan"), float("inf")):
+            with pytest.raises(ValueError):
+                _native.set_wait_limit(bad)
+        assert _native.set_wait_limit(before) == 9
+    finally:
+        _native.set_wait_limit(before)

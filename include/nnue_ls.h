@@ -109,7 +109,9 @@ int nnue_ls_linear_backward(const nnue_ls_linear *a, void *workspace, size_t wor
  *   h = norm(y) * pre_weight + pre_bias       (only with pre_weight)
  * x, f, y, h: [rows, width], contiguous.  norm(v) = (v - m) / sqrt(mean((v -
  * m)^2) + eps) with m = mean(v) for NNUE_LS_NORM_LAYER and 0 for
- * NNUE_LS_NORM_RMS.  1 <= width <= NNUE_LS_NORM_MAX_WIDTH. */
+ * NNUE_LS_NORM_RMS.  Squares are summed in fp32: a row whose sum passes its range
+ * (values from 1.8e19 / sqrt(width) up) becomes NaN.
+ * 1 <= width <= NNUE_LS_NORM_MAX_WIDTH. */
 #define NNUE_LS_NORM_RMS 0
 #define NNUE_LS_NORM_LAYER 1
 #define NNUE_LS_GATE_NONE 0
@@ -148,7 +150,7 @@ int nnue_ls_norm_backward(const nnue_ls_norm *a, void *workspace, size_t workspa
  * over the n rows that count: valid[b] != 0 (all rows when valid is null) and
  * some logit other than -inf.  A row that does not count, and a choice beyond
  * the row's logits above -inf, has index -1 and gate 0.  A NaN logit is never
- * chosen and makes its row's gates and the loss NaN.
+ * chosen and makes the gates of its row's choices and the loss NaN.
  * 1 <= k <= experts <= NNUE_LS_MAX_EXPERTS. */
 #define NNUE_LS_MAX_EXPERTS 1024
 

@@ -582,8 +582,8 @@ __host__ __device__ constexpr int norm_backward_threads(int v, bool both, bool m
 
 // BOTH: the call has f with its norm and the norm after it.  MORE: it may have
 // biases or a learned scale.  Without BOTH what is there is looked up.
-// What bounds the kernels on 16-bit rows is instruction issue (60-70% of the
-// slots at 16 to 32 warps an SM), so a thread takes eight columns:
+// The busiest unit on 16-bit rows is instruction issue (60-70% of its slots at 16
+// to 32 warps an SM), so a thread takes eight columns:
 // what a row costs besides its columns (addresses, copies, the exchange of sums)
 // is shared by eight instead of four.  65536 x 1040, row gate, rms norms:
 // forward fp32 184 us (90% of the HBM copy rate over its four arrays), bf16 120

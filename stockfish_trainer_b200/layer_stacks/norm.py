@@ -87,9 +87,11 @@ def block_norm(x: torch.Tensor, f: torch.Tensor | None = None, *, post_weight: t
     x's shape, in x's type); a shape that says both, such as ``[n]`` beside
     ``[n, n]``, is refused: give it as ``[n, 1]`` or ``[1, n]``.  With
     ``gate_activation="sigmoid"`` the gate goes through a sigmoid first.
-    ``residual_scale`` is a number or a learned ``[width]`` tensor.  The parameters share one type, x's or fp32.  Statistics and sums
-    are held in fp32, h is normalised from the unrounded y, and each output is
-    rounded once.  Differentiable once, in every tensor argument.
+    ``residual_scale`` is a number or a learned ``[width]`` tensor.  The
+    parameters share one type, x's or fp32.  Statistics and sums are held in
+    fp32 (a row whose squares sum past its range, with values from 1.8e19 /
+    sqrt(width) up, becomes NaN), h is normalised from the unrounded y, and each
+    output is rounded once.  Differentiable once, in every tensor argument.
     """
     check = _native.check_tensor
     gpu = check(x, "x")

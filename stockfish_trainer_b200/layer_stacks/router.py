@@ -82,8 +82,8 @@ def route(logits: torch.Tensor, k: int, *, valid: torch.Tensor | None = None, re
     if ``valid`` (bool ``[...]``, default all) says so and it has a logit other
     than -inf; an expert at -inf is closed to the row.  Rows that do not count,
     and choices beyond the open experts, have index -1 and gate 0, and get no
-    gradient.  A NaN logit is never chosen and makes its row's gates and the
-    loss NaN.  ``gates`` and ``balance_loss`` carry gradients to ``logits``;
+    gradient.  A NaN logit is never chosen and makes the gates of its row's
+    choices and the loss NaN.  ``gates`` and ``balance_loss`` carry gradients to ``logits``;
     the counts enter them as constants.  Probabilities, gates and sums are held
     in fp32.
     """

@@ -139,3 +139,14 @@ def test_sigmoid_gates_far_below_zero(cuda, width, gate):
     if gate == "row":
         want = want.sum(1)
     assert ((g.grad.double() - want).abs() <= 16 * 2.0**-23 * want).all(), float(((g.grad.double() - want).abs() / want).max())
+
+
+@pytest.mark.parametrize("width", [64, 61, 5000])
+def test_a_sum_of_squares_beyond_fp32_shows(cuda, width):
+    """Values below 1.8e19 / sqrt(width) are normalised; above that the row is NaN, and no other."""
+    for dt in (torch.float32, torch.bfloat16):
+        x = torch.ones(3, width, device=cuda, dtype=dt)
+        x[0] = 1e17
+        x[1] = 3e19
+        h = block_norm(x, pre_weight=torch.ones(width, device=cuda))[1]
+        assert h[1].isnan().all() and ((h[[0, 2]] - 1).abs() < 1e-2).all()
